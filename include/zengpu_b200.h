@@ -432,6 +432,53 @@ int zg_sgemm_f32_noalloc(int mode, int m, int n, int k, float alpha, const float
 int zg_fill_uniform_f32(float *x, uint64_t n, uint64_t seed, float lo, float hi, void *stream);
 int zg_fill_normal_f32(float *x, uint64_t n, uint64_t seed, void *stream);
 
+/* ---- AdamW over many tensors, and the gradient norm that clips it.  Beside
+ * saxpy / sscal (zengpu-blas/src/level1.rs:51-139); the reference has no
+ * optimiser.
+ *
+ * zg_adamw: one step t over `count` tensors in one launch (one for every 440
+ * of them), in place:
+ *     g' = s g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
+ *     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in f32, each operation rounded on its own.  Weights: F32, or BF16 / F16 with
+ * an f32 `master` (the sum lives there, the weight is its rounding) or without
+ * (master NULL: the sum is rounded to the weight's type).  Gradients: F32, BF16
+ * or F16.  state_bits 32: exp_avg and exp_avg_sq are f32 of n elements (m and
+ * v).  state_bits 8: they are n e4m3 codes each, of m and of sqrt(v), with one
+ * f32 scale for every ZG_ADAMW_BLOCK elements (the last block may be short);
+ * value = code * scale, all zeros is the start.  A block with a value that is
+ * not finite gets a NaN scale.
+ *     step_dev, lr_dev: device scalars that replace h->step and h->lr (NULL:
+ * the host's), read by the kernel, so that a captured step can be replayed with
+ * new ones.  grad_scale_dev: device scalar s (NULL: 1); when it is not finite
+ * the call changes nothing.  The tensors of a call must not overlap. */
+#define ZG_ADAMW_BLOCK 256
+typedef struct zg_adamw_tensor {
+    void *param;
+    const void *grad;
+    void *master;            /* f32, or NULL */
+    void *exp_avg;           /* f32, or e4m3 codes */
+    void *exp_avg_sq;        /* f32, or e4m3 codes of its root */
+    float *exp_avg_scale;    /* state_bits 8: ceil(n / 256) */
+    float *exp_avg_sq_scale; /* state_bits 8: ceil(n / 256) */
+    uint64_t n;
+} zg_adamw_tensor;
+typedef struct zg_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step; /* t, from 1 */
+} zg_adamw_hyper;
+int zg_adamw(uint32_t param_dtype, uint32_t grad_dtype, int state_bits, uint32_t count,
+             const zg_adamw_tensor *tensors, const zg_adamw_hyper *h, const int64_t *step_dev,
+             const float *lr_dev, const float *grad_scale_dev, void *stream);
+
+/* out[0] = the 2-norm over all gradients (64-bit sums in a fixed order), out[1]
+ * = min(1, max_norm / norm), the factor zg_adamw takes as grad_scale_dev; NaN
+ * when the norm is not finite.  `out`: two f32 on the device. */
+uint64_t zg_grad_norm_workspace_bytes(uint32_t count);
+int zg_grad_norm(uint32_t grad_dtype, uint32_t count, const void *const *grads,
+                 const uint64_t *sizes, double max_norm, float *out, void *workspace,
+                 uint64_t workspace_bytes, void *stream);
+
 /* Name of the main kernel zg_sgemm_f32 / zg_sgemm_packed launch for
  * (mode, m, n, k) on the current device ("" for an unknown mode or an empty
  * output), for reports and profiler filters.  The tensor-core modes take the

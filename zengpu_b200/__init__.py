@@ -10,7 +10,7 @@ Layers (all over libzengpu_b200.so, include/zengpu_b200.h):
              (ShardedGemm)
 """
 from .api import (  # noqa: F401
-    Backend, BindingMismatch, Blas, BufferPool, BufferUsage, CudaDevice, DeviceArray,
+    Activation, Backend, BindingMismatch, Blas, BufferPool, BufferUsage, CudaDevice, DeviceArray,
     DeviceLost, Dispatch, DType, ElementwiseKernels, GemmKernel, GemmMode, GpuError,
     InvalidUsage, KernelWait, Level1Kernels, MemoryUsage, MissingUsage, NoDevice,
     OutOfMemory, PipelineCreation, ShaderCompile, ShaderKind, StaleHandle, Submission,

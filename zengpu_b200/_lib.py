@@ -86,6 +86,30 @@ class CGemmKernel(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("param", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("master", C.c_void_p),
+        ("exp_avg", C.c_void_p),
+        ("exp_avg_sq", C.c_void_p),
+        ("exp_avg_scale", C.c_void_p),
+        ("exp_avg_sq_scale", C.c_void_p),
+        ("n", C.c_uint64),
+    ]
+
+
+class AdamWHyper(C.Structure):
+    _fields_ = [
+        ("lr", C.c_double),
+        ("beta1", C.c_double),
+        ("beta2", C.c_double),
+        ("eps", C.c_double),
+        ("weight_decay", C.c_double),
+        ("step", C.c_int64),
+    ]
+
+
 _vp = C.c_void_p
 _i = C.c_int
 _u32 = C.c_uint32
@@ -167,6 +191,11 @@ SIGNATURES: dict[str, tuple] = {
     "zg_sgemm_f32_noalloc": (_i, [_i, _i, _i, _i, _f, _fp, _fp, _fp, _fp, _i, _vp]),
     "zg_fill_uniform_f32": (_i, [_fp, _u64, _u64, _f, _f, _vp]),
     "zg_fill_normal_f32": (_i, [_fp, _u64, _u64, _vp]),
+    "zg_adamw": (_i, [_u32, _u32, _i, _u32, C.POINTER(AdamWTensor), C.POINTER(AdamWHyper), _vp,
+                      _vp, _vp, _vp]),
+    "zg_grad_norm_workspace_bytes": (_u64, [_u32]),
+    "zg_grad_norm": (_i, [_u32, _u32, C.POINTER(_vp), C.POINTER(_u64), C.c_double, _vp, _vp, _u64,
+                          _vp]),
     "zg_kernel_status": (_i, [C.POINTER(_u32)]),
     "zg_sgemm_kernel_name": (C.c_char_p, [_i, _i, _i, _i]),
     "zg_bchain_create": (_i, [_i, _i, _i, _i, C.POINTER(_vp), C.POINTER(C.c_uint8)]),

@@ -124,6 +124,14 @@ class GemmMode(enum.IntEnum):
     BF16X3 = 4
 
 
+class Activation(enum.IntEnum):
+    """Activation of the gated feed-forward block (ZG_ACT_*)."""
+    SILU = 0
+    GELU = 1       # with the error function
+    GELU_TANH = 2  # its tanh approximation
+    RELU = 3
+
+
 class ShaderKind(enum.IntEnum):
     CUBIN = 0
     PTX = 1

@@ -1,0 +1,588 @@
+// optimizer.cu - one AdamW step over many tensors at once, and the gradient
+// norm that clips it.  Beside Level-1 saxpy / sscal (elementwise.cu), the
+// in-place updates of zengpu-blas/src/level1.rs:51-139; the reference has no
+// optimiser.
+//
+// AdamW.  With s = *grad_scale (1 when absent) and step t, per element
+//     g' = s g
+//     m  = b1 m + (1 - b1) g'
+//     v  = b2 v + ((1 - b2) g') g'
+//     p  = p (1 - lr wd) - ((lr / (1 - b1^t)) m) / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// in f32, every operation rounded on its own in the order written, as the
+// other elementwise kernels here do: the result does not depend on which
+// vector or scalar path an element takes, nor on the launch.  Weights are
+// f32, or bf16 / f16 either with an f32 master that carries the sum (the
+// 16-bit weight is its rounding) or without one (the sum itself is rounded).
+//
+// Moments in 8 bits: a block of 256 consecutive elements of a tensor stores m
+// as e4m3 codes times one f32 scale, and r = sqrt(v) likewise (the root halves
+// the exponent range the code has to span).  scale = max|x| / 448, the largest
+// code for the largest value.  e4m3 rounds to 2^-4 relative, over 2^17.8 below
+// the block's maximum; smaller m becomes zero, but r > 0 is held at the
+// smallest code or more, so that no denominator collapses to eps.  The weight
+// is updated from m and r before they are rounded.  A block in which m or r is
+// not finite gets a NaN scale.
+//
+// All tensors of a call share one launch: the table of their pointers travels
+// in the kernel's parameters (no copy to the device, nothing that a captured
+// graph could find overwritten).  A CTA owns a chunk of one tensor, a warp a
+// 256-element block of it per turn, as two runs of 128 elements with four
+// neighbours per lane (16-byte loads of f32).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <vector>
+
+#include "zg_common.cuh"
+
+namespace zg {
+namespace {
+
+constexpr int kOptThreads = 256;
+constexpr int kBlockElems = ZG_ADAMW_BLOCK;  // per warp and turn, and per 8-bit scale
+constexpr int kTurnElems = kBlockElems * (kOptThreads / 32);
+static_assert(kBlockElems == 32 * 8, "a lane holds eight elements of a block");
+
+template <class T> struct Elem;
+template <> struct Elem<float> {
+    __device__ static float get(float x) { return x; }
+    __device__ static float put(float x) { return x; }
+};
+template <> struct Elem<__nv_bfloat16> {
+    __device__ static float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+    __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+template <> struct Elem<__half> {
+    __device__ static float get(__half x) { return __half2float(x); }
+    __device__ static __half put(float x) { return __float2half_rn(x); }
+};
+
+template <class T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+
+// Eight elements of the block at `x`: vector form for a whole, aligned block,
+// else one element at a time up to `left`.  Element (j, i) of lane l is
+// 128 j + 4 l + i in the vector form and 128 j + 32 i + l in the other.
+template <class T>
+__device__ __forceinline__ void load8(const T* x, bool vec, int lane, int64_t left, T (&out)[8]) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const Four<T> f = *reinterpret_cast<const Four<T>*>(x + 128 * j + 4 * lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[4 * j + i] = f.v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = 32 * i + lane;
+            out[i] = e < left ? x[e] : T(0.0f);
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* x, bool vec, int lane, int64_t left, const T (&in)[8]) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            Four<T> f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.v[i] = in[4 * j + i];
+            *reinterpret_cast<Four<T>*>(x + 128 * j + 4 * lane) = f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = 32 * i + lane;
+            if (e < left) x[e] = in[i];
+        }
+    }
+}
+
+struct Factors {
+    float b1, c1, b2, c2;  // beta and 1 - beta, each rounded from 64 bits
+    float step_size;       // lr / (1 - b1^t)
+    float root;            // 1 / sqrt(1 - b2^t)
+    float eps, decay;      // decay: 1 - lr wd
+};
+
+struct DeviceHyper {  // values a captured graph reads anew at each replay
+    const int64_t* step;
+    const float* lr;
+    const float* grad_scale;
+};
+
+// 1 - b^t without the cancellation that b^t near 1 would bring.
+__host__ __device__ inline double bias_correction(double beta, double t) {
+    return beta > 0.0 ? -expm1(t * log(beta)) : 1.0;
+}
+__host__ __device__ inline void schedule(Factors& f, double lr, double beta1, double beta2,
+                                         double wd, double t) {
+    f.step_size = static_cast<float>(lr / bias_correction(beta1, t));
+    f.root = static_cast<float>(1.0 / sqrt(bias_correction(beta2, t)));
+    f.decay = static_cast<float>(1.0 - lr * wd);
+}
+
+template <int CAP, class Tensor>
+struct Table {
+    Tensor t[CAP];
+    uint32_t first[CAP + 1];  // first chunk of tensor i; first[count] is the number of chunks
+    int count;
+};
+
+// The tensor that chunk c belongs to: the last one whose first chunk is <= c.
+template <int CAP, class Tensor>
+__device__ __forceinline__ int tensor_of(const Table<CAP, Tensor>& tab, uint32_t c) {
+    int lo = 0, hi = tab.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tab.first[mid] <= c) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+
+// The scale of a block whose largest magnitude is `top` (finite), and its inverse.
+__device__ __forceinline__ float block_scale(float top, float& inv) {
+    if (!(top > 0.0f)) {
+        inv = 0.0f;
+        return 0.0f;
+    }
+    const float s = fmaxf(__fmul_rn(top, 1.0f / 448.0f), 0x1p-126f);
+    inv = __frcp_rn(s);
+    return s;
+}
+
+struct E4M3 {
+    __device__ static float get(uint8_t c) {
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+    }
+    __device__ static uint8_t put(float x) {
+        return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+    }
+};
+
+// Stores eight f32 of a block as codes with one scale; `floor_code`: values
+// above zero keep at least the smallest code.
+__device__ __forceinline__ void store_8bit(uint8_t* codes, float* scale, bool vec, int lane,
+                                           int64_t left, const float (&x)[8], float floor_code) {
+    float top = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        top = fmaxf(top, fabsf(x[i]));
+        finite = finite && isfinite(x[i]);
+    }
+    top = warp_max(top);
+    finite = __all_sync(0xffffffffu, finite);
+    float inv, s = block_scale(top, inv);
+    uint8_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float y = __fmul_rn(x[i], inv);
+        if (x[i] > 0.0f) y = fmaxf(y, floor_code);
+        q[i] = E4M3::put(y);
+    }
+    if (!finite) s = __int_as_float(0x7fc00000);
+    if (lane == 0) *scale = s;
+    store8<uint8_t>(codes, vec, lane, left, q);
+}
+
+// What bounds it: HBM.  f32 weights, gradients and moments move 28 bytes per
+// element, 16-bit weights with a master and 8-bit moments 16.1.
+template <class P, class G, int BITS, int CAP>
+__global__ void __launch_bounds__(kOptThreads)
+    adamw_kernel(const __grid_constant__ Table<CAP, zg_adamw_tensor> tab, int64_t chunk, Factors f,
+                 const zg_adamw_hyper hyper, const DeviceHyper dev) {
+    const int i = tensor_of(tab, blockIdx.x);
+    const zg_adamw_tensor& t = tab.t[i];
+    const int64_t begin = static_cast<int64_t>(blockIdx.x - tab.first[i]) * chunk;
+    const int64_t end = min(static_cast<int64_t>(t.n), begin + chunk);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    float gscale = 1.0f;
+    if (dev.grad_scale) {
+        gscale = *dev.grad_scale;
+        if (!isfinite(gscale)) return;  // the step is skipped: nothing changes
+    }
+    if (dev.step || dev.lr) {
+        __shared__ Factors shared;
+        if (threadIdx.x == 0) {
+            shared = f;
+            schedule(shared, dev.lr ? *dev.lr : hyper.lr, hyper.beta1, hyper.beta2,
+                     hyper.weight_decay,
+                     static_cast<double>(dev.step ? *dev.step : hyper.step));
+        }
+        __syncthreads();
+        f = shared;
+    }
+
+    P* p = static_cast<P*>(t.param);
+    const G* g = static_cast<const G*>(t.grad);
+    float* master = static_cast<float*>(t.master);
+    const bool aligned =
+        ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(P) - 1)) |
+         (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) |
+         (reinterpret_cast<uintptr_t>(master) & 15) |
+         ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) &
+          (BITS == 8 ? 3 : 15))) == 0;
+
+    for (int64_t b = begin + warp * kBlockElems; b < end; b += kTurnElems) {
+        const int64_t left = end - b;
+        const bool vec = aligned && left >= kBlockElems;
+        P pv[8];
+        G gv[8];
+        float w[8], m[8], v[8];
+        load8<G>(g + b, vec, lane, left, gv);
+        if (master) {
+            load8<float>(master + b, vec, lane, left, w);
+        } else {
+            load8<P>(p + b, vec, lane, left, pv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = Elem<P>::get(pv[e]);
+        }
+        if (BITS == 32) {
+            load8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, m);
+            load8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, v);
+        } else {
+            uint8_t mc[8], vc[8];
+            load8<uint8_t>(static_cast<uint8_t*>(t.exp_avg) + b, vec, lane, left, mc);
+            load8<uint8_t>(static_cast<uint8_t*>(t.exp_avg_sq) + b, vec, lane, left, vc);
+            const float ms = t.exp_avg_scale[b / kBlockElems];
+            const float vs = t.exp_avg_sq_scale[b / kBlockElems];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = __fmul_rn(E4M3::get(mc[e]), ms);
+                const float r = __fmul_rn(E4M3::get(vc[e]), vs);
+                v[e] = __fmul_rn(r, r);
+            }
+        }
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float ge = __fmul_rn(Elem<G>::get(gv[e]), gscale);
+            m[e] = __fadd_rn(__fmul_rn(m[e], f.b1), __fmul_rn(ge, f.c1));
+            v[e] = __fadd_rn(__fmul_rn(v[e], f.b2), __fmul_rn(__fmul_rn(ge, f.c2), ge));
+            r[e] = __fsqrt_rn(v[e]);
+            const float den = __fadd_rn(__fmul_rn(r[e], f.root), f.eps);
+            w[e] = __fsub_rn(__fmul_rn(w[e], f.decay),
+                             __fdiv_rn(__fmul_rn(m[e], f.step_size), den));
+            pv[e] = Elem<P>::put(w[e]);
+        }
+        store8<P>(p + b, vec, lane, left, pv);
+        if (master) store8<float>(master + b, vec, lane, left, w);
+        if (BITS == 32) {
+            store8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, m);
+            store8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, v);
+        } else {
+            // lanes past a tensor's end hold zeros, which change no block's maximum,
+            // except that 0 / (0 + eps) may be NaN: only w sees that, and is not stored
+            store_8bit(static_cast<uint8_t*>(t.exp_avg) + b, t.exp_avg_scale + b / kBlockElems,
+                       vec, lane, left, m, -448.0f);
+            store_8bit(static_cast<uint8_t*>(t.exp_avg_sq) + b,
+                       t.exp_avg_sq_scale + b / kBlockElems, vec, lane, left, r, 0x1p-9f);
+        }
+    }
+}
+
+// ---- gradient norm ---------------------------------------------------------------
+// norm = sqrt(sum g^2) in 64 bits throughout (a square of f32 has at most 48
+// bits, so only the sums round, and no f32 gradient overflows), summed in a fixed
+// order: per thread over its elements, per CTA by a tree, then one CTA over the
+// partial sums.  Reads each gradient once: HBM bound.
+struct NormTensor {
+    const void* g;
+    uint64_t n;
+};
+
+__device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == 0) part[warp] = x;
+    __syncthreads();
+    x = warp == 0 && lane < static_cast<int>(blockDim.x >> 5) ? part[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;  // complete in warp 0
+}
+
+template <class G, int CAP>
+__global__ void __launch_bounds__(kOptThreads)
+    norm_partial_kernel(const __grid_constant__ Table<CAP, NormTensor> tab, int64_t chunk,
+                        double* partial) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t chunks = tab.first[tab.count];
+    double sum = 0.0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int i = tensor_of(tab, c);
+        const G* g = static_cast<const G*>(tab.t[i].g);
+        const int64_t begin = static_cast<int64_t>(c - tab.first[i]) * chunk;
+        const int64_t end = min(static_cast<int64_t>(tab.t[i].n), begin + chunk);
+        const bool aligned = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
+        for (int64_t b = begin + warp * kBlockElems; b < end; b += kTurnElems) {
+            G gv[8];
+            load8<G>(g + b, aligned && end - b >= kBlockElems, lane, end - b, gv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double x = static_cast<double>(Elem<G>::get(gv[e]));
+                sum = fma(x, x, sum);
+            }
+        }
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+// out[0] = norm, out[1] = min(1, max_norm / norm); NaN when the norm is not finite.
+__global__ void __launch_bounds__(1024)
+    norm_final_kernel(const double* partial, int count, double max_norm, float* out) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < count; i += 1024) sum += partial[i];
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(sum);
+        out[0] = static_cast<float>(norm);
+        out[1] = !isfinite(norm) ? __int_as_float(0x7fc00000)
+                                 : norm > max_norm ? static_cast<float>(max_norm / norm) : 1.0f;
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------
+int sm_count() {
+    static thread_local int cached_dev = -1, cached = 0;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev != cached_dev) {
+        cudaDeviceGetAttribute(&cached, cudaDevAttrMultiProcessorCount, dev);
+        if (cached <= 0) cached = 148;
+        cached_dev = dev;
+    }
+    return cached;
+}
+
+// Tables of two sizes: a launch copies its whole parameter block, so a call of a
+// few tensors does not carry the largest one (32764 bytes of parameters at most).
+constexpr int kSmallTable = 32;
+constexpr int kLargeTable = 440;
+
+// Elements per chunk: whole turns of a CTA, about four chunks for each of the
+// 8 CTAs an SM holds when there is that much work, else as little as one turn.
+int64_t chunk_elems(uint64_t total) {
+    const uint64_t want = total / (static_cast<uint64_t>(sm_count()) * 32);
+    const uint64_t turns = std::min<uint64_t>(std::max<uint64_t>(want / kTurnElems, 1), 8);
+    return static_cast<int64_t>(turns * kTurnElems);
+}
+
+template <int CAP, class Tensor>
+void fill(Table<CAP, Tensor>& tab, const Tensor* t, int count, int64_t chunk) {
+    uint32_t chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        tab.t[i] = t[i];
+        tab.first[i] = chunks;
+        chunks += static_cast<uint32_t>((t[i].n + chunk - 1) / chunk);
+    }
+    tab.first[count] = chunks;
+    tab.count = count;
+}
+
+struct AdamCall {
+    Factors f;
+    zg_adamw_hyper hyper;
+    DeviceHyper dev;
+    int64_t chunk;
+    cudaStream_t stream;
+};
+
+template <class P, class G, int BITS, int CAP>
+int launch_adamw_table(const zg_adamw_tensor* t, int count, const AdamCall& c) {
+    static_assert(sizeof(Table<CAP, zg_adamw_tensor>) + 256 <= 32764, "kernel parameters");
+    Table<CAP, zg_adamw_tensor> tab;
+    fill(tab, t, count, c.chunk);
+    adamw_kernel<P, G, BITS, CAP><<<tab.first[count], kOptThreads, 0, c.stream>>>(
+        tab, c.chunk, c.f, c.hyper, c.dev);
+    return cuda_status(cudaGetLastError(), "zg_adamw");
+}
+
+template <class P, class G, int BITS>
+int launch_adamw(const std::vector<zg_adamw_tensor>& t, const AdamCall& c) {
+    for (size_t at = 0; at < t.size(); at += kLargeTable) {
+        const int n = static_cast<int>(std::min<size_t>(t.size() - at, kLargeTable));
+        const int rc = n <= kSmallTable
+                           ? launch_adamw_table<P, G, BITS, kSmallTable>(t.data() + at, n, c)
+                           : launch_adamw_table<P, G, BITS, kLargeTable>(t.data() + at, n, c);
+        if (rc) return rc;
+    }
+    return ZG_OK;
+}
+
+template <class P, class G>
+int launch_adamw_bits(int bits, const std::vector<zg_adamw_tensor>& t, const AdamCall& c) {
+    return bits == 8 ? launch_adamw<P, G, 8>(t, c) : launch_adamw<P, G, 32>(t, c);
+}
+
+template <class P>
+int launch_adamw_grad(uint32_t grad, int bits, const std::vector<zg_adamw_tensor>& t,
+                      const AdamCall& c) {
+    switch (grad) {
+        case ZG_DTYPE_F32: return launch_adamw_bits<P, float>(bits, t, c);
+        case ZG_DTYPE_BF16: return launch_adamw_bits<P, __nv_bfloat16>(bits, t, c);
+        default: return launch_adamw_bits<P, __half>(bits, t, c);
+    }
+}
+
+bool float_dtype(uint32_t d) {
+    return d == ZG_DTYPE_F32 || d == ZG_DTYPE_F16 || d == ZG_DTYPE_BF16;
+}
+
+uint64_t elem_bytes(uint32_t d) { return d == ZG_DTYPE_F32 ? 4 : 2; }
+bool misaligned(const void* p, uint64_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+template <int CAP, class G>
+int launch_norm_table(const NormTensor* t, int count, int64_t chunk, int grid, double* partial,
+                      cudaStream_t s) {
+    Table<CAP, NormTensor> tab;
+    fill(tab, t, count, chunk);
+    norm_partial_kernel<G, CAP><<<grid, kOptThreads, 0, s>>>(tab, chunk, partial);
+    return cuda_status(cudaGetLastError(), "zg_grad_norm");
+}
+
+template <class G>
+int launch_norm(const NormTensor* t, int count, int64_t chunk, int grid, double* partial,
+                cudaStream_t s) {
+    return count <= kSmallTable
+               ? launch_norm_table<kSmallTable, G>(t, count, chunk, grid, partial, s)
+               : launch_norm_table<kLargeTable, G>(t, count, chunk, grid, partial, s);
+}
+
+// CTAs of one partial launch: at most 8 per SM of the largest part sold (so the
+// workspace does not depend on the device).
+constexpr int kNormGridMax = 8 * 160;
+
+}  // namespace
+}  // namespace zg
+
+using namespace zg;
+
+extern "C" int zg_adamw(uint32_t param_dtype, uint32_t grad_dtype, int state_bits,
+                        uint32_t count, const zg_adamw_tensor* tensors, const zg_adamw_hyper* h,
+                        const int64_t* step_dev, const float* lr_dev, const float* grad_scale_dev,
+                        void* stream) {
+    if (!float_dtype(param_dtype) || !float_dtype(grad_dtype))
+        return set_error(ZG_ERR_DISPATCH, "adamw: weights and gradients are f32, bf16 or f16, got dtypes %u and %u",
+                         param_dtype, grad_dtype);
+    if (state_bits != 32 && state_bits != 8)
+        return set_error(ZG_ERR_DISPATCH, "adamw: moments have 32 or 8 bits, got %d", state_bits);
+    if (!h || (count && !tensors)) return set_error(ZG_ERR_DISPATCH, "adamw: null argument");
+    if (!(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0))
+        return set_error(ZG_ERR_DISPATCH, "adamw: betas must be in [0, 1), got %g and %g", h->beta1,
+                         h->beta2);
+    if (!(h->eps >= 0.0) || !std::isfinite(h->eps) || !std::isfinite(h->weight_decay) ||
+        (!lr_dev && !std::isfinite(h->lr)))
+        return set_error(ZG_ERR_DISPATCH, "adamw: lr, eps and weight_decay must be finite, eps >= 0");
+    if (!step_dev && h->step < 1)
+        return set_error(ZG_ERR_DISPATCH, "adamw: steps count from 1, got %lld", (long long)h->step);
+    std::vector<zg_adamw_tensor> used;
+    used.reserve(count);
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        const zg_adamw_tensor& t = tensors[i];
+        if (t.n == 0) continue;
+        if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
+            (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
+            return set_error(ZG_ERR_DISPATCH, "adamw: null pointer in tensor %u of %llu elements", i,
+                             (unsigned long long)t.n);
+        if (t.master && param_dtype == ZG_DTYPE_F32)
+            return set_error(ZG_ERR_DISPATCH, "adamw: f32 weights take no master (tensor %u)", i);
+        if (t.n >= 1ull << 40)
+            return set_error(ZG_ERR_DISPATCH, "adamw: tensor %u has %llu elements", i,
+                             (unsigned long long)t.n);
+        if (misaligned(t.param, elem_bytes(param_dtype)) || misaligned(t.grad, elem_bytes(grad_dtype)) ||
+            misaligned(t.master, 4) || misaligned(t.exp_avg_scale, 4) ||
+            misaligned(t.exp_avg_sq_scale, 4) ||
+            (state_bits == 32 && (misaligned(t.exp_avg, 4) || misaligned(t.exp_avg_sq, 4))))
+            return set_error(ZG_ERR_DISPATCH, "adamw: a pointer of tensor %u is not aligned to its type", i);
+        used.push_back(t);
+        total += t.n;
+    }
+    if (used.empty()) return ZG_OK;
+    AdamCall c;
+    c.hyper = *h;
+    c.dev = {step_dev, lr_dev, grad_scale_dev};
+    c.f.b1 = static_cast<float>(h->beta1);
+    c.f.c1 = static_cast<float>(1.0 - h->beta1);
+    c.f.b2 = static_cast<float>(h->beta2);
+    c.f.c2 = static_cast<float>(1.0 - h->beta2);
+    c.f.eps = static_cast<float>(h->eps);
+    schedule(c.f, lr_dev ? 0.0 : h->lr, h->beta1, h->beta2, h->weight_decay,
+             step_dev ? 1.0 : static_cast<double>(h->step));
+    c.chunk = chunk_elems(total);
+    c.stream = static_cast<cudaStream_t>(stream);
+    switch (param_dtype) {
+        case ZG_DTYPE_F32: return launch_adamw_grad<float>(grad_dtype, state_bits, used, c);
+        case ZG_DTYPE_BF16: return launch_adamw_grad<__nv_bfloat16>(grad_dtype, state_bits, used, c);
+        default: return launch_adamw_grad<__half>(grad_dtype, state_bits, used, c);
+    }
+}
+
+extern "C" uint64_t zg_grad_norm_workspace_bytes(uint32_t count) {
+    const uint64_t launches = (static_cast<uint64_t>(count) + kLargeTable - 1) / kLargeTable;
+    return launches * kNormGridMax * sizeof(double);
+}
+
+extern "C" int zg_grad_norm(uint32_t grad_dtype, uint32_t count, const void* const* grads,
+                            const uint64_t* sizes, double max_norm, float* out, void* workspace,
+                            uint64_t workspace_bytes, void* stream) {
+    if (!float_dtype(grad_dtype))
+        return set_error(ZG_ERR_DISPATCH, "grad_norm: gradients are f32, bf16 or f16, got dtype %u",
+                         grad_dtype);
+    if (!out || (count && (!grads || !sizes)))
+        return set_error(ZG_ERR_DISPATCH, "grad_norm: null argument");
+    if (!(max_norm > 0.0))
+        return set_error(ZG_ERR_DISPATCH, "grad_norm: max_norm must be above zero, got %g", max_norm);
+    const uint64_t need = zg_grad_norm_workspace_bytes(count);
+    if (need && (!workspace || workspace_bytes < need || misaligned(workspace, 8)))
+        return set_error(ZG_ERR_DISPATCH,
+                         "grad_norm: an 8-byte aligned workspace of %llu bytes is needed, got %llu",
+                         (unsigned long long)need, (unsigned long long)workspace_bytes);
+    std::vector<NormTensor> used;
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (sizes[i] == 0) continue;
+        if (!grads[i] || misaligned(grads[i], elem_bytes(grad_dtype)) || sizes[i] >= 1ull << 40)
+            return set_error(ZG_ERR_DISPATCH, "grad_norm: bad pointer or size in tensor %u", i);
+        used.push_back({grads[i], sizes[i]});
+        total += sizes[i];
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    double* partial = static_cast<double*>(workspace);
+    const int64_t chunk = chunk_elems(total);
+    int parts = 0;
+    for (size_t at = 0; at < used.size(); at += kLargeTable) {
+        const int n = static_cast<int>(std::min<size_t>(used.size() - at, kLargeTable));
+        uint64_t chunks = 0;
+        for (int i = 0; i < n; ++i) chunks += (used[at + i].n + chunk - 1) / chunk;
+        const int grid = static_cast<int>(std::min<uint64_t>(chunks, std::min(8 * sm_count(), kNormGridMax)));
+        const NormTensor* t = used.data() + at;
+        int rc;
+        switch (grad_dtype) {
+            case ZG_DTYPE_F32: rc = launch_norm<float>(t, n, chunk, grid, partial + parts, s); break;
+            case ZG_DTYPE_BF16: rc = launch_norm<__nv_bfloat16>(t, n, chunk, grid, partial + parts, s); break;
+            default: rc = launch_norm<__half>(t, n, chunk, grid, partial + parts, s); break;
+        }
+        if (rc) return rc;
+        parts += grid;
+    }
+    norm_final_kernel<<<1, 1024, 0, s>>>(partial, parts, max_norm, out);
+    return cuda_status(cudaGetLastError(), "zg_grad_norm");
+}

@@ -7,12 +7,16 @@ is this library's own sm_100a code.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+from typing import Sequence
 
 import torch
 
 from . import _lib as L
-from .api import GemmMode, check
+from .api import DType, GemmMode, check
+
+ADAMW_BLOCK = 256  # elements that share a scale in 8-bit moments (ZG_ADAMW_BLOCK)
 
 # One scratch tensor per (device, stream): GEMMs issued on different streams
 # may overlap, and each stream reuses its own scratch in stream order.
@@ -208,3 +212,148 @@ def sgemm_packed(pa: Packed, pb: Packed, c: torch.Tensor | None = None, alpha: f
                                    bias.data_ptr() if bias is not None else None,
                                    1 if relu else 0, _stream(c)))
     return c
+
+
+# ---- AdamW over many tensors, gradient norm (zg_adamw, zg_grad_norm) -------------------
+_FLOATS = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.Bf16}
+
+
+def _on(device: torch.device):
+    """Makes `device` the current one for a call (free when it already is)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() \
+        else torch.cuda.device(device)
+
+
+def _same(name: str, tensors: Sequence[torch.Tensor], like: Sequence[int],
+          device: torch.device, dtypes: Sequence[torch.dtype]) -> None:
+    """Checks a list of contiguous CUDA tensors: one dtype out of `dtypes`, `like` elements each."""
+    if len(tensors) != len(like):
+        raise ValueError(f"{name}: {len(tensors)} tensors, expected {len(like)}")
+    for t, n in zip(tensors, like):
+        if t.device != device or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous tensors on {device}")
+        if t.dtype not in dtypes or t.dtype != tensors[0].dtype:
+            raise ValueError(f"{name}: unexpected dtype {t.dtype}")
+        if t.numel() != n:
+            raise ValueError(f"{name}: {t.numel()} elements, expected {n}")
+
+
+def _device_scalar(name: str, t: torch.Tensor | None, dtype: torch.dtype,
+                   device: torch.device) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != 1 or t.device != device:
+        raise ValueError(f"{name}: expected one {dtype} on {device}")
+    return t.data_ptr()
+
+
+class AdamW:
+    """AdamW over many tensors, one launch a step (zg_adamw): in place on the
+    weights, their moments and, for 16-bit weights, their f32 `master` copies.
+
+    params: f32, bf16 or f16 CUDA tensors of one dtype; grads: as many, of one
+    dtype, the buffers every step reads; state_bits: 32 (f32 moments) or 8 (e4m3
+    codes of m and of sqrt(v), with an f32 scale for each 256 elements).
+    `state` takes the moments a program already has, as lists by name; by
+    default they start at zero.  All tensors are contiguous and none overlaps
+    another.  The object keeps them alive; a step runs on the current stream."""
+
+    def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+                 state_bits: int = 32, master: Sequence[torch.Tensor] | None = None,
+                 state: dict[str, Sequence[torch.Tensor]] | None = None):
+        if not params:
+            raise ValueError("AdamW: no tensors")
+        if state_bits not in (32, 8):
+            raise ValueError(f"AdamW: state_bits is 32 or 8, got {state_bits}")
+        device = params[0].device
+        if device.type != "cuda":
+            raise ValueError("AdamW: expected CUDA tensors")
+        sizes = [p.numel() for p in params]
+        blocks = [-(-n // ADAMW_BLOCK) for n in sizes]
+        _same("AdamW params", params, sizes, device, tuple(_FLOATS))
+        _same("AdamW grads", grads, sizes, device, tuple(_FLOATS))
+        if master is not None:
+            if params[0].dtype == torch.float32:
+                raise ValueError("AdamW: f32 weights take no master")
+            _same("AdamW master", master, sizes, device, (torch.float32,))
+        moments = {"exp_avg": sizes, "exp_avg_sq": sizes}
+        if state_bits == 8:
+            moments |= {"exp_avg_scale": blocks, "exp_avg_sq_scale": blocks}
+        if state is not None and set(state) != set(moments):
+            raise ValueError(f"AdamW: state has {sorted(state)}, expected {sorted(moments)}")
+        self.state: dict[str, list[torch.Tensor]] = {}
+        for name, counts in moments.items():
+            codes = state_bits == 8 and not name.endswith("scale")
+            dtype = torch.float8_e4m3fn if codes else torch.float32
+            if state is None:
+                self.state[name] = [torch.zeros(n, dtype=torch.uint8 if codes else dtype,
+                                                device=device).view(dtype) for n in counts]
+            else:
+                _same(f"AdamW {name}", state[name], counts, device, (dtype,))
+                self.state[name] = list(state[name])
+        self.params, self.grads, self.state_bits = list(params), list(grads), state_bits
+        self.master = list(master) if master is not None else None
+        written = [self.params, self.master or [], *self.state.values()]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), kind)
+                       for kind, ts in ((1, sum(written, [])), (0, self.grads))
+                       for t in ts if t.numel())
+        end, kind = 0, 0
+        for a, b, k in spans:
+            if a < end and (k or kind):  # two gradients may be the same memory
+                raise ValueError("AdamW: tensors overlap")
+            end, kind = (b, k) if b >= end else (end, kind | k)
+        self._device = device
+        self._table = (L.AdamWTensor * len(params))()
+        for i, row in enumerate(self._table):
+            row.param, row.grad, row.n = params[i].data_ptr(), grads[i].data_ptr(), sizes[i]
+            row.master = self.master[i].data_ptr() if self.master else None
+            for name, ts in self.state.items():
+                setattr(row, name, ts[i].data_ptr())
+
+    def step(self, step: int | torch.Tensor, lr: float | torch.Tensor = 1e-3, beta1: float = 0.9,
+             beta2: float = 0.999, eps: float = 1e-8, weight_decay: float = 0.01,
+             grad_scale: torch.Tensor | None = None) -> None:
+        """Step number `step` (from 1).  `step` (int64) and `lr` (float32) may be
+        device scalars, which a captured step reads anew at each replay.
+        grad_scale: a float32 device scalar the gradients are multiplied by, as
+        GradNorm gives it; when it is not finite the step changes nothing."""
+        device = self._device
+        step_dev = _device_scalar("AdamW step", step, torch.int64, device) \
+            if isinstance(step, torch.Tensor) else None
+        lr_dev = _device_scalar("AdamW lr", lr, torch.float32, device) \
+            if isinstance(lr, torch.Tensor) else None
+        hyper = L.AdamWHyper(0.0 if lr_dev else lr, beta1, beta2, eps, weight_decay,
+                             0 if step_dev else int(step))
+        with _on(device):
+            check(L.load().zg_adamw(
+                _FLOATS[self.params[0].dtype], _FLOATS[self.grads[0].dtype], self.state_bits,
+                len(self._table), self._table, C.byref(hyper), step_dev, lr_dev,
+                _device_scalar("AdamW grad_scale", grad_scale, torch.float32, device),
+                _stream(self.params[0])))
+
+
+class GradNorm:
+    """The 2-norm over many gradients (zg_grad_norm), and the factor that clips
+    them.  grads: contiguous CUDA tensors of one dtype (f32, bf16 or f16), read
+    anew by every call."""
+
+    def __init__(self, grads: Sequence[torch.Tensor]):
+        if not grads or grads[0].device.type != "cuda":
+            raise ValueError("GradNorm: expected CUDA tensors")
+        self._device = grads[0].device
+        _same("GradNorm", grads, [g.numel() for g in grads], self._device, tuple(_FLOATS))
+        self.grads = list(grads)
+        self._ptrs = (C.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
+        self._sizes = (C.c_uint64 * len(grads))(*[g.numel() for g in grads])
+        self._ws_bytes = int(L.load().zg_grad_norm_workspace_bytes(len(grads)))
+
+    def clip_scale(self, max_norm: float) -> torch.Tensor:
+        """[norm, min(1, max_norm / norm)] as two f32 on the device; the factor is
+        NaN when the norm is not finite.  out[1:] is AdamW.step's grad_scale."""
+        with _on(self._device):
+            out = torch.empty(2, dtype=torch.float32, device=self._device)
+            ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self._device)
+            check(L.load().zg_grad_norm(_FLOATS[self.grads[0].dtype], len(self.grads), self._ptrs,
+                                        self._sizes, float(max_norm), out.data_ptr(),
+                                        ws.data_ptr(), self._ws_bytes, _stream(out)))
+        return out

@@ -432,6 +432,40 @@ int zg_sgemm_f32_noalloc(int mode, int m, int n, int k, float alpha, const float
 int zg_fill_uniform_f32(float *x, uint64_t n, uint64_t seed, float lo, float hi, void *stream);
 int zg_fill_normal_f32(float *x, uint64_t n, uint64_t seed, void *stream);
 
+/* ---- Gated feed-forward block and its backward pass.  Beside the fused GEMM +
+ * bias + ReLU; the reference has neither a gated layer nor a backward pass.
+ *
+ *   zg_gated_ff           y = (act(x w_gate) * (x w_up)) w_down
+ *   zg_gated_ff_backward  dx, dw_gate, dw_up, dw_down for dy, the gradient of y
+ *
+ * x [m, k], w_gate and w_up [k, f], w_down [f, d], y and dy [m, d]; gradients have
+ * their tensors' shapes.  All row-major and contiguous, of one dtype: F32, BF16
+ * or F16, 16-byte aligned.  Sums are f32.  BF16 and F16 run on the tensor cores
+ * as they are (mode is not read); h = act(x w_gate) * (x w_up), and in the
+ * backward pass the gradients of the two products, are rounded once to the
+ * dtype, as operands of the next product.  F32 runs in `mode` (ZG_GEMM_*), with
+ * f32 throughout.
+ *     pre_gate, pre_up: f32 [m, f], written by the forward pass when both are
+ * given (x w_gate and x w_up before the activation), read by the backward pass.
+ *     workspace: zg_gated_ff_workspace_bytes(...), 256-byte aligned, not shared by
+ * calls that may overlap.  m = 0 computes nothing (the weights' gradients are
+ * zero); k, f, d are at least 1.  Outputs must not overlap inputs. */
+#define ZG_ACT_SILU 0      /* g / (1 + e^-g) */
+#define ZG_ACT_GELU 1      /* g Phi(g) */
+#define ZG_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
+#define ZG_ACT_RELU 3      /* as zg_relu_f32; its slope is 0 where it returns 0 */
+uint64_t zg_gated_ff_workspace_bytes(uint32_t dtype, int mode, int m, int k, int f, int d,
+                                     int backward);
+int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int f, int d, const void *x,
+                const void *w_gate, const void *w_up, const void *w_down, void *y,
+                float *pre_gate, float *pre_up, void *workspace, uint64_t workspace_bytes,
+                void *stream);
+int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
+                         const void *dy, const void *x, const void *w_gate, const void *w_up,
+                         const void *w_down, const float *pre_gate, const float *pre_up, void *dx,
+                         void *dw_gate, void *dw_up, void *dw_down, void *workspace,
+                         uint64_t workspace_bytes, void *stream);
+
 /* ---- AdamW over many tensors, and the gradient norm that clips it.  Beside
  * saxpy / sscal (zengpu-blas/src/level1.rs:51-139); the reference has no
  * optimiser.

@@ -191,6 +191,11 @@ SIGNATURES: dict[str, tuple] = {
     "zg_sgemm_f32_noalloc": (_i, [_i, _i, _i, _i, _f, _fp, _fp, _fp, _fp, _i, _vp]),
     "zg_fill_uniform_f32": (_i, [_fp, _u64, _u64, _f, _f, _vp]),
     "zg_fill_normal_f32": (_i, [_fp, _u64, _u64, _vp]),
+    "zg_gated_ff_workspace_bytes": (_u64, [_u32, _i, _i, _i, _i, _i, _i]),
+    "zg_gated_ff": (_i, [_u32, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                         _u64, _vp]),
+    "zg_gated_ff_backward": (_i, [_u32, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
     "zg_adamw": (_i, [_u32, _u32, _i, _u32, C.POINTER(AdamWTensor), C.POINTER(AdamWHyper), _vp,
                       _vp, _vp, _vp]),
     "zg_grad_norm_workspace_bytes": (_u64, [_u32]),

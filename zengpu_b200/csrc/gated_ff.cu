@@ -1,0 +1,290 @@
+// gated_ff.cu - the gated feed-forward block y = (act(x Wg) * (x Wu)) Wd and its
+// backward pass (formulas and roundings: gated_ff.cuh), beside the fused GEMM +
+// bias + ReLU.  The reference has no gated layer and no backward pass; its
+// op_graph_lower chain (examples/op_graph_lower.rs:39-68) is the ungated,
+// forward-only form.
+#include <algorithm>
+#include <cstdint>
+#include <initializer_list>
+
+#include "gated_ff.cuh"
+
+namespace zg {
+namespace {
+
+// ---- CUDA-core product ------------------------------------------------------------
+// 64 x 64 of D per CTA, 4 x 4 per thread (twice for the gated pair), operands
+// through shared memory 16 of the sum at a time.  f32 throughout.
+constexpr int kTile = 64, kStep = 16;
+
+template <class T>
+__device__ __forceinline__ void load_panel(float (&sh)[kStep][kTile + 4], const FfOperand& o,
+                                           int rows, int r0, int k, int i0) {
+    // the thread order follows the operand's contiguous direction
+    for (int e = threadIdx.x; e < kTile * kStep; e += 256) {
+        const int r = o.mn ? e % kTile : e / kStep, i = o.mn ? e / kTile : e % kStep;
+        float v = 0.0f;
+        if (r0 + r < rows && i0 + i < k)
+            v = FfElem<T>::get(static_cast<const T*>(
+                o.p)[o.mn ? (i0 + i) * o.ld + r0 + r : (r0 + r) * o.ld + i0 + i]);
+        sh[i][r] = v;
+    }
+}
+
+template <class T, int EPI, int ACT>
+__global__ void __launch_bounds__(256) ff_simt_kernel(const FfProduct p) {
+    __shared__ float sa[kStep][kTile + 4], sb[2][kStep][kTile + 4];
+    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float acc[2][4][4] = {};
+    for (int seg = 0; seg < (EPI == kFfStore ? 2 : 1); ++seg) {
+        for (int i0 = 0; i0 < p.k[seg]; i0 += kStep) {
+            load_panel<T>(sa, p.a[seg], p.M, m0, p.k[seg], i0);
+            load_panel<T>(sb[0], p.b[seg], p.N, n0, p.k[seg], i0);
+            if (EPI == kFfGated) load_panel<T>(sb[1], p.b[1], p.N, n0, p.k[0], i0);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                float a[4], b[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[r] = sa[i][ty * 4 + r];
+#pragma unroll
+                for (int w = 0; w < (EPI == kFfGated ? 2 : 1); ++w) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) b[c] = sb[w][i][tx * 4 + c];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[w][r][c] = fmaf(a[r], b[c], acc[w][r][c]);
+                }
+            }
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t row = m0 + ty * 4 + r;
+        if (row >= p.M) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int col = n0 + tx * 4 + c;
+            if (col >= p.N) break;
+            const int64_t at = row * p.ldc + col, pre = row * p.N + col;
+            const float x = acc[0][r][c];
+            if (EPI == kFfStore) static_cast<T*>(p.c)[at] = FfElem<T>::put(x);
+            if (EPI == kFfGated) {
+                const float u = acc[1][r][c];
+                static_cast<T*>(p.c)[at] = FfElem<T>::put(activate<ACT, sizeof(T) == 2>(x).a * u);
+                if (p.pre_g) {
+                    p.pre_g[pre] = x;
+                    p.pre_u[pre] = u;
+                }
+            }
+            if (EPI == kFfSlope) {
+                const float u = p.pre_u[pre];
+                const ActValue v = activate<ACT, sizeof(T) == 2>(p.pre_g[pre]);
+                static_cast<T*>(p.c)[at] = FfElem<T>::put(x * u * v.slope);
+                static_cast<T*>(p.c2)[at] = FfElem<T>::put(x * v.a);
+                static_cast<T*>(p.c3)[at] = FfElem<T>::put(v.a * u);
+            }
+        }
+    }
+}
+
+template <class T, int EPI>
+int launch_simt(int act, const FfProduct& p, cudaStream_t s) {
+    const dim3 grid((p.N + kTile - 1) / kTile, (p.M + kTile - 1) / kTile);
+    if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many rows");
+    switch (EPI == kFfStore ? ZG_ACT_RELU : act) {
+        case ZG_ACT_SILU: ff_simt_kernel<T, EPI, ZG_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
+        case ZG_ACT_GELU: ff_simt_kernel<T, EPI, ZG_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
+        case ZG_ACT_GELU_TANH: ff_simt_kernel<T, EPI, ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
+        default: ff_simt_kernel<T, EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
+    }
+    return cuda_status(cudaGetLastError(), "gated_ff");
+}
+
+template <class T>
+int launch_simt_epi(FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s) {
+    switch (epi) {
+        case kFfStore: return launch_simt<T, kFfStore>(act, p, s);
+        case kFfGated: return launch_simt<T, kFfGated>(act, p, s);
+        default: return launch_simt<T, kFfSlope>(act, p, s);
+    }
+}
+
+}  // namespace
+
+int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s) {
+    if (p.M == 0 || p.N == 0) return ZG_OK;
+    switch (dtype) {
+        case ZG_DTYPE_F32: return launch_simt_epi<float>(epi, act, p, s);
+        case ZG_DTYPE_BF16: return launch_simt_epi<__nv_bfloat16>(epi, act, p, s);
+        default: return launch_simt_epi<__half>(epi, act, p, s);
+    }
+}
+
+namespace {
+
+uint64_t round_up(uint64_t x, uint64_t a) { return (x + a - 1) / a * a; }
+
+struct FfCall {
+    uint32_t dtype;
+    int mode, act;
+    int m, k, f, d;
+    uint64_t size;  // bytes of an element
+    bool backward;
+};
+
+// Workspace: h, then for the backward pass dg and du, [m, f] each.
+struct FfLayout {
+    int64_t ld_f;
+    uint64_t plane, total;
+};
+FfLayout ff_layout(const FfCall& c) {
+    FfLayout l;
+    l.ld_f = static_cast<int64_t>(round_up(c.f, 8));
+    l.plane = round_up(static_cast<uint64_t>(c.m) * l.ld_f * c.size, 256);
+    l.total = l.plane * (c.backward ? 3 : 1);
+    return l;
+}
+
+int check_call(FfCall& c, const char* what) {
+    if (c.dtype != ZG_DTYPE_F32 && c.dtype != ZG_DTYPE_F16 && c.dtype != ZG_DTYPE_BF16)
+        return set_error(ZG_ERR_DISPATCH, "%s: tensors are f32, bf16 or f16, got dtype %u", what,
+                         c.dtype);
+    c.size = c.dtype == ZG_DTYPE_F32 ? 4 : 2;
+    if (c.act < ZG_ACT_SILU || c.act > ZG_ACT_RELU)
+        return set_error(ZG_ERR_DISPATCH, "%s: unknown activation %d", what, c.act);
+    if (c.dtype == ZG_DTYPE_F32 && (c.mode < ZG_GEMM_SIMT_FP32 || c.mode > ZG_GEMM_BF16X3))
+        return set_error(ZG_ERR_DISPATCH, "%s: unknown mode %d", what, c.mode);
+    if (c.m < 0 || c.k < 1 || c.f < 1 || c.d < 1)
+        return set_error(ZG_ERR_DISPATCH, "%s: bad shape: %d rows, sizes %d, %d, %d", what, c.m,
+                         c.k, c.f, c.d);
+    return ZG_OK;
+}
+
+int check_workspace(const FfCall& c, const void* ws, uint64_t bytes, const char* what) {
+    const uint64_t need = ff_layout(c).total;
+    if (c.m > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
+        return set_error(ZG_ERR_DISPATCH,
+                         "%s: a 256-byte aligned workspace of %llu bytes is needed, got %llu", what,
+                         (unsigned long long)need, (unsigned long long)bytes);
+    return ZG_OK;
+}
+
+// Inputs start on 16-byte boundaries (the tensor maps' and vector loads' rule),
+// outputs on their element's.
+int check_pointers(std::initializer_list<const void*> in, std::initializer_list<const void*> out,
+                   const FfCall& c, const char* what) {
+    for (const void* p : in)
+        if (!p || (reinterpret_cast<uintptr_t>(p) & 15u))
+            return set_error(ZG_ERR_DISPATCH, "%s: null or not 16-byte aligned input", what);
+    for (const void* p : out)
+        if (!p || reinterpret_cast<uintptr_t>(p) % c.size)
+            return set_error(ZG_ERR_DISPATCH, "%s: null or misaligned output", what);
+    return ZG_OK;
+}
+
+int product(const FfCall& c, FfEpilogue epi, const FfProduct& p, cudaStream_t s) {
+    return ff_simt(c.dtype, epi, c.act, p, s);
+}
+
+}  // namespace
+}  // namespace zg
+
+using namespace zg;
+
+extern "C" uint64_t zg_gated_ff_workspace_bytes(uint32_t dtype, int mode, int m, int k, int f,
+                                                int d, int backward) {
+    FfCall c{dtype, mode, ZG_ACT_SILU, m, k, f, d, 0, backward != 0};
+    if (check_call(c, "gated_ff") != ZG_OK || m == 0) return 0;
+    return ff_layout(c).total;
+}
+
+extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
+                           const void* x, const void* w_gate, const void* w_up,
+                           const void* w_down, void* y, float* pre_gate, float* pre_up,
+                           void* workspace, uint64_t workspace_bytes, void* stream) {
+    FfCall c{dtype, mode, act, m, k, f, d, 0, false};
+    int rc = check_call(c, "gated_ff");
+    if (rc || m == 0) return rc;
+    if ((rc = check_pointers({x, w_gate, w_up, w_down}, {y}, c, "gated_ff"))) return rc;
+    if ((pre_gate == nullptr) != (pre_up == nullptr) ||
+        ((reinterpret_cast<uintptr_t>(pre_gate) | reinterpret_cast<uintptr_t>(pre_up)) & 15u))
+        return set_error(ZG_ERR_DISPATCH,
+                         "gated_ff: pre_gate and pre_up are both null or both 16-byte aligned");
+    if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff"))) return rc;
+    const FfLayout l = ff_layout(c);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    FfProduct p;
+    p.M = m, p.N = f, p.k[0] = k;
+    p.a[0] = {x, k, false};
+    p.b[0] = {w_gate, f, true};
+    p.b[1] = {w_up, f, true};
+    p.c = workspace, p.ldc = l.ld_f;
+    p.pre_g = pre_gate, p.pre_u = pre_up;
+    if ((rc = product(c, kFfGated, p, s))) return rc;
+    FfProduct q;
+    q.M = m, q.N = d, q.k[0] = f;
+    q.a[0] = {workspace, l.ld_f, false};
+    q.b[0] = {w_down, d, true};
+    q.c = y, q.ldc = d;
+    return product(c, kFfStore, q, s);
+}
+
+extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
+                                    const void* dy, const void* x, const void* w_gate,
+                                    const void* w_up, const void* w_down, const float* pre_gate,
+                                    const float* pre_up, void* dx, void* dw_gate, void* dw_up,
+                                    void* dw_down, void* workspace, uint64_t workspace_bytes,
+                                    void* stream) {
+    FfCall c{dtype, mode, act, m, k, f, d, 0, true};
+    int rc = check_call(c, "gated_ff_backward");
+    if (rc) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if ((rc = check_pointers({}, {dw_gate, dw_up, dw_down}, c, "gated_ff_backward"))) return rc;
+    if (m == 0) {  // sums over no rows
+        const uint64_t up = static_cast<uint64_t>(k) * f * c.size;
+        const uint64_t down = static_cast<uint64_t>(f) * d * c.size;
+        if ((rc = cuda_status(cudaMemsetAsync(dw_gate, 0, up, s), "gated_ff_backward"))) return rc;
+        if ((rc = cuda_status(cudaMemsetAsync(dw_up, 0, up, s), "gated_ff_backward"))) return rc;
+        return cuda_status(cudaMemsetAsync(dw_down, 0, down, s), "gated_ff_backward");
+    }
+    if ((rc = check_pointers({dy, x, w_gate, w_up, w_down, pre_gate, pre_up}, {dx}, c,
+                             "gated_ff_backward")))
+        return rc;
+    if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff_backward"))) return rc;
+    const FfLayout l = ff_layout(c);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    void *h = ws, *dg = ws + l.plane, *du = ws + 2 * l.plane;
+    FfProduct p;  // dh, and from it dg, du, h
+    p.M = m, p.N = f, p.k[0] = d;
+    p.a[0] = {dy, d, false};
+    p.b[0] = {w_down, d, false};
+    p.c = dg, p.c2 = du, p.c3 = h, p.ldc = l.ld_f;
+    p.pre_g = const_cast<float*>(pre_gate), p.pre_u = const_cast<float*>(pre_up);
+    if ((rc = product(c, kFfSlope, p, s))) return rc;
+    FfProduct q;  // dx
+    q.M = m, q.N = k, q.k[0] = q.k[1] = f;
+    q.a[0] = {dg, l.ld_f, false};
+    q.b[0] = {w_gate, f, false};
+    q.a[1] = {du, l.ld_f, false};
+    q.b[1] = {w_up, f, false};
+    q.c = dx, q.ldc = k;
+    if ((rc = product(c, kFfStore, q, s))) return rc;
+    for (int w = 0; w < 2; ++w) {  // dWg, dWu
+        FfProduct r;
+        r.M = k, r.N = f, r.k[0] = m;
+        r.a[0] = {x, k, true};
+        r.b[0] = {w ? du : dg, l.ld_f, true};
+        r.c = w ? dw_up : dw_gate, r.ldc = f;
+        if ((rc = product(c, kFfStore, r, s))) return rc;
+    }
+    FfProduct r;  // dWd
+    r.M = f, r.N = d, r.k[0] = m;
+    r.a[0] = {h, l.ld_f, true};
+    r.b[0] = {dy, d, true};
+    r.c = dw_down, r.ldc = d;
+    return product(c, kFfStore, r, s);
+}

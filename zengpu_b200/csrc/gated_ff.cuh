@@ -1,0 +1,103 @@
+// gated_ff.cuh - what the kernels of the gated feed-forward block share: the
+// activations and their derivatives, the products' operands, the epilogues.
+//
+//   forward   g = x Wg, u = x Wu, h = act(g) u, y = h Wd
+//   backward  dh = dy Wd^T, dg = dh u act'(g), du = dh act(g),
+//             dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du, dWd = h^T dy
+//
+// Sums, g and u are f32.  With 16-bit tensors h, dg and du are rounded once to
+// the tensors' type, because the next product reads them as tensor-core operands
+// of that type; g and u stay f32 between the passes, so that the backward pass
+// adds no rounding of its own to those three.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "zg_common.cuh"
+
+namespace zg {
+
+template <class T> struct FfElem;
+template <> struct FfElem<float> {
+    __device__ static float get(float x) { return x; }
+    __device__ static float put(float x) { return x; }
+};
+template <> struct FfElem<__nv_bfloat16> {
+    __device__ static float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+    __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+template <> struct FfElem<__half> {
+    __device__ static float get(__half x) { return __half2float(x); }
+    __device__ static __half put(float x) { return __float2half_rn(x); }
+};
+
+// a = act(g) and slope = act'(g).
+//   SiLU       s = 1 / (1 + e^-g): g s, s (1 + g (1 - s))
+//   GELU       c = Phi(g) = erfc(-g / sqrt 2) / 2: g c, c + g phi(g)
+//   GELU_TANH  the same with c = (1 + tanh q) / 2 = 1 / (1 + e^-2q),
+//              q = sqrt(2 / pi) (g + 0.044715 g^3): c' = 2 c (1 - c) q'
+//   ReLU       relu1: 0 (slope 0) for g <= 0 and NaN
+// erfc instead of 1 + erf, and 1 / (1 + e^-2q) instead of 1 + tanh, keep the
+// left tails' relative accuracy, where those sums cancel.
+struct ActValue {
+    float a, slope;
+};
+
+// FAST (16-bit tensors): __expf, whose error grows to 2^-18 relative at |g| = 30,
+// far below the rounding that follows; f32 tensors take expf and a true quotient.
+template <bool FAST>
+__device__ __forceinline__ float logistic(float x) {
+    return FAST ? __frcp_rn(1.0f + __expf(-x)) : 1.0f / (1.0f + expf(-x));
+}
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ ActValue activate(float g) {
+    if (ACT == ZG_ACT_RELU) return {relu1(g), g > 0.0f ? 1.0f : 0.0f};
+    if (ACT == ZG_ACT_SILU) {
+        const float s = logistic<FAST>(g);
+        return {g * s, s * (1.0f + g * (1.0f - s))};
+    }
+    if (ACT == ZG_ACT_GELU) {
+        const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+        const float e = -0.5f * g * g;
+        return {g * c, c + g * 0.39894228040143268f * (FAST ? __expf(e) : expf(e))};
+    }
+    const float k = 0.79788456080286536f;
+    const float q = k * (g + 0.044715f * g * g * g);
+    const float c = logistic<FAST>(2.0f * q);
+    return {g * c, c + g * 2.0f * c * (1.0f - c) * k * (1.0f + 3.0f * 0.044715f * g * g)};
+}
+
+// One operand of a product over `k`: row r (of M or N), position i of the sum.
+//   k-major   p[r * ld + i]
+//   mn-major  p[i * ld + r]
+struct FfOperand {
+    const void* p = nullptr;
+    int64_t ld = 0;
+    bool mn = false;
+};
+
+enum FfEpilogue { kFfStore, kFfGated, kFfSlope };
+
+// D[M x N].  kFfStore: c = a[0] b[0] (+ a[1] b[1] when k[1] > 0).
+// kFfGated: g = a[0] b[0], u = a[0] b[1]; c = act(g) u, and g, u to pre_g, pre_u
+// unless they are null.  kFfSlope: dh = a[0] b[0] with pre_g and pre_u read:
+// c = dg, c2 = du, c3 = h.  c, c2, c3: the tensors' type, pitch ldc; pre_g,
+// pre_u: f32, pitch N.
+struct FfProduct {
+    int M = 0, N = 0;
+    int k[2] = {0, 0};
+    FfOperand a[2], b[2];
+    void* c = nullptr;
+    void* c2 = nullptr;
+    void* c3 = nullptr;
+    int64_t ldc = 0;
+    float* pre_g = nullptr;
+    float* pre_u = nullptr;
+};
+
+// Plain CUDA-core product for any layout, f32 sums (gated_ff.cu).
+int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
+
+}  // namespace zg

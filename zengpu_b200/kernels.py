@@ -14,7 +14,7 @@ from typing import Sequence
 import torch
 
 from . import _lib as L
-from .api import DType, GemmMode, check
+from .api import Activation, DType, GemmMode, check
 
 ADAMW_BLOCK = 256  # elements that share a scale in 8-bit moments (ZG_ADAMW_BLOCK)
 
@@ -212,6 +212,104 @@ def sgemm_packed(pa: Packed, pb: Packed, c: torch.Tensor | None = None, alpha: f
                                    bias.data_ptr() if bias is not None else None,
                                    1 if relu else 0, _stream(c)))
     return c
+
+
+# ---- gated feed-forward block (zg_gated_ff, zg_gated_ff_backward) ----------------------
+def _ff_operand(name: str, t: torch.Tensor, shape: tuple[int, ...],
+                like: torch.Tensor) -> torch.Tensor:
+    if t.dtype != like.dtype or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {like.dtype} tensor on {like.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    # the kernels' copies start on 16-byte boundaries; a view that does not is copied
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ff_output(name: str, t: torch.Tensor | None, shape: tuple[int, ...],
+               like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    dtype = dtype or like.dtype
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if t.dtype != dtype or t.device != like.device or not t.is_contiguous() or \
+            tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape}")
+    return t
+
+
+def _ff_sizes(x: torch.Tensor, w_gate: torch.Tensor, w_down: torch.Tensor) -> tuple[int, ...]:
+    if x.device.type != "cuda" or x.dtype not in _FLOATS:
+        raise ValueError("gated_ff: expected f32, bf16 or f16 CUDA tensors")
+    if x.dim() != 2 or w_gate.dim() != 2 or w_down.dim() != 2:
+        raise ValueError("gated_ff: expected 2-D tensors")
+    return x.shape[0], x.shape[1], w_gate.shape[1], w_down.shape[1]
+
+
+def _ff_workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
+    """The stream's scratch; a capture gets memory of its own, which no other
+    graph or stream shares."""
+    if nbytes and torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return workspace_for(device, nbytes)
+
+
+def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+             act: int = Activation.SILU, mode: int = GemmMode.TF32X3, save: bool = False,
+             out: torch.Tensor | None = None):
+    """y = (act(x @ w_gate) * (x @ w_up)) @ w_down for contiguous x [m, k], w_gate
+    and w_up [k, f], w_down [f, d] of one dtype: f32 (in `mode`, as sgemm), bf16 or
+    f16 (f32 sums; the inner product is rounded once to the dtype).  save=True
+    returns (y, saved), `saved` being what gated_ff_backward needs: the two inner
+    products before the activation, f32 [m, f] each."""
+    m, k, f, d = _ff_sizes(x, w_gate, w_down)
+    with _on(x.device):
+        x = _ff_operand("x", x, (m, k), x)
+        w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
+        w_up = _ff_operand("w_up", w_up, (k, f), x)
+        w_down = _ff_operand("w_down", w_down, (f, d), x)
+        y = _ff_output("out", out, (m, d), x)
+        saved = tuple(_ff_output("saved", None, (m, f), x, torch.float32)
+                      for _ in range(2)) if save else ()
+        lib, dt = L.load(), _FLOATS[x.dtype]
+        need = int(lib.zg_gated_ff_workspace_bytes(dt, int(mode), m, k, f, d, 0))
+        ws = _ff_workspace(x.device, need)
+        check(lib.zg_gated_ff(dt, int(mode), int(act), m, k, f, d, x.data_ptr(), w_gate.data_ptr(),
+                              w_up.data_ptr(), w_down.data_ptr(), y.data_ptr(),
+                              *([t.data_ptr() for t in saved] or (None, None)),
+                              ws.data_ptr() if ws is not None else None, need, _stream(x)))
+    return (y, saved) if save else y
+
+
+def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
+                      w_up: torch.Tensor, w_down: torch.Tensor,
+                      saved: tuple[torch.Tensor, torch.Tensor], act: int = Activation.SILU,
+                      mode: int = GemmMode.TF32X3,
+                      out: Sequence[torch.Tensor | None] = (None, None, None, None)):
+    """(dx, dw_gate, dw_up, dw_down) of gated_ff for dy, the gradient of its y;
+    `saved` as gated_ff(..., save=True) gave it for the same x and weights.  `out`
+    takes tensors to write them to."""
+    m, k, f, d = _ff_sizes(x, w_gate, w_down)
+    with _on(x.device):
+        x = _ff_operand("x", x, (m, k), x)
+        dy = _ff_operand("dy", dy, (m, d), x)
+        w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
+        w_up = _ff_operand("w_up", w_up, (k, f), x)
+        w_down = _ff_operand("w_down", w_down, (f, d), x)
+        if len(saved) != 2 or any(t is None for t in saved):
+            raise ValueError("gated_ff_backward: saved has two tensors")
+        pre = [_ff_output("saved", t, (m, f), x, torch.float32) for t in saved]
+        pre = [t if t.data_ptr() % 16 == 0 else t.clone() for t in pre]
+        names = ("dx", "dw_gate", "dw_up", "dw_down")
+        got = tuple(_ff_output(n, t, s, x) for n, t, s in
+                    zip(names, out, ((m, k), (k, f), (k, f), (f, d)), strict=True))
+        lib, dt = L.load(), _FLOATS[x.dtype]
+        need = int(lib.zg_gated_ff_workspace_bytes(dt, int(mode), m, k, f, d, 1))
+        ws = _ff_workspace(x.device, need)
+        check(lib.zg_gated_ff_backward(
+            dt, int(mode), int(act), m, k, f, d, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+            w_up.data_ptr(), w_down.data_ptr(), pre[0].data_ptr(), pre[1].data_ptr(),
+            *[t.data_ptr() for t in got], ws.data_ptr() if ws is not None else None, need,
+            _stream(x)))
+    return got
 
 
 # ---- AdamW over many tensors, gradient norm (zg_adamw, zg_grad_norm) -------------------

@@ -136,17 +136,90 @@ struct FfCall {
     bool backward;
 };
 
-// Workspace: h, then for the backward pass dg and du, [m, f] each.
+// 16-bit rows copied to a pitch that is a multiple of 8 (16 bytes, the tensor
+// maps' rule), for sizes that are not: up to five tensors in one launch.
+struct PadCopy {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t rows;
+    int cols, ld;
+};
+struct PadCopies {
+    PadCopy t[5];
+    int64_t first[6];  // first group of eight elements of each tensor
+    int count;
+};
+
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadCopies c) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g < c.first[c.count];
+         g += step) {
+        int i = 0;
+        while (g >= c.first[i + 1]) ++i;
+        const PadCopy& t = c.t[i];
+        const int64_t at = (g - c.first[i]) * 8;
+        const int64_t row = at / t.ld;
+        const int col = static_cast<int>(at - row * t.ld);
+        const uint16_t* src = t.src + row * t.cols + col;
+        uint16_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = col + e < t.cols ? src[e] : 0;
+        uint4 q;
+        __builtin_memcpy(&q, v, 16);
+        *reinterpret_cast<uint4*>(t.dst + at) = q;
+    }
+}
+
+// Workspace: h, then for the backward pass dg and du, [m, f] each; then padded
+// copies of the 16-bit inputs that need them.
+enum { kX, kWg, kWu, kWd, kDy, kInputs };
 struct FfLayout {
     int64_t ld_f;
     uint64_t plane, total;
+    bool pad[kInputs];
+    uint64_t at[kInputs];
 };
 FfLayout ff_layout(const FfCall& c) {
     FfLayout l;
     l.ld_f = static_cast<int64_t>(round_up(c.f, 8));
     l.plane = round_up(static_cast<uint64_t>(c.m) * l.ld_f * c.size, 256);
     l.total = l.plane * (c.backward ? 3 : 1);
+    const int rows[kInputs] = {c.m, c.k, c.k, c.f, c.m}, cols[kInputs] = {c.k, c.f, c.f, c.d, c.d};
+    for (int i = 0; i < kInputs; ++i) {
+        l.pad[i] = c.size == 2 && cols[i] % 8 != 0 && (c.backward || i != kDy);
+        l.at[i] = l.total;
+        if (l.pad[i]) l.total += round_up(rows[i] * round_up(cols[i], 8) * c.size, 256);
+    }
     return l;
+}
+
+struct FfInput {
+    const void* p;
+    int64_t ld;
+};
+
+// The inputs as the products read them: where they lie, or padded.
+int place_inputs(const FfCall& c, const FfLayout& l, uint8_t* ws, const void* const* src,
+                 FfInput* out, cudaStream_t s) {
+    const int rows[kInputs] = {c.m, c.k, c.k, c.f, c.m}, cols[kInputs] = {c.k, c.f, c.f, c.d, c.d};
+    PadCopies pc;
+    pc.count = 0;
+    pc.first[0] = 0;
+    for (int i = 0; i < kInputs; ++i) {
+        out[i] = {src[i], cols[i]};
+        if (!l.pad[i]) continue;
+        PadCopy& t = pc.t[pc.count];
+        t.src = static_cast<const uint16_t*>(src[i]);
+        t.dst = reinterpret_cast<uint16_t*>(ws + l.at[i]);
+        t.rows = rows[i], t.cols = cols[i], t.ld = static_cast<int>(round_up(cols[i], 8));
+        pc.first[pc.count + 1] = pc.first[pc.count] + t.rows * (t.ld / 8);
+        ++pc.count;
+        out[i] = {t.dst, t.ld};
+    }
+    if (!pc.count) return ZG_OK;
+    const int64_t blocks = (pc.first[pc.count] + 255) / 256;
+    pad_rows_kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 16)), 256, 0, s>>>(pc);
+    return cuda_status(cudaGetLastError(), "gated_ff padding");
 }
 
 int check_call(FfCall& c, const char* what) {
@@ -186,8 +259,11 @@ int check_pointers(std::initializer_list<const void*> in, std::initializer_list<
     return ZG_OK;
 }
 
-int product(const FfCall& c, FfEpilogue epi, const FfProduct& p, cudaStream_t s) {
-    return ff_simt(c.dtype, epi, c.act, p, s);
+int products(const FfCall& c, FfEpilogue epi, const FfProduct* p, int count, cudaStream_t s) {
+    if (c.size == 2) return ff_pair(c.dtype, epi, c.act, p, count, s);
+    int rc = ZG_OK;
+    for (int i = 0; i < count && !rc; ++i) rc = ff_simt(c.dtype, epi, c.act, p[i], s);
+    return rc;
 }
 
 }  // namespace
@@ -217,20 +293,23 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
     if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff"))) return rc;
     const FfLayout l = ff_layout(c);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    FfProduct p;
+    const void* src[kInputs] = {x, w_gate, w_up, w_down, nullptr};
+    FfInput in[kInputs];
+    if ((rc = place_inputs(c, l, static_cast<uint8_t*>(workspace), src, in, s))) return rc;
+    FfProduct p;  // h
     p.M = m, p.N = f, p.k[0] = k;
-    p.a[0] = {x, k, false};
-    p.b[0] = {w_gate, f, true};
-    p.b[1] = {w_up, f, true};
+    p.a[0] = {in[kX].p, in[kX].ld, false};
+    p.b[0] = {in[kWg].p, in[kWg].ld, true};
+    p.b[1] = {in[kWu].p, in[kWu].ld, true};
     p.c = workspace, p.ldc = l.ld_f;
     p.pre_g = pre_gate, p.pre_u = pre_up;
-    if ((rc = product(c, kFfGated, p, s))) return rc;
-    FfProduct q;
+    if ((rc = products(c, kFfGated, &p, 1, s))) return rc;
+    FfProduct q;  // y
     q.M = m, q.N = d, q.k[0] = f;
     q.a[0] = {workspace, l.ld_f, false};
-    q.b[0] = {w_down, d, true};
+    q.b[0] = {in[kWd].p, in[kWd].ld, true};
     q.c = y, q.ldc = d;
-    return product(c, kFfStore, q, s);
+    return products(c, kFfStore, &q, 1, s);
 }
 
 extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
@@ -258,33 +337,32 @@ extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, in
     const FfLayout l = ff_layout(c);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     void *h = ws, *dg = ws + l.plane, *du = ws + 2 * l.plane;
+    const void* src[kInputs] = {x, w_gate, w_up, w_down, dy};
+    FfInput in[kInputs];
+    if ((rc = place_inputs(c, l, ws, src, in, s))) return rc;
     FfProduct p;  // dh, and from it dg, du, h
     p.M = m, p.N = f, p.k[0] = d;
-    p.a[0] = {dy, d, false};
-    p.b[0] = {w_down, d, false};
+    p.a[0] = {in[kDy].p, in[kDy].ld, false};
+    p.b[0] = {in[kWd].p, in[kWd].ld, false};
     p.c = dg, p.c2 = du, p.c3 = h, p.ldc = l.ld_f;
     p.pre_g = const_cast<float*>(pre_gate), p.pre_u = const_cast<float*>(pre_up);
-    if ((rc = product(c, kFfSlope, p, s))) return rc;
+    if ((rc = products(c, kFfSlope, &p, 1, s))) return rc;
     FfProduct q;  // dx
     q.M = m, q.N = k, q.k[0] = q.k[1] = f;
     q.a[0] = {dg, l.ld_f, false};
-    q.b[0] = {w_gate, f, false};
+    q.b[0] = {in[kWg].p, in[kWg].ld, false};
     q.a[1] = {du, l.ld_f, false};
-    q.b[1] = {w_up, f, false};
+    q.b[1] = {in[kWu].p, in[kWu].ld, false};
     q.c = dx, q.ldc = k;
-    if ((rc = product(c, kFfStore, q, s))) return rc;
-    for (int w = 0; w < 2; ++w) {  // dWg, dWu
-        FfProduct r;
-        r.M = k, r.N = f, r.k[0] = m;
-        r.a[0] = {x, k, true};
-        r.b[0] = {w ? du : dg, l.ld_f, true};
-        r.c = w ? dw_up : dw_gate, r.ldc = f;
-        if ((rc = product(c, kFfStore, r, s))) return rc;
-    }
-    FfProduct r;  // dWd
-    r.M = f, r.N = d, r.k[0] = m;
-    r.a[0] = {h, l.ld_f, true};
-    r.b[0] = {dy, d, true};
-    r.c = dw_down, r.ldc = d;
-    return product(c, kFfStore, r, s);
+    if ((rc = products(c, kFfStore, &q, 1, s))) return rc;
+    FfProduct w[3];  // dWg, dWu, dWd
+    for (int i = 0; i < 3; ++i) w[i].k[0] = m;
+    w[0].M = w[1].M = k, w[0].N = w[1].N = f, w[0].ldc = w[1].ldc = f;
+    w[0].a[0] = w[1].a[0] = {in[kX].p, in[kX].ld, true};
+    w[0].b[0] = {dg, l.ld_f, true}, w[0].c = dw_gate;
+    w[1].b[0] = {du, l.ld_f, true}, w[1].c = dw_up;
+    w[2].M = f, w[2].N = d, w[2].ldc = d;
+    w[2].a[0] = {h, l.ld_f, true};
+    w[2].b[0] = {in[kDy].p, in[kDy].ld, true}, w[2].c = dw_down;
+    return products(c, kFfStore, w, 3, s);
 }

@@ -100,4 +100,10 @@ struct FfProduct {
 // Plain CUDA-core product for any layout, f32 sums (gated_ff.cu).
 int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
 
+// 16-bit tensors on the tensor cores (gated_ff_tc.cu): `count` products of one
+// epilogue in one launch (at most three).  Operands: 16-byte aligned, pitch a
+// multiple of 8.
+int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
+            cudaStream_t s);
+
 }  // namespace zg

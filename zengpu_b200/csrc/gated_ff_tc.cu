@@ -1,0 +1,438 @@
+// gated_ff_tc.cu - the products of the gated feed-forward block on 16-bit tensors:
+// tcgen05 CTA pairs, operands read as they lie in memory.
+//
+// Every product of the block (gated_ff.cuh) is D[M x N] = A B with A's rows and
+// B's columns contiguous along the sum (k-major: x, h, dg, du, dy; Wd^T, Wg^T, Wu^T
+// in the backward pass) or across it (mn-major: the weights in the forward pass;
+// x^T, h^T, dg, du, dy under the weights' gradients).  16-bit MMAs take both from
+// shared memory, so nothing is transposed or packed first.
+//
+// Two CTAs of a cluster (tcgen05 cta_group::2) compute a 256 x 256 tile; CTA r
+// holds rows [128 r, 128 r + 128) of A and of D, and half of B's columns.  Stages
+// hold 64 of the sum: 16 KB of A and of B per CTA, each as two boxes of 64 rows
+// (k-major: 64 rows of 64 of the sum; mn-major: 64 of the sum for 64 rows), 8 KB
+// with 128-byte swizzle:
+//   k-major   8-row groups 1024 bytes apart; an MMA's 16 of the sum are 32 bytes
+//             along the rows
+//   mn-major  8-groups of the sum 1024 bytes apart, the second 64 rows 8192; an
+//             MMA's 16 of the sum are 2048 bytes further
+// For the gated pair of products CTA 0 loads 128 columns of Wg and CTA 1 the same
+// columns of Wu: one accumulator holds 128 columns of g beside 128 of u, the
+// epilogue threads find both for their row, and neither goes through memory.
+// dh's epilogue reads g and u and writes dg, du and h; dh itself stays in TMEM.
+// dx sums two products in one accumulator; the three weights' gradients share one
+// launch.
+//
+// Roles as in the f32 kernels (sgemm_tc.cu): warp 0 TMA, warp 1 MMA (CTA 0 of the
+// pair issues), warps 2-9 epilogue.  The f32 accumulator stays in TMEM over the
+// whole sum: its additions truncate, about n / 16 2^-24 of the result for n terms,
+// which at n = 12288 is 5e-5, a tenth of half an f16 step.  Two accumulators: a
+// tile's epilogue overlaps the next tile's MMAs.  When the last wave would keep
+// at most half of the pairs busy its tiles run as two column halves.
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+#include <cstring>
+
+#include "gated_ff.cuh"
+#include "zg_gemm_internal.h"
+
+namespace zg {
+namespace {
+
+constexpr int kThreads = 320, kEpiWarps = 8;
+constexpr int kBK = 64, kBox = 64;             // of the sum per stage; rows per box
+constexpr int kBoxBytes = kBox * 128;          // 8 KB
+constexpr int kOperandBytes = 2 * kBoxBytes;   // 128 rows
+constexpr int kStageBytes = 2 * kOperandBytes; // A and B: 32 KB per CTA
+constexpr int kStages = 6;
+constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*bars*/;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxProblems = 3;
+
+struct alignas(64) PairProblem {
+    CUtensorMap a[2], b[2];
+    void* c;
+    void* c2;
+    void* c3;
+    float* pre_g;
+    float* pre_u;
+    int64_t ldc;
+    int M, N;
+    int nkb[2];  // stages of the two sums
+    int a_mn, b_mn;
+    int vec_c, vec_pre;
+    int tiles;  // of this problem and those before it
+};
+
+struct PairArgs {
+    PairProblem p[kMaxProblems];
+    int count;
+    int full_units, split;
+    uint32_t* status;
+};
+
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
+           (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+           (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: f32 D, M = 256, N, types and majors.
+template <class T>
+__device__ __forceinline__ uint32_t instr_desc(int n, int a_mn, int b_mn) {
+    const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(256 >> 4) << 24);
+}
+
+// Two 64-row boxes (one when `rows` is 64) of an operand, rows from r0, the sum
+// from i0.
+__device__ __forceinline__ void load_operand(uint8_t* smem, const CUtensorMap* map, int mn, int r0,
+                                             int i0, int rows, uint32_t bar) {
+    for (int b = 0; b < rows; b += kBox)
+        tma_load_2d_pair(smem + b * 128, map, mn ? r0 + b : i0, mn ? i0 : r0 + b, bar);
+}
+
+// Grouped raster, as the f32 kernels' (eight row tiles before the next column).
+__device__ __forceinline__ void raster(int tile, int mt, int nt, int& mi, int& ni) {
+    const int group = tile / (8 * nt), first = group * 8;
+    const int gm = min(mt - first, 8), r = tile - group * 8 * nt;
+    mi = first + r % gm;
+    ni = r / gm;
+}
+
+// A unit of work: a tile, or a column half of one of the last tiles.
+struct Unit {
+    const PairProblem* p;
+    int m0, n0, width;  // width: columns of D in TMEM, 256 or 128
+};
+template <int EPI>
+__device__ __forceinline__ Unit unit_of(const PairArgs& args, int u) {
+    const bool half = u >= args.full_units && args.split > 1;
+    const int tile = half ? args.full_units + (u - args.full_units) / 2 : u;
+    int i = 0;
+    while (i + 1 < args.count && tile >= args.p[i].tiles) ++i;
+    const PairProblem& p = args.p[i];
+    constexpr int cols = EPI == kFfGated ? 128 : 256;  // columns of the output
+    int mi, ni;
+    raster(tile - (i ? args.p[i - 1].tiles : 0), (p.M + 255) / 256, (p.N + cols - 1) / cols, mi,
+           ni);
+    Unit w;
+    w.p = &p;
+    w.m0 = mi * 256;
+    w.n0 = ni * cols + (half ? ((u - args.full_units) & 1) * (cols / 2) : 0);
+    w.width = half ? 128 : 256;
+    return w;
+}
+
+// 32 neighbouring values of a row, `cols` of them inside the matrix.
+template <class T>
+__device__ __forceinline__ void store32(T* dst, const float (&v)[32], int cols, bool vec) {
+    if (vec && cols >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 16 / sizeof(T)) {
+            uint4 q;
+            T* t = reinterpret_cast<T*>(&q);
+#pragma unroll
+            for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e)
+                t[e] = FfElem<T>::put(v[i + e]);
+            *reinterpret_cast<uint4*>(dst + i) = q;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < cols) dst[i] = FfElem<T>::put(v[i]);
+    }
+}
+__device__ __forceinline__ void load32(const float* src, float (&v)[32], int cols, bool vec) {
+    if (vec && cols >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(src + i);
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i < cols ? src[i] : 0.0f;
+    }
+}
+
+template <int EPI, int ACT, class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    ff_pair_kernel(const __grid_constant__ PairArgs args) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+    uint64_t* empty = full + kStages;
+    uint64_t* acc_full = empty + kStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int units =
+        args.full_units + (args.p[args.count - 1].tiles - args.full_units) * args.split;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 2 * kEpiWarps);
+        }
+        mbar_init(drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, kTmemCols);
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int u = pair; u < units && ok; u += npairs) {
+                const Unit w = unit_of<EPI>(args, u);
+                const PairProblem& p = *w.p;
+                const int b_rows = w.width / 2;
+                // gated: CTA 0 takes Wg's columns, CTA 1 the same columns of Wu
+                const int b0 = EPI == kFfGated ? w.n0 : w.n0 + b_rows * static_cast<int>(rank);
+                const int nkb = p.nkb[0] + p.nkb[1];
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const int s = it % kStages;
+                    if (!mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, args.status,
+                                           kErrFfProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    if (leader)
+                        mbar_arrive_expect_tx(&full[s], 2 * (kOperandBytes + b_rows * 128));
+                    const uint32_t bar = mapa_shared(&full[s], 0);
+                    uint8_t* st = smem + s * kStageBytes;
+                    const int seg = kb < p.nkb[0] ? 0 : 1;
+                    const int i0 = (kb - (seg ? p.nkb[0] : 0)) * kBK;
+                    load_operand(st, &p.a[seg], p.a_mn, w.m0 + 128 * static_cast<int>(rank), i0,
+                                 128, bar);
+                    load_operand(st + kOperandBytes, &p.b[EPI == kFfGated ? rank : seg], p.b_mn,
+                                 b0, i0, b_rows, bar);
+                }
+            }
+            // no copy may still be landing at exit: wait until the last stages were read
+            for (int i = it > kStages ? it - kStages : 0; i < it; ++i)
+                mbar_wait_bounded(&empty[i % kStages], (i / kStages) & 1, args.status, kErrFfDrain);
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (CTA 0) ----------------
+        if (leader && lane == 0) {
+            bool ok = true;
+            int it = 0, n = 0;
+            for (int u = pair; u < units && ok; u += npairs, ++n) {
+                const Unit w = unit_of<EPI>(args, u);
+                const PairProblem& p = *w.p;
+                const int buf = n & 1;
+                const uint32_t d_tmem = tmem_base + buf * 256;
+                if (n >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((n >> 1) - 1) & 1, args.status,
+                                                 kErrFfMma)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t idesc = instr_desc<T>(w.width, p.a_mn, p.b_mn);
+                const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+                const int nkb = p.nkb[0] + p.nkb[1];
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const int s = it % kStages;
+                    if (!mbar_wait_bounded(&full[s], (it / kStages) & 1, args.status, kErrFfMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + s * kStageBytes), b = a + kOperandBytes;
+#pragma unroll
+                    for (int i = 0; i < kBK / 16; ++i)
+                        mma_f16_ss_pair(d_tmem, smem_desc(a + i * a_step, kBoxBytes),
+                                        smem_desc(b + i * b_step, kBoxBytes), idesc,
+                                        (kb | i) != 0);
+                    mma_commit_pair(&empty[s], 0x3);
+                }
+                if (ok) mma_commit_pair(&acc_full[buf], 0x3);
+            }
+            if (!ok) {
+                mma_commit_pair(drain, 0x1);
+                mbar_wait_bounded(drain, 0, args.status, kErrFfDrain);
+            }
+        }
+    } else {
+        // ---------------- epilogue (warps 2..9, both CTAs) ----------------
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+        const uint32_t leader_empty0 = mapa_shared(&acc_empty[0], 0);
+        const uint32_t leader_empty1 = mapa_shared(&acc_empty[1], 0);
+        int n = 0;
+        for (int u = pair; u < units; u += npairs, ++n) {
+            const Unit w = unit_of<EPI>(args, u);
+            const PairProblem& p = *w.p;
+            const int64_t row = w.m0 + 128 * static_cast<int>(rank) + q * 32 + lane;
+            const int buf = n & 1;
+            const bool got = mbar_wait_bounded(&acc_full[buf], (n >> 1) & 1, args.status,
+                                               kErrFfEpilogue);
+            // the TMEM loads below are warp-collective: the warp gives up together
+            if (!__all_sync(0xffffffffu, got)) break;
+            tc_fence_after();
+            const uint32_t d = lane_base + buf * 256;
+            // columns of the output this warp covers
+            const int span = EPI == kFfGated ? w.width / 4 : w.width / 2;
+            for (int c0 = half * span; c0 < (half + 1) * span; c0 += 32) {
+                uint32_t r[32];
+                float v[32];
+                tmem_ld_32x32b_x32(d + c0, r);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                const int col = w.n0 + c0, cols = p.N - col;
+                const bool in = row < p.M && cols > 0;
+                const int64_t at = row * p.ldc + col, pre = row * p.N + col;
+                T* c = static_cast<T*>(p.c) + at;
+                if (EPI == kFfStore && in) store32<T>(c, v, cols, p.vec_c);
+                if (EPI == kFfGated) {
+                    tmem_ld_32x32b_x32(d + w.width / 2 + c0, r);
+                    if (in) {
+                        float x[32];
+                        if (p.pre_g) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+                            store32<float>(p.pre_g + pre, v, cols, p.vec_pre);
+                            store32<float>(p.pre_u + pre, x, cols, p.vec_pre);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            v[i] = activate<ACT, true>(v[i]).a * __uint_as_float(r[i]);
+                        store32<T>(c, v, cols, p.vec_c);
+                    }
+                }
+                if (EPI == kFfSlope && in) {
+                    float g[32], x[32];
+                    load32(p.pre_g + pre, g, cols, p.vec_pre);
+                    load32(p.pre_u + pre, x, cols, p.vec_pre);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const ActValue a = activate<ACT, true>(g[i]);
+                        g[i] = v[i] * x[i] * a.slope;
+                        v[i] = v[i] * a.a;
+                        x[i] = a.a * x[i];
+                    }
+                    store32<T>(c, g, cols, p.vec_c);
+                    store32<T>(static_cast<T*>(p.c2) + at, v, cols, p.vec_c);
+                    store32<T>(static_cast<T*>(p.c3) + at, x, cols, p.vec_c);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(buf ? leader_empty1 : leader_empty0);
+        }
+    }
+
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+int sm_pairs() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return std::max((sms > 0 ? sms : 148) / 2, 1);
+}
+
+// An operand as 64 x 64 boxes: inner dimension along the memory.
+int operand_map(CUtensorMap* map, uint32_t dtype, const FfOperand& o, int rows, int sum) {
+    return encode_16bit_map(map, dtype, o.p, o.mn ? rows : sum, o.mn ? sum : rows, o.ld, kBox, kBox);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int EPI, int ACT, class T>
+int launch(const PairArgs& args, int units, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(ff_pair_kernel<EPI, ACT, T>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    }
+    if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
+    ff_pair_kernel<EPI, ACT, T><<<2 * std::min(units, sm_pairs()), kThreads, kSmemBytes, s>>>(args);
+    return cuda_status(cudaGetLastError(), "gated_ff");
+}
+
+template <class T>
+int launch_epi(FfEpilogue epi, int act, const PairArgs& a, int units, cudaStream_t s) {
+    if (epi == kFfStore) return launch<kFfStore, ZG_ACT_RELU, T>(a, units, s);
+    if (epi == kFfGated) switch (act) {
+            case ZG_ACT_SILU: return launch<kFfGated, ZG_ACT_SILU, T>(a, units, s);
+            case ZG_ACT_GELU: return launch<kFfGated, ZG_ACT_GELU, T>(a, units, s);
+            case ZG_ACT_GELU_TANH: return launch<kFfGated, ZG_ACT_GELU_TANH, T>(a, units, s);
+            default: return launch<kFfGated, ZG_ACT_RELU, T>(a, units, s);
+        }
+    switch (act) {
+        case ZG_ACT_SILU: return launch<kFfSlope, ZG_ACT_SILU, T>(a, units, s);
+        case ZG_ACT_GELU: return launch<kFfSlope, ZG_ACT_GELU, T>(a, units, s);
+        case ZG_ACT_GELU_TANH: return launch<kFfSlope, ZG_ACT_GELU_TANH, T>(a, units, s);
+        default: return launch<kFfSlope, ZG_ACT_RELU, T>(a, units, s);
+    }
+}
+
+}  // namespace
+
+int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
+            cudaStream_t s) {
+    PairArgs args;
+    std::memset(&args, 0, sizeof(args));
+    args.count = count;
+    int rc = status_word(&args.status), tiles = 0;
+    const int cols = epi == kFfGated ? 128 : 256;
+    for (int i = 0; i < count && !rc; ++i) {
+        const FfProduct& f = products[i];
+        PairProblem& p = args.p[i];
+        p.M = f.M, p.N = f.N;
+        p.a_mn = f.a[0].mn, p.b_mn = f.b[0].mn;
+        p.c = f.c, p.c2 = f.c2, p.c3 = f.c3, p.ldc = f.ldc;
+        p.pre_g = f.pre_g, p.pre_u = f.pre_u;
+        p.vec_c = f.ldc % 8 == 0 && aligned16(f.c) && aligned16(f.c2) && aligned16(f.c3);
+        p.vec_pre = f.N % 4 == 0 && aligned16(f.pre_g) && aligned16(f.pre_u);
+        for (int seg = 0; seg < 2; ++seg) p.nkb[seg] = (f.k[seg] + kBK - 1) / kBK;
+        rc = operand_map(&p.a[0], dtype, f.a[0], f.M, f.k[0]);
+        if (!rc) rc = operand_map(&p.b[0], dtype, f.b[0], f.N, f.k[0]);
+        if (!rc && f.k[1]) rc = operand_map(&p.a[1], dtype, f.a[1], f.M, f.k[1]);
+        if (!rc && f.b[1].p) rc = operand_map(&p.b[1], dtype, f.b[1], f.N, f.k[1] ? f.k[1] : f.k[0]);
+        const int64_t total =
+            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + cols - 1) / cols);
+        if (total > (1 << 29)) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many tiles");
+        p.tiles = tiles = static_cast<int>(total);
+    }
+    if (rc) return rc;
+    const int pairs = sm_pairs(), rem = tiles % pairs;
+    args.split = rem > 0 && 2 * rem <= pairs ? 2 : 1;
+    args.full_units = args.split > 1 ? tiles - rem : tiles;
+    const int units = args.full_units + (tiles - args.full_units) * args.split;
+    return dtype == ZG_DTYPE_BF16 ? launch_epi<__nv_bfloat16>(epi, act, args, units, s)
+                                  : launch_epi<__half>(epi, act, args, units, s);
+}
+
+}  // namespace zg

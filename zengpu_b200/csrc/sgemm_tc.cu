@@ -1123,6 +1123,34 @@ int encode_f32_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t r
     return ZG_OK;
 }
 
+int encode_16bit_map(CUtensorMap* map, uint32_t dtype, const void* base, uint64_t cols,
+                     uint64_t rows, uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
+    auto fn = get_encode_fn();
+    if (!fn) return set_error(ZG_ERR_BACKEND, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld * 2};
+    cuuint32_t box[2] = {box_cols, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map,
+                    dtype == ZG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                    2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(ZG_ERR_BACKEND, "cuTensorMapEncodeTiled failed (%d): %llux%llu ld=%llu",
+                         static_cast<int>(r), (unsigned long long)rows, (unsigned long long)cols,
+                         (unsigned long long)ld);
+    return ZG_OK;
+}
+
+int status_word(uint32_t** word) {
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_status);
+    *word = static_cast<uint32_t*>(p);
+    return e == cudaSuccess ? ZG_OK : cuda_status(e, "device status word");
+}
+
 // ---- GEMM building blocks (shared with the packed API and the host GEMM) -----------
 bool gemm_a_needs_planes(int mode, int K) {
     return mode == ZG_GEMM_TF32X3 || mode == ZG_GEMM_TF32_BF16X2 || mode == ZG_GEMM_BF16X3 ||

@@ -21,6 +21,10 @@ enum : uint32_t {
     kErrSimtProducer = 1u << 5,  // TMA-fed SIMT SGEMM: a stage was never freed
     kErrSimtConsumer = 1u << 6,  // ... a stage never arrived
     kErrSimtDrain = 1u << 7,     // ... an issued copy never landed before exit
+    kErrFfProducer = 1u << 8,    // gated feed-forward: a stage was never freed
+    kErrFfMma = 1u << 9,         // ... a stage never arrived, or an accumulator was never read
+    kErrFfEpilogue = 1u << 10,   // ... an accumulator was never completed
+    kErrFfDrain = 1u << 11,      // ... an issued copy or MMA never finished before exit
 };
 
 // Every on-device wait gives up after this long and reports instead of
@@ -304,6 +308,12 @@ int cuda_status(cudaError_t e, const char* what);
 // {box_cols, box_rows}; out-of-range elements load as zero.
 int encode_f32_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t ld,
                    uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+// The same over 16-bit elements (dtype ZG_DTYPE_BF16 or _F16), 128-byte swizzle:
+// `rows` rows of `cols` elements, pitch `ld` elements (a multiple of 8).
+int encode_16bit_map(CUtensorMap* map, uint32_t dtype, const void* base, uint64_t cols,
+                     uint64_t rows, uint64_t ld, uint32_t box_cols, uint32_t box_rows);
+// Address of the tensor-core kernels' status word on the current device.
+int status_word(uint32_t** word);
 // Reads and clears the SIMT SGEMM's device status word (bits kErrSimt*).
 cudaError_t take_simt_status(uint32_t* v);
 }  // namespace zg

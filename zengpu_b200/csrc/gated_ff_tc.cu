@@ -45,8 +45,22 @@ constexpr int kBK = 64, kBox = 64;             // of the sum per stage; rows per
 constexpr int kBoxBytes = kBox * 128;          // 8 KB
 constexpr int kOperandBytes = 2 * kBoxBytes;   // 128 rows
 constexpr int kStageBytes = 2 * kOperandBytes; // A and B: 32 KB per CTA
-constexpr int kStages = 6;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*align*/ + 256 /*bars*/;
+// Stages: five; dh's epilogue, which also holds blocks of g and u, leaves room for
+// four.
+constexpr int kStageCount[3] = {5, 5, 4};
+// An epilogue warp turns blocks of 32 x 32 between "a row per lane" (TMEM) and
+// "neighbours along a row" (memory) through shared memory of its own, with rows of
+// 144 bytes (f32) or 80 (16 bits): an odd number of 16-byte pieces, so that accesses
+// of either kind meet no bank twice.
+template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
+constexpr int kBlock32 = 32 * kPitch<float>;
+constexpr int kBlock16 = 32 * kPitch<__half>;
+constexpr int kTurnBytes[3] = {kBlock16, kBlock32, kBlock16 + 2 * kBlock32};
+constexpr int smem_bytes(int epi) {
+    return kStageCount[epi] * kStageBytes + kEpiWarps * kTurnBytes[epi] + 1024 /*align*/ +
+           256 /*bars*/;
+}
+static_assert(smem_bytes(2) <= 232448, "shared memory of an SM");
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxProblems = 3;
 
@@ -127,45 +141,80 @@ __device__ __forceinline__ Unit unit_of(const PairArgs& args, int u) {
     return w;
 }
 
-// 32 neighbouring values of a row, `cols` of them inside the matrix.
+// A lane's row of 32 values as 16-bit pairs, for the tensors' type.
 template <class T>
-__device__ __forceinline__ void store32(T* dst, const float (&v)[32], int cols, bool vec) {
-    if (vec && cols >= 32) {
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {
+    T t[2] = {FfElem<T>::put(lo), FfElem<T>::put(hi)};
+    uint32_t w;
+    __builtin_memcpy(&w, t, 4);
+    return w;
+}
+
+// Stores a warp's 32 x 32 block of T, row `lane` in the words of v, at `dst` (its
+// row 0, column 0); `rows` and `cols` of it lie inside the matrix.  vec: 16-byte
+// pieces of rows; otherwise (odd pitch or base) one element a lane, neighbours
+// side by side.
+template <class T>
+__device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int cols, bool vec,
+                                            const uint32_t (&v)[8 * sizeof(T)], uint8_t* turn,
+                                            int lane) {
+    constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer, kTurnPitch = kPitch<T>;
+    __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 32; i += 16 / sizeof(T)) {
-            uint4 q;
-            T* t = reinterpret_cast<T*>(&q);
+    for (int i = 0; i < kPieces; ++i)
+        *reinterpret_cast<uint4*>(turn + lane * kTurnPitch + i * 16) =
+            make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+    if (vec) {
 #pragma unroll
-            for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e)
-                t[e] = FfElem<T>::put(v[i + e]);
-            *reinterpret_cast<uint4*>(dst + i) = q;
+        for (int j = 0; j < kPieces; ++j) {
+            const int r = (j * 32 + lane) / kPieces, piece = lane % kPieces;
+            if (r < rows && piece * kPer < cols)
+                *reinterpret_cast<uint4*>(dst + r * ld + piece * kPer) =
+                    *reinterpret_cast<const uint4*>(turn + r * kTurnPitch + piece * 16);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < cols) dst[i] = FfElem<T>::put(v[i]);
+    } else if (lane < cols) {
+        for (int r = 0; r < rows; ++r)
+            dst[r * ld + lane] = reinterpret_cast<const T*>(turn + r * kTurnPitch)[lane];
     }
 }
-__device__ __forceinline__ void load32(const float* src, float (&v)[32], int cols, bool vec) {
-    if (vec && cols >= 32) {
+
+// The reverse for f32, asynchronous: copies the block's rows into `turn`, zeros
+// outside the matrix.  Pieces as store_block's.
+__device__ __forceinline__ void fetch_block(const float* src, int64_t ld, int rows, int cols,
+                                            bool vec, uint8_t* turn, int lane) {
+    const uint32_t to = smem_u32(turn);
+    if (vec) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(src + i);
-            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        for (int j = 0; j < 8; ++j) {
+            const int r = (j * 32 + lane) / 8, piece = lane % 8;
+            const bool in = r < rows && piece * 4 < cols;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             to + r * kPitch<float> + piece * 16),
+                         "l"(in ? src + r * ld + piece * 4 : src), "r"(in ? 16 : 0)
+                         : "memory");
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i < cols ? src[i] : 0.0f;
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+            const bool in = r < rows && lane < cols;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                             to + r * kPitch<float> + lane * 4),
+                         "l"(in ? src + r * ld + lane : src), "r"(in ? 4 : 0)
+                         : "memory");
+        }
     }
 }
 
 template <int EPI, int ACT, class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ff_pair_kernel(const __grid_constant__ PairArgs args) {
+    constexpr int kStages = kStageCount[EPI];
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+    uint8_t* turns = smem + kStages * kStageBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turns + kEpiWarps * kTurnBytes[EPI]);
     uint64_t* empty = full + kStages;
     uint64_t* acc_full = empty + kStages;
     uint64_t* acc_empty = acc_full + 2;
@@ -279,11 +328,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         const uint32_t leader_empty0 = mapa_shared(&acc_empty[0], 0);
         const uint32_t leader_empty1 = mapa_shared(&acc_empty[1], 0);
+        uint8_t* turn = turns + (warp - 2) * kTurnBytes[EPI];
+        uint8_t *turn_g = turn + kBlock16, *turn_u = turn_g + kBlock32;  // dh's epilogue
         int n = 0;
         for (int u = pair; u < units; u += npairs, ++n) {
             const Unit w = unit_of<EPI>(args, u);
             const PairProblem& p = *w.p;
-            const int64_t row = w.m0 + 128 * static_cast<int>(rank) + q * 32 + lane;
+            const int64_t row0 = w.m0 + 128 * static_cast<int>(rank) + q * 32;
+            const int rows = static_cast<int>(min(p.M - row0, static_cast<int64_t>(32)));
+            // columns of the output this warp covers
+            const int span = EPI == kFfGated ? w.width / 4 : w.width / 2;
+            const int begin = half * span, end = begin + span;
+            auto fetch = [&](int c0) {
+                // a block that lies outside altogether is not even addressed
+                const int cols = min(p.N - w.n0 - c0, 32);
+                const int64_t pre = rows > 0 && cols > 0 ? row0 * p.N + w.n0 + c0 : 0;
+                fetch_block(p.pre_g + pre, p.N, rows, cols, p.vec_pre, turn_g, lane);
+                fetch_block(p.pre_u + pre, p.N, rows, cols, p.vec_pre, turn_u, lane);
+            };
+            if (EPI == kFfSlope) fetch(begin);  // on its way while the sums finish
             const int buf = n & 1;
             const bool got = mbar_wait_bounded(&acc_full[buf], (n >> 1) & 1, args.status,
                                                kErrFfEpilogue);
@@ -291,55 +354,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after();
             const uint32_t d = lane_base + buf * 256;
-            // columns of the output this warp covers
-            const int span = EPI == kFfGated ? w.width / 4 : w.width / 2;
-            for (int c0 = half * span; c0 < (half + 1) * span; c0 += 32) {
-                uint32_t r[32];
-                float v[32];
+            for (int c0 = begin; c0 < end; c0 += 32) {
+                uint32_t r[32], o[16];
                 tmem_ld_32x32b_x32(d + c0, r);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                const int col = w.n0 + c0, cols = p.N - col;
-                const bool in = row < p.M && cols > 0;
-                const int64_t at = row * p.ldc + col, pre = row * p.N + col;
+                const int col = w.n0 + c0, cols = min(p.N - col, 32);
+                const int64_t at = row0 * p.ldc + col, pre = row0 * p.N + col;
                 T* c = static_cast<T*>(p.c) + at;
-                if (EPI == kFfStore && in) store32<T>(c, v, cols, p.vec_c);
-                if (EPI == kFfGated) {
-                    tmem_ld_32x32b_x32(d + w.width / 2 + c0, r);
-                    if (in) {
-                        float x[32];
-                        if (p.pre_g) {
+                auto f = [](uint32_t x) { return __uint_as_float(x); };
+                if (EPI == kFfStore) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
-                            store32<float>(p.pre_g + pre, v, cols, p.vec_pre);
-                            store32<float>(p.pre_u + pre, x, cols, p.vec_pre);
+                    for (int i = 0; i < 16; ++i) o[i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
+                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                }
+                if (EPI == kFfGated) {
+                    uint32_t x[32];
+                    tmem_ld_32x32b_x32(d + w.width / 2 + c0, x);
+                    if (p.pre_g) {
+                        store_block<float>(p.pre_g + pre, p.N, rows, cols, p.vec_pre, r, turn, lane);
+                        store_block<float>(p.pre_u + pre, p.N, rows, cols, p.vec_pre, x, turn, lane);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[i] = pair16<T>(activate<ACT, true>(f(r[2 * i])).a * f(x[2 * i]),
+                                         activate<ACT, true>(f(r[2 * i + 1])).a * f(x[2 * i + 1]));
+                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                }
+                if (EPI == kFfSlope) {
+                    uint32_t ou[16], oh[16];
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float4 g4 =
+                            *reinterpret_cast<const float4*>(turn_g + lane * kPitch<float> + i * 8);
+                        const float4 u4 =
+                            *reinterpret_cast<const float4*>(turn_u + lane * kPitch<float> + i * 8);
+                        const float g[4] = {g4.x, g4.y, g4.z, g4.w};
+                        const float x[4] = {u4.x, u4.y, u4.z, u4.w};
+                        float dg[4], du[4], h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const ActValue a = activate<ACT, true>(g[e]);
+                            const float dh = f(r[2 * i + e]);
+                            dg[e] = dh * x[e] * a.slope;
+                            du[e] = dh * a.a;
+                            h[e] = a.a * x[e];
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            v[i] = activate<ACT, true>(v[i]).a * __uint_as_float(r[i]);
-                        store32<T>(c, v, cols, p.vec_c);
+                        for (int e = 0; e < 2; ++e) {
+                            o[i + e] = pair16<T>(dg[2 * e], dg[2 * e + 1]);
+                            ou[i + e] = pair16<T>(du[2 * e], du[2 * e + 1]);
+                            oh[i + e] = pair16<T>(h[2 * e], h[2 * e + 1]);
+                        }
                     }
-                }
-                if (EPI == kFfSlope && in) {
-                    float g[32], x[32];
-                    load32(p.pre_g + pre, g, cols, p.vec_pre);
-                    load32(p.pre_u + pre, x, cols, p.vec_pre);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const ActValue a = activate<ACT, true>(g[i]);
-                        g[i] = v[i] * x[i] * a.slope;
-                        v[i] = v[i] * a.a;
-                        x[i] = a.a * x[i];
-                    }
-                    store32<T>(c, g, cols, p.vec_c);
-                    store32<T>(static_cast<T*>(p.c2) + at, v, cols, p.vec_c);
-                    store32<T>(static_cast<T*>(p.c3) + at, x, cols, p.vec_c);
+                    __syncwarp();
+                    if (c0 + 32 < end) fetch(c0 + 32);  // while this block is stored
+                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                    store_block<T>(static_cast<T*>(p.c2) + at, p.ldc, rows, cols, p.vec_c, ou, turn,
+                                   lane);
+                    store_block<T>(static_cast<T*>(p.c3) + at, p.ldc, rows, cols, p.vec_c, oh, turn,
+                                   lane);
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(buf ? leader_empty1 : leader_empty0);
         }
+        if (EPI == kFfSlope) asm volatile("cp.async.wait_all;" ::: "memory");  // gave up early
     }
 
     tc_fence_before();
@@ -373,11 +454,13 @@ int launch(const PairArgs& args, int units, cudaStream_t s) {
     const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
     if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(ff_pair_kernel<EPI, ACT, T>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 smem_bytes(EPI));
         if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     }
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
-    ff_pair_kernel<EPI, ACT, T><<<2 * std::min(units, sm_pairs()), kThreads, kSmemBytes, s>>>(args);
+    ff_pair_kernel<EPI, ACT, T><<<2 * std::min(units, sm_pairs()), kThreads, smem_bytes(EPI), s>>>(
+        args);
     return cuda_status(cudaGetLastError(), "gated_ff");
 }
 

@@ -8,6 +8,7 @@
 #include <initializer_list>
 
 #include "gated_ff.cuh"
+#include "zg_gemm_internal.h"
 
 namespace zg {
 namespace {
@@ -222,6 +223,147 @@ int place_inputs(const FfCall& c, const FfLayout& l, uint8_t* ws, const void* co
     return cuda_status(cudaGetLastError(), "gated_ff padding");
 }
 
+// ---- f32 on the tensor cores -----------------------------------------------------
+// The split-precision GEMMs of sgemm_tc.cu on operand planes (k innermost), with
+// elementwise kernels between.  Every operand of the block becomes planes once per
+// pass: by rows where it lies along the sum, transposed where it does not.
+// dx's two products are one GEMM over [dg | du] and [Wg | Wu], each padded to whole
+// k blocks with zeros.
+
+bool f32_tensor(const FfCall& c) { return c.size == 4 && c.mode != ZG_GEMM_SIMT_FP32; }
+
+struct Planes {
+    FfCall c;
+    uint8_t* ws;        // null: only counts
+    uint64_t used = 0;
+    cudaStream_t s;
+    int rc = ZG_OK;
+
+    void* take(uint64_t bytes) {
+        void* p = ws ? ws + used : nullptr;
+        used += round_up(bytes, 256);
+        return p;
+    }
+    float* matrix(int rows, int cols) {
+        return static_cast<float*>(take(static_cast<uint64_t>(rows) * cols * 4));
+    }
+    // Planes of `rows` rows over k = K, from a [rows, K] matrix or the [K, rows] one
+    // whose transpose it is.
+    OperandView of(const float* src, int rows, int K, bool transposed) {
+        const OperandView v =
+            gemm_carve_planes(take(gemm_planes_bytes(c.mode, rows, K)), c.mode, rows, K);
+        if (ws && !rc)
+            rc = transposed ? gemm_prep_b(c.mode, K, rows, src, rows, v, s)
+                            : gemm_prep_rows(c.mode, rows, K, src, K, v, s);
+        return v;
+    }
+    // Two [rows, K] matrices side by side along k.
+    OperandView beside(const float* a, const float* b, int rows, int K) {
+        OperandView v = gemm_carve_planes(nullptr, c.mode, rows, K), w = v;
+        const int64_t one = v.ld;
+        v.ld *= 2;
+        v.p = take(static_cast<uint64_t>(rows) * v.ld * 4);
+        if (ws && !rc) rc = gemm_prep_rows(c.mode, rows, K, a, K, v, s);
+        w.ld = v.ld;
+        if (ws && !rc) {
+            w.p = static_cast<float*>(v.p) + one;
+            rc = gemm_prep_rows(c.mode, rows, K, b, K, w, s);
+        }
+        return v;
+    }
+    void gemm(const OperandView& a, const OperandView& b, int M, int N, int K, float* out) {
+        if (ws && !rc)
+            rc = gemm_run({c.mode, a, b}, M, N, K, 1.0f, out, N, nullptr, 0, s, nullptr, true);
+    }
+};
+
+// h = act(g) u; with dh: dg = dh u act'(g) (over dh), du = dh act(g), h.
+template <int ACT>
+__global__ void __launch_bounds__(256)
+    ff_act_kernel(const float* g, const float* u, float* h, int64_t n) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step)
+        h[i] = activate<ACT, false>(g[i]).a * u[i];
+}
+template <int ACT>
+__global__ void __launch_bounds__(256)
+    ff_slope_kernel(const float* g, const float* u, float* dh_dg, float* du, float* h, int64_t n) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
+        const ActValue a = activate<ACT, false>(g[i]);
+        const float x = dh_dg[i], y = u[i];
+        dh_dg[i] = x * y * a.slope;
+        du[i] = x * a.a;
+        h[i] = a.a * y;
+    }
+}
+
+unsigned stream_grid(int64_t n) {
+    return static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 148 * 16));
+}
+
+int launch_act(int act, const float* g, const float* u, float* h, int64_t n, cudaStream_t s) {
+    const unsigned grid = stream_grid(n);
+    switch (act) {
+        case ZG_ACT_SILU: ff_act_kernel<ZG_ACT_SILU><<<grid, 256, 0, s>>>(g, u, h, n); break;
+        case ZG_ACT_GELU: ff_act_kernel<ZG_ACT_GELU><<<grid, 256, 0, s>>>(g, u, h, n); break;
+        case ZG_ACT_GELU_TANH: ff_act_kernel<ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(g, u, h, n); break;
+        default: ff_act_kernel<ZG_ACT_RELU><<<grid, 256, 0, s>>>(g, u, h, n); break;
+    }
+    return cuda_status(cudaGetLastError(), "gated_ff activation");
+}
+
+int launch_slope(int act, const float* g, const float* u, float* dh, float* du, float* h,
+                 int64_t n, cudaStream_t s) {
+    const unsigned grid = stream_grid(n);
+    switch (act) {
+        case ZG_ACT_SILU: ff_slope_kernel<ZG_ACT_SILU><<<grid, 256, 0, s>>>(g, u, dh, du, h, n); break;
+        case ZG_ACT_GELU: ff_slope_kernel<ZG_ACT_GELU><<<grid, 256, 0, s>>>(g, u, dh, du, h, n); break;
+        case ZG_ACT_GELU_TANH: ff_slope_kernel<ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(g, u, dh, du, h, n); break;
+        default: ff_slope_kernel<ZG_ACT_RELU><<<grid, 256, 0, s>>>(g, u, dh, du, h, n); break;
+    }
+    return cuda_status(cudaGetLastError(), "gated_ff activation gradient");
+}
+
+struct F32Tensors {
+    const float *x, *wg, *wu, *wd, *dy;
+    float *pre_g, *pre_u, *y, *dx, *dwg, *dwu, *dwd;
+};
+
+// Runs the pass; with ws null only counts the workspace it takes.
+uint64_t f32_forward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s, int* rc) {
+    Planes p{c, ws, 0, s};
+    // counted without pre-activations given: the case that takes more
+    float* g = ws && t.pre_g ? t.pre_g : p.matrix(c.m, c.f);
+    float* u = ws && t.pre_g ? t.pre_u : p.matrix(c.m, c.f);
+    const OperandView x = p.of(t.x, c.m, c.k, false);
+    p.gemm(x, p.of(t.wg, c.f, c.k, true), c.m, c.f, c.k, g);
+    p.gemm(x, p.of(t.wu, c.f, c.k, true), c.m, c.f, c.k, u);
+    float* h = p.matrix(c.m, c.f);
+    if (ws && !p.rc) p.rc = launch_act(c.act, g, u, h, static_cast<int64_t>(c.m) * c.f, s);
+    const OperandView hp = p.of(h, c.m, c.f, false);
+    p.gemm(hp, p.of(t.wd, c.d, c.f, true), c.m, c.d, c.f, t.y);
+    *rc = p.rc;
+    return p.used;
+}
+
+uint64_t f32_backward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s, int* rc) {
+    Planes p{c, ws, 0, s};
+    float *dg = p.matrix(c.m, c.f), *du = p.matrix(c.m, c.f), *h = p.matrix(c.m, c.f);
+    p.gemm(p.of(t.dy, c.m, c.d, false), p.of(t.wd, c.f, c.d, false), c.m, c.f, c.d, dg);  // dh
+    if (ws && !p.rc)
+        p.rc = launch_slope(c.act, t.pre_g, t.pre_u, dg, du, h, static_cast<int64_t>(c.m) * c.f, s);
+    const OperandView dgu = p.beside(dg, du, c.m, c.f);
+    p.gemm(dgu, p.beside(t.wg, t.wu, c.k, c.f), c.m, c.k, 2 * gemm_planes_k(c.mode, c.f), t.dx);
+    const OperandView x = p.of(t.x, c.k, c.m, true);
+    p.gemm(x, p.of(dg, c.f, c.m, true), c.k, c.f, c.m, t.dwg);
+    p.gemm(x, p.of(du, c.f, c.m, true), c.k, c.f, c.m, t.dwu);
+    const OperandView ht = p.of(h, c.f, c.m, true);
+    p.gemm(ht, p.of(t.dy, c.d, c.m, true), c.f, c.d, c.m, t.dwd);
+    *rc = p.rc;
+    return p.used;
+}
+
 int check_call(FfCall& c, const char* what) {
     if (c.dtype != ZG_DTYPE_F32 && c.dtype != ZG_DTYPE_F16 && c.dtype != ZG_DTYPE_BF16)
         return set_error(ZG_ERR_DISPATCH, "%s: tensors are f32, bf16 or f16, got dtype %u", what,
@@ -237,8 +379,15 @@ int check_call(FfCall& c, const char* what) {
     return ZG_OK;
 }
 
+uint64_t ff_workspace(const FfCall& c) {
+    if (!f32_tensor(c)) return ff_layout(c).total;
+    int rc;
+    return c.backward ? f32_backward(c, {}, nullptr, nullptr, &rc)
+                      : f32_forward(c, {}, nullptr, nullptr, &rc);
+}
+
 int check_workspace(const FfCall& c, const void* ws, uint64_t bytes, const char* what) {
-    const uint64_t need = ff_layout(c).total;
+    const uint64_t need = ff_workspace(c);
     if (c.m > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
         return set_error(ZG_ERR_DISPATCH,
                          "%s: a 256-byte aligned workspace of %llu bytes is needed, got %llu", what,
@@ -275,7 +424,7 @@ extern "C" uint64_t zg_gated_ff_workspace_bytes(uint32_t dtype, int mode, int m,
                                                 int d, int backward) {
     FfCall c{dtype, mode, ZG_ACT_SILU, m, k, f, d, 0, backward != 0};
     if (check_call(c, "gated_ff") != ZG_OK || m == 0) return 0;
-    return ff_layout(c).total;
+    return ff_workspace(c);
 }
 
 extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
@@ -291,8 +440,16 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
         return set_error(ZG_ERR_DISPATCH,
                          "gated_ff: pre_gate and pre_up are both null or both 16-byte aligned");
     if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff"))) return rc;
-    const FfLayout l = ff_layout(c);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (f32_tensor(c)) {
+        F32Tensors t{};
+        t.x = static_cast<const float*>(x), t.wg = static_cast<const float*>(w_gate);
+        t.wu = static_cast<const float*>(w_up), t.wd = static_cast<const float*>(w_down);
+        t.pre_g = pre_gate, t.pre_u = pre_up, t.y = static_cast<float*>(y);
+        f32_forward(c, t, static_cast<uint8_t*>(workspace), s, &rc);
+        return rc;
+    }
+    const FfLayout l = ff_layout(c);
     const void* src[kInputs] = {x, w_gate, w_up, w_down, nullptr};
     FfInput in[kInputs];
     if ((rc = place_inputs(c, l, static_cast<uint8_t*>(workspace), src, in, s))) return rc;
@@ -334,8 +491,19 @@ extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, in
                              "gated_ff_backward")))
         return rc;
     if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff_backward"))) return rc;
-    const FfLayout l = ff_layout(c);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (f32_tensor(c)) {
+        F32Tensors t{};
+        t.x = static_cast<const float*>(x), t.wg = static_cast<const float*>(w_gate);
+        t.wu = static_cast<const float*>(w_up), t.wd = static_cast<const float*>(w_down);
+        t.dy = static_cast<const float*>(dy);
+        t.pre_g = const_cast<float*>(pre_gate), t.pre_u = const_cast<float*>(pre_up);
+        t.dx = static_cast<float*>(dx), t.dwg = static_cast<float*>(dw_gate);
+        t.dwu = static_cast<float*>(dw_up), t.dwd = static_cast<float*>(dw_down);
+        f32_backward(c, t, ws, s, &rc);
+        return rc;
+    }
+    const FfLayout l = ff_layout(c);
     void *h = ws, *dg = ws + l.plane, *du = ws + 2 * l.plane;
     const void* src[kInputs] = {x, w_gate, w_up, w_down, dy};
     FfInput in[kInputs];

@@ -49,6 +49,12 @@ OperandView gemm_raw_operand(const float* x, int64_t ld);
 // Pre-pass of A (M x K, pitch lda) into `out` (carved for mode, M, K).
 int gemm_prep_a(int mode, int M, int K, const float* A, int64_t lda, const OperandView& out,
                 cudaStream_t s);
+// The same without gemm_a_needs_planes' shortcut: rows x K, pitch lds, into
+// planes in every tensor-core mode.  gemm_planes_k: the k values a row of planes
+// holds (those from K on are zero).
+int gemm_prep_rows(int mode, int rows, int K, const float* src, int64_t lds,
+                   const OperandView& out, cudaStream_t s);
+int gemm_planes_k(int mode, int K);
 // Pre-pass of B (K x N, pitch ldb) into B^T form (carved for mode, N, K).
 int gemm_prep_b(int mode, int K, int N, const float* B, int64_t ldb, const OperandView& out,
                 cudaStream_t s);
@@ -74,7 +80,9 @@ struct GemmGate {
 
 // C[M x N, pitch ldc] = epilogue(alpha * A @ B) on prepared operands; `gate`
 // (tensor-core modes only) holds back B loads until their chunk has arrived.
+// `fine`: TF32X3 drains its accumulators every 64 of k instead of every 512.
 int gemm_run(const GemmOperands& op, int M, int N, int K, float alpha, float* C, int64_t ldc,
-             const float* bias, int relu, cudaStream_t s, const GemmGate* gate = nullptr);
+             const float* bias, int relu, cudaStream_t s, const GemmGate* gate = nullptr,
+             bool fine = false);
 
 }  // namespace zg

@@ -460,13 +460,14 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
     p.b[1] = {in[kWu].p, in[kWu].ld, true};
     p.c = workspace, p.ldc = l.ld_f;
     p.pre_g = pre_gate, p.pre_u = pre_up;
-    if ((rc = products(c, kFfGated, &p, 1, s))) return rc;
+    const bool few = c.size == 2 && m <= kFfRows;
+    if ((rc = few ? ff_rows(dtype, true, act, p, s) : products(c, kFfGated, &p, 1, s))) return rc;
     FfProduct q;  // y
     q.M = m, q.N = d, q.k[0] = f;
     q.a[0] = {workspace, l.ld_f, false};
     q.b[0] = {in[kWd].p, in[kWd].ld, true};
     q.c = y, q.ldc = d;
-    return products(c, kFfStore, &q, 1, s);
+    return few ? ff_rows(dtype, false, act, q, s) : products(c, kFfStore, &q, 1, s);
 }
 
 extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,

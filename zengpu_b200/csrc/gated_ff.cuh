@@ -106,4 +106,10 @@ int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStr
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
             cudaStream_t s);
 
+// The forward products for up to kFfRows rows of 16-bit tensors (gated_ff_rows.cu):
+// `gated` as kFfGated, else as kFfStore of one product, launched right behind the
+// gated one whose result it reads.
+constexpr int kFfRows = 128;
+int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& product, cudaStream_t s);
+
 }  // namespace zg

@@ -1,0 +1,344 @@
+// gated_ff_rows.cu - the forward products of the gated feed-forward block for few
+// rows (tokens being decoded), 16-bit tensors: every weight is read once, and the
+// time is that of reading them.
+//
+// The weights take the MMA's M side: D^T[128 columns of W x rows of x] = W^T x^T, so
+// a tile wastes nothing on missing rows: the MMA's N is the rows rounded up to
+// 16, 32, 64 or 128.  W is read as it lies (mn-major, see gated_ff_tc.cu), x or h as
+// the k-major B operand.  The gated product holds two accumulators, of Wg and Wu.
+//
+// A CTA takes 128 columns and a part of the sum; the CTAs of a cluster share the
+// columns and split the sum, then add their partial results through distributed
+// shared memory, in rank order, so the result does not depend on timing.  Each CTA
+// finishes the rows r with r % cluster size == its rank.
+//
+// Bound by HBM: what counts is bytes in flight, a ring of 64-of-the-sum stages (32 KB
+// of weights for the gated pair, 16 KB for Wd) of about 100 KB per CTA, two CTAs to
+// an SM.  y's kernel is launched while h's still runs (programmatic dependent
+// launch): it fills its ring with Wd, which nobody writes meanwhile, before it waits
+// for h.
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+#include <cstring>
+#include <type_traits>
+
+#include "gated_ff.cuh"
+#include "zg_gemm_internal.h"
+
+namespace zg {
+namespace {
+
+constexpr int kRowsThreads = 192;  // TMA, MMA, four epilogue warps
+constexpr int kRowsMaxStages = 12;
+constexpr int kSumStep = 64;
+constexpr int kColumns = 128;  // of W per CTA
+constexpr int kWeightBytes = kColumns * kSumStep * 2;
+
+struct alignas(64) RowsArgs {
+    CUtensorMap w[2], x;
+    void* c;
+    float* pre_g;
+    float* pre_u;
+    int64_t ldc;
+    int M, N, nkb, stages;
+    uint32_t* status;
+};
+
+__device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t lbo) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
+           (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+           (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ float ld_cluster_f32(const float* mine, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(mine, rank)));
+    return v;
+}
+
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+        " {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__host__ __device__ constexpr uint32_t tmem_columns(int n) {
+    return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
+}
+
+// GATED: c = act(x Wg) * (x Wu), and the two products to pre_g, pre_u unless null.
+// Otherwise c = x W.  ROWS: the MMA's N.
+template <bool GATED, int ACT, class T, int ROWS>
+__global__ void __launch_bounds__(kRowsThreads)
+    ff_rows_kernel(const __grid_constant__ RowsArgs args) {
+    constexpr int kMats = GATED ? 2 : 1;
+    constexpr int kStage = kMats * kWeightBytes + ROWS * 128;
+    constexpr uint32_t kCols = tmem_columns(kMats * ROWS);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~uintptr_t(1023));
+    __shared__ uint64_t full[kRowsMaxStages], empty[kRowsMaxStages], acc_full, drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stages = args.stages;
+    const int split = gridDim.x, rank = blockIdx.x;  // the grid's x is the cluster
+    const int n0 = blockIdx.y * kColumns;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(args.nkb) * rank / split);
+    const int kb1 = static_cast<int>(static_cast<int64_t>(args.nkb) * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&acc_full, 1);
+        mbar_init(&drain, 1);
+        failed = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_slot, kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    // after the allocation: a dependent CTA must not hold TMEM that this grid waits for
+    if (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto weights = [&](int kb) {
+                const int s = (kb - kb0) % stages;
+                uint8_t* st = smem + s * kStage;
+                mbar_arrive_expect_tx(&full[s], kStage);
+                for (int w = 0; w < kMats; ++w)
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_2d(st + w * kWeightBytes + h * (kWeightBytes / 2), &args.w[w],
+                                    n0 + 64 * h, kb * kSumStep, &full[s]);
+            };
+            auto rows = [&](int kb) {
+                const int s = (kb - kb0) % stages;
+                tma_load_2d(smem + s * kStage + kMats * kWeightBytes, &args.x, kb * kSumStep, 0,
+                            &full[s]);
+            };
+            int issued = kb0;
+            const int ahead = min(kb1, kb0 + stages);
+            for (; issued < ahead; ++issued) weights(issued);
+            // x or h may still be in the making by the kernel before
+            if (!GATED)
+                asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
+            for (int kb = kb0; kb < ahead; ++kb) rows(kb);
+            for (; issued < kb1; ++issued) {
+                const int it = issued - kb0;
+                if (!mbar_wait_bounded(&empty[it % stages], ((it / stages) & 1) ^ 1, args.status,
+                                       kErrFfProducer))
+                    break;
+                weights(issued);
+                rows(issued);
+            }
+            // no copy may still be landing when the ring is reused or the CTA ends
+            const int n = issued - kb0;
+            for (int i = max(0, n - stages); i < n; ++i)
+                mbar_wait_bounded(&full[i % stages], (i / stages) & 1, args.status, kErrFfDrain);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) |
+                                       (static_cast<uint32_t>(ROWS >> 3) << 17) | (8u << 24);
+            bool ok = true;
+            for (int kb = kb0; kb < kb1 && ok; ++kb) {
+                const int it = kb - kb0, s = it % stages;
+                if (!mbar_wait_bounded(&full[s], (it / stages) & 1, args.status, kErrFfMma)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t st = smem_u32(smem + s * kStage);
+#pragma unroll
+                for (int i = 0; i < kSumStep / 16; ++i)
+#pragma unroll
+                    for (int w = 0; w < kMats; ++w)
+                        mma_f16_ss(tmem + w * ROWS,
+                                   rows_desc(st + w * kWeightBytes + i * 2048, kWeightBytes / 2),
+                                   rows_desc(st + kMats * kWeightBytes + i * 32, 16), idesc,
+                                   (it | i) != 0);
+                mma_commit(&empty[s]);
+            }
+            if (ok) {
+                mma_commit(&acc_full);
+            } else {
+                mma_commit(&drain);
+                mbar_wait_bounded(&drain, 0, args.status, kErrFfDrain);
+            }
+        }
+    }
+
+    // ---------------- results ----------------
+    const int q = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const int column = q * 32 + lane, col = n0 + column;
+    auto finish = [&](int row, float g, float u) {
+        if (col >= args.N || row >= args.M) return;
+        T* c = static_cast<T*>(args.c) + row * args.ldc + col;
+        if (GATED) {
+            if (args.pre_g) {
+                const int64_t pre = static_cast<int64_t>(row) * args.N + col;
+                args.pre_g[pre] = g;
+                args.pre_u[pre] = u;
+            }
+            *c = FfElem<T>::put(activate<ACT, true>(g).a * u);
+        } else {
+            *c = FfElem<T>::put(g);
+        }
+    };
+    bool ok = true;
+    if (warp >= 2) {
+        ok = mbar_wait_bounded(&acc_full, 0, args.status, kErrFfEpilogue);
+        ok = __all_sync(0xffffffffu, ok);  // the TMEM loads are warp-collective
+        tc_fence_after();
+        if (ok && split == 1) {
+#pragma unroll
+            for (int r0 = 0; r0 < ROWS; r0 += 16) {
+                if (r0 >= args.M) break;
+                uint32_t g[16], u[16];
+                tmem_ld_16(lanes + r0, g);
+                if (GATED) tmem_ld_16(lanes + ROWS + r0, u);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    finish(r0 + i, __uint_as_float(g[i]), GATED ? __uint_as_float(u[i]) : 0.0f);
+            }
+        }
+    }
+    if (split > 1) {
+        // The ring is free: every copy has landed (the producer waited) and every MMA
+        // has read it (acc_full).  Its memory takes the partial results.
+        float* part = reinterpret_cast<float*>(smem);
+        if (warp >= 2 && ok) {
+#pragma unroll
+            for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                for (int r0 = 0; r0 < ROWS; r0 += 16) {
+                    if (r0 >= args.M) break;
+                    uint32_t v[16];
+                    tmem_ld_16(lanes + w * ROWS + r0, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        part[(w * ROWS + r0 + i) * kColumns + column] = __uint_as_float(v[i]);
+                }
+        }
+        if (warp >= 2 && !ok) failed = 1;
+        cluster_sync();
+        if (warp >= 2) {
+            bool all = true;
+            for (int p = 0; p < split; ++p)
+                all = all && __float_as_uint(ld_cluster_f32(
+                                 reinterpret_cast<const float*>(&failed), p)) == 0;
+            for (int row = rank; row < args.M && all; row += split) {
+                float g = 0.0f, u = 0.0f;
+                for (int p = 0; p < split; ++p) {
+                    g += ld_cluster_f32(part + row * kColumns + column, p);
+                    if (GATED) u += ld_cluster_f32(part + (ROWS + row) * kColumns + column, p);
+                }
+                finish(row, g, u);
+            }
+        }
+        cluster_sync();  // nobody leaves while its memory is read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kCols);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+int rows_sms() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms > 0 ? sms : 148;
+}
+
+template <bool GATED, int ACT, class T, int ROWS>
+int launch_rows(RowsArgs& args, cudaStream_t s) {
+    constexpr int kStage = (GATED ? 2 : 1) * kWeightBytes + ROWS * 128;
+    constexpr int kRing = 104 * 1024;  // two CTAs to an SM
+    constexpr int kPart = (GATED ? 2 : 1) * ROWS * kColumns * 4;
+    const int tiles = (args.N + kColumns - 1) / kColumns;
+    int split = 1;
+    while (split < 8 && 2 * split * tiles <= 2 * rows_sms() && 2 * split <= args.nkb) split *= 2;
+    const int per = (args.nkb + split - 1) / split;
+    args.stages = std::min(std::min(std::max(kRing / kStage, 2), kRowsMaxStages), per);
+    // at least half an SM's shared memory each, so that no third CTA waits for TMEM
+    const int smem = std::max(std::max(args.stages * kStage, split > 1 ? kPart : 0), kRing) + 1024;
+    auto kernel = ff_rows_kernel<GATED, ACT, T, ROWS>;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    }
+    if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, tiles);
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = GATED ? 1 : 2;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args), "gated_ff rows");
+}
+
+template <bool GATED, int ACT, class T>
+int launch_rows_n(RowsArgs& a, cudaStream_t s) {
+    if (a.M <= 16) return launch_rows<GATED, ACT, T, 16>(a, s);
+    if (a.M <= 32) return launch_rows<GATED, ACT, T, 32>(a, s);
+    if (a.M <= 64) return launch_rows<GATED, ACT, T, 64>(a, s);
+    return launch_rows<GATED, ACT, T, 128>(a, s);
+}
+
+template <class T>
+int launch_rows_act(bool gated, int act, RowsArgs& a, cudaStream_t s) {
+    if (!gated) return launch_rows_n<false, ZG_ACT_RELU, T>(a, s);
+    switch (act) {
+        case ZG_ACT_SILU: return launch_rows_n<true, ZG_ACT_SILU, T>(a, s);
+        case ZG_ACT_GELU: return launch_rows_n<true, ZG_ACT_GELU, T>(a, s);
+        case ZG_ACT_GELU_TANH: return launch_rows_n<true, ZG_ACT_GELU_TANH, T>(a, s);
+        default: return launch_rows_n<true, ZG_ACT_RELU, T>(a, s);
+    }
+}
+
+}  // namespace
+
+int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& f, cudaStream_t s) {
+    RowsArgs args;
+    std::memset(&args, 0, sizeof(args));
+    args.c = f.c, args.ldc = f.ldc, args.pre_g = f.pre_g, args.pre_u = f.pre_u;
+    args.M = f.M, args.N = f.N, args.nkb = (f.k[0] + kSumStep - 1) / kSumStep;
+    const int rows = f.M <= 16 ? 16 : f.M <= 32 ? 32 : f.M <= 64 ? 64 : 128;
+    int rc = status_word(&args.status);
+    for (int w = 0; w < (gated ? 2 : 1) && !rc; ++w)
+        rc = encode_16bit_map(&args.w[w], dtype, f.b[w].p, f.N, f.k[0], f.b[w].ld, 64, kSumStep);
+    if (!rc) rc = encode_16bit_map(&args.x, dtype, f.a[0].p, f.k[0], f.M, f.a[0].ld, 64, rows);
+    if (rc) return rc;
+    return dtype == ZG_DTYPE_BF16 ? launch_rows_act<__nv_bfloat16>(gated, act, args, s)
+                                  : launch_rows_act<__half>(gated, act, args, s);
+}
+
+}  // namespace zg

@@ -51,9 +51,14 @@ __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t lbo) {
            (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-__device__ __forceinline__ float ld_cluster_f32(const float* mine, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(mine, rank)));
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t mine, uint32_t rank) {
+    float4 v;
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(mine), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
     return v;
 }
 
@@ -86,7 +91,6 @@ __global__ void __launch_bounds__(kRowsThreads)
                                                ~uintptr_t(1023));
     __shared__ uint64_t full[kRowsMaxStages], empty[kRowsMaxStages], acc_full, drain;
     __shared__ uint32_t tmem_slot;
-    __shared__ uint32_t failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int stages = args.stages;
     const int split = gridDim.x, rank = blockIdx.x;  // the grid's x is the cluster
@@ -101,8 +105,12 @@ __global__ void __launch_bounds__(kRowsThreads)
         }
         mbar_init(&acc_full, 1);
         mbar_init(&drain, 1);
-        failed = 0;
         fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tensormap(&args.w[0]);
+        if (GATED) prefetch_tensormap(&args.w[1]);
+        prefetch_tensormap(&args.x);
     }
     if (warp == 1) tmem_alloc(&tmem_slot, kCols);
     tc_fence_before();
@@ -184,8 +192,8 @@ __global__ void __launch_bounds__(kRowsThreads)
     // ---------------- results ----------------
     const int q = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    const int column = q * 32 + lane, col = n0 + column;
-    auto finish = [&](int row, float g, float u) {
+    const int column = q * 32 + lane;
+    auto finish = [&](int row, int col, float g, float u) {
         if (col >= args.N || row >= args.M) return;
         T* c = static_cast<T*>(args.c) + row * args.ldc + col;
         if (GATED) {
@@ -213,7 +221,8 @@ __global__ void __launch_bounds__(kRowsThreads)
                 if (GATED) tmem_ld_16(lanes + ROWS + r0, u);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    finish(r0 + i, __uint_as_float(g[i]), GATED ? __uint_as_float(u[i]) : 0.0f);
+                    finish(r0 + i, n0 + column, __uint_as_float(g[i]),
+                           GATED ? __uint_as_float(u[i]) : 0.0f);
             }
         }
     }
@@ -234,20 +243,27 @@ __global__ void __launch_bounds__(kRowsThreads)
                         part[(w * ROWS + r0 + i) * kColumns + column] = __uint_as_float(v[i]);
                 }
         }
-        if (warp >= 2 && !ok) failed = 1;
         cluster_sync();
         if (warp >= 2) {
-            bool all = true;
-            for (int p = 0; p < split; ++p)
-                all = all && __float_as_uint(ld_cluster_f32(
-                                 reinterpret_cast<const float*>(&failed), p)) == 0;
-            for (int row = rank; row < args.M && all; row += split) {
-                float g = 0.0f, u = 0.0f;
+            // a warp to a row, four columns to a lane; one rank's loads of a row (and
+            // of both products) are in flight together.  After an expired wait the
+            // sums mean nothing, as the status word says, but are in bounds.
+            const uint32_t at = smem_u32(part) + lane * 16;
+            for (int row = rank + split * (warp - 2); row < args.M; row += split * 4) {
+                float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f), u = g;
+#pragma unroll 4
                 for (int p = 0; p < split; ++p) {
-                    g += ld_cluster_f32(part + row * kColumns + column, p);
-                    if (GATED) u += ld_cluster_f32(part + (ROWS + row) * kColumns + column, p);
+                    const float4 x = ld_cluster_f32x4(at + row * (kColumns * 4), p);
+                    g.x += x.x, g.y += x.y, g.z += x.z, g.w += x.w;
+                    if (GATED) {
+                        const float4 z = ld_cluster_f32x4(at + (ROWS + row) * (kColumns * 4), p);
+                        u.x += z.x, u.y += z.y, u.z += z.z, u.w += z.w;
+                    }
                 }
-                finish(row, g, u);
+                finish(row, n0 + lane * 4, g.x, u.x);
+                finish(row, n0 + lane * 4 + 1, g.y, u.y);
+                finish(row, n0 + lane * 4 + 2, g.z, u.z);
+                finish(row, n0 + lane * 4 + 3, g.w, u.w);
             }
         }
         cluster_sync();  // nobody leaves while its memory is read

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from typing import Sequence
 
 import torch
@@ -215,41 +216,64 @@ def sgemm_packed(pa: Packed, pb: Packed, c: torch.Tensor | None = None, alpha: f
 
 
 # ---- gated feed-forward block (zg_gated_ff, zg_gated_ff_backward) ----------------------
+_FLOATS = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.Bf16}
+
+
+def _on(index: int):
+    """Makes device `index` the current one for a call (free when it already is)."""
+    return contextlib.nullcontext() if index == torch._C._cuda_getDevice() \
+        else torch.cuda.device(index)
+
+
+def _raw_stream(index: int) -> int:
+    """_stream without the Stream object around it: a call of a few microseconds notices."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _scratch(index: int, stream: int, nbytes: int) -> torch.Tensor | None:
+    """workspace_for of a device and stream known by number.  A capture gets memory
+    of its own, which no other graph or stream shares."""
+    if nbytes == 0:
+        return None
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    ws = _workspaces.get((index, stream))
+    return ws if ws is not None and ws.numel() >= nbytes \
+        else workspace_for(torch.device("cuda", index), nbytes)
+
+
 def _ff_operand(name: str, t: torch.Tensor, shape: tuple[int, ...],
                 like: torch.Tensor) -> torch.Tensor:
-    if t.dtype != like.dtype or t.device != like.device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {like.dtype} tensor on {like.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype is not like.dtype or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {like.dtype} tensor on {like.device}")
     # the kernels' copies start on 16-byte boundaries; a view that does not is copied
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _ff_output(name: str, t: torch.Tensor | None, shape: tuple[int, ...],
                like: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
-    dtype = dtype or like.dtype
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if t.dtype != dtype or t.device != like.device or not t.is_contiguous() or \
-            tuple(t.shape) != shape:
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+    dtype = dtype or like.dtype
+    if t.dtype != dtype or t.device != like.device or not t.is_contiguous() or t.shape != shape:
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape}")
     return t
 
 
 def _ff_sizes(x: torch.Tensor, w_gate: torch.Tensor, w_down: torch.Tensor) -> tuple[int, ...]:
-    if x.device.type != "cuda" or x.dtype not in _FLOATS:
+    if not x.is_cuda or x.dtype not in _FLOATS:
         raise ValueError("gated_ff: expected f32, bf16 or f16 CUDA tensors")
     if x.dim() != 2 or w_gate.dim() != 2 or w_down.dim() != 2:
         raise ValueError("gated_ff: expected 2-D tensors")
-    return x.shape[0], x.shape[1], w_gate.shape[1], w_down.shape[1]
+    return *x.shape, w_gate.shape[1], w_down.shape[1]
 
 
-def _ff_workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
-    """The stream's scratch; a capture gets memory of its own, which no other
-    graph or stream shares."""
-    if nbytes and torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return workspace_for(device, nbytes)
+@functools.lru_cache(maxsize=1024)
+def _ff_workspace_bytes(dtype: int, mode: int, m: int, k: int, f: int, d: int,
+                        backward: int) -> int:
+    return int(L.load().zg_gated_ff_workspace_bytes(dtype, mode, m, k, f, d, backward))
 
 
 def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -261,21 +285,23 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: 
     returns (y, saved), `saved` being what gated_ff_backward needs: the two inner
     products before the activation, f32 [m, f] each."""
     m, k, f, d = _ff_sizes(x, w_gate, w_down)
-    with _on(x.device):
+    index, act, mode = x.get_device(), int(act), int(mode)
+    with _on(index):
         x = _ff_operand("x", x, (m, k), x)
         w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
         w_up = _ff_operand("w_up", w_up, (k, f), x)
         w_down = _ff_operand("w_down", w_down, (f, d), x)
         y = _ff_output("out", out, (m, d), x)
-        saved = tuple(_ff_output("saved", None, (m, f), x, torch.float32)
-                      for _ in range(2)) if save else ()
-        lib, dt = L.load(), _FLOATS[x.dtype]
-        need = int(lib.zg_gated_ff_workspace_bytes(dt, int(mode), m, k, f, d, 0))
-        ws = _ff_workspace(x.device, need)
-        check(lib.zg_gated_ff(dt, int(mode), int(act), m, k, f, d, x.data_ptr(), w_gate.data_ptr(),
-                              w_up.data_ptr(), w_down.data_ptr(), y.data_ptr(),
-                              *([t.data_ptr() for t in saved] or (None, None)),
-                              ws.data_ptr() if ws is not None else None, need, _stream(x)))
+        saved = (x.new_empty((m, f), dtype=torch.float32),
+                 x.new_empty((m, f), dtype=torch.float32)) if save else None
+        dt, stream = _FLOATS[x.dtype].value, _raw_stream(index)
+        need = _ff_workspace_bytes(dt, mode, m, k, f, d, 0)
+        ws = _scratch(index, stream, need)
+        check(L.load().zg_gated_ff(
+            dt, mode, act, m, k, f, d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+            w_down.data_ptr(), y.data_ptr(), saved[0].data_ptr() if save else None,
+            saved[1].data_ptr() if save else None, ws.data_ptr() if ws is not None else None, need,
+            stream))
     return (y, saved) if save else y
 
 
@@ -288,40 +314,32 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
     `saved` as gated_ff(..., save=True) gave it for the same x and weights.  `out`
     takes tensors to write them to."""
     m, k, f, d = _ff_sizes(x, w_gate, w_down)
-    with _on(x.device):
+    index, act, mode = x.get_device(), int(act), int(mode)
+    if len(saved) != 2 or any(t is None for t in saved):
+        raise ValueError("gated_ff_backward: saved has two tensors")
+    if len(out) != 4:
+        raise ValueError("gated_ff_backward: out has four places")
+    with _on(index):
         x = _ff_operand("x", x, (m, k), x)
         dy = _ff_operand("dy", dy, (m, d), x)
         w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
         w_up = _ff_operand("w_up", w_up, (k, f), x)
         w_down = _ff_operand("w_down", w_down, (f, d), x)
-        if len(saved) != 2 or any(t is None for t in saved):
-            raise ValueError("gated_ff_backward: saved has two tensors")
         pre = [_ff_output("saved", t, (m, f), x, torch.float32) for t in saved]
         pre = [t if t.data_ptr() % 16 == 0 else t.clone() for t in pre]
-        names = ("dx", "dw_gate", "dw_up", "dw_down")
-        got = tuple(_ff_output(n, t, s, x) for n, t, s in
-                    zip(names, out, ((m, k), (k, f), (k, f), (f, d)), strict=True))
-        lib, dt = L.load(), _FLOATS[x.dtype]
-        need = int(lib.zg_gated_ff_workspace_bytes(dt, int(mode), m, k, f, d, 1))
-        ws = _ff_workspace(x.device, need)
-        check(lib.zg_gated_ff_backward(
-            dt, int(mode), int(act), m, k, f, d, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+        got = (_ff_output("dx", out[0], (m, k), x), _ff_output("dw_gate", out[1], (k, f), x),
+               _ff_output("dw_up", out[2], (k, f), x), _ff_output("dw_down", out[3], (f, d), x))
+        dt, stream = _FLOATS[x.dtype].value, _raw_stream(index)
+        need = _ff_workspace_bytes(dt, mode, m, k, f, d, 1)
+        ws = _scratch(index, stream, need)
+        check(L.load().zg_gated_ff_backward(
+            dt, mode, act, m, k, f, d, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
             w_up.data_ptr(), w_down.data_ptr(), pre[0].data_ptr(), pre[1].data_ptr(),
-            *[t.data_ptr() for t in got], ws.data_ptr() if ws is not None else None, need,
-            _stream(x)))
+            *[t.data_ptr() for t in got], ws.data_ptr() if ws is not None else None, need, stream))
     return got
 
 
 # ---- AdamW over many tensors, gradient norm (zg_adamw, zg_grad_norm) -------------------
-_FLOATS = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.Bf16}
-
-
-def _on(device: torch.device):
-    """Makes `device` the current one for a call (free when it already is)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() \
-        else torch.cuda.device(device)
-
-
 def _same(name: str, tensors: Sequence[torch.Tensor], like: Sequence[int],
           device: torch.device, dtypes: Sequence[torch.dtype]) -> None:
     """Checks a list of contiguous CUDA tensors: one dtype out of `dtypes`, `like` elements each."""
@@ -336,10 +354,8 @@ def _same(name: str, tensors: Sequence[torch.Tensor], like: Sequence[int],
             raise ValueError(f"{name}: {t.numel()} elements, expected {n}")
 
 
-def _device_scalar(name: str, t: torch.Tensor | None, dtype: torch.dtype,
-                   device: torch.device) -> int | None:
-    if t is None:
-        return None
+def _device_scalar(name: str, t: torch.Tensor, dtype: torch.dtype,
+                   device: torch.device) -> int:
     if t.dtype != dtype or t.numel() != 1 or t.device != device:
         raise ValueError(f"{name}: expected one {dtype} on {device}")
     return t.data_ptr()
@@ -401,6 +417,7 @@ class AdamW:
                 raise ValueError("AdamW: tensors overlap")
             end, kind = (b, k) if b >= end else (end, kind | k)
         self._device = device
+        self._types = (_FLOATS[params[0].dtype].value, _FLOATS[grads[0].dtype].value)
         self._table = (L.AdamWTensor * len(params))()
         for i, row in enumerate(self._table):
             row.param, row.grad, row.n = params[i].data_ptr(), grads[i].data_ptr(), sizes[i]
@@ -416,18 +433,17 @@ class AdamW:
         grad_scale: a float32 device scalar the gradients are multiplied by, as
         GradNorm gives it; when it is not finite the step changes nothing."""
         device = self._device
-        step_dev = _device_scalar("AdamW step", step, torch.int64, device) \
-            if isinstance(step, torch.Tensor) else None
-        lr_dev = _device_scalar("AdamW lr", lr, torch.float32, device) \
-            if isinstance(lr, torch.Tensor) else None
-        hyper = L.AdamWHyper(0.0 if lr_dev else lr, beta1, beta2, eps, weight_decay,
-                             0 if step_dev else int(step))
-        with _on(device):
-            check(L.load().zg_adamw(
-                _FLOATS[self.params[0].dtype], _FLOATS[self.grads[0].dtype], self.state_bits,
-                len(self._table), self._table, C.byref(hyper), step_dev, lr_dev,
-                _device_scalar("AdamW grad_scale", grad_scale, torch.float32, device),
-                _stream(self.params[0])))
+        step_dev = lr_dev = scale_dev = None
+        if isinstance(step, torch.Tensor):
+            step_dev, step = _device_scalar("AdamW step", step, torch.int64, device), 0
+        if isinstance(lr, torch.Tensor):
+            lr_dev, lr = _device_scalar("AdamW lr", lr, torch.float32, device), 0.0
+        if grad_scale is not None:
+            scale_dev = _device_scalar("AdamW grad_scale", grad_scale, torch.float32, device)
+        hyper = L.AdamWHyper(lr, beta1, beta2, eps, weight_decay, step)
+        with _on(device.index):
+            check(L.load().zg_adamw(*self._types, self.state_bits, len(self._table), self._table,
+                                    hyper, step_dev, lr_dev, scale_dev, _raw_stream(device.index)))
 
 
 class GradNorm:
@@ -441,6 +457,7 @@ class GradNorm:
         self._device = grads[0].device
         _same("GradNorm", grads, [g.numel() for g in grads], self._device, tuple(_FLOATS))
         self.grads = list(grads)
+        self._type = _FLOATS[grads[0].dtype].value
         self._ptrs = (C.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
         self._sizes = (C.c_uint64 * len(grads))(*[g.numel() for g in grads])
         self._ws_bytes = int(L.load().zg_grad_norm_workspace_bytes(len(grads)))
@@ -448,10 +465,12 @@ class GradNorm:
     def clip_scale(self, max_norm: float) -> torch.Tensor:
         """[norm, min(1, max_norm / norm)] as two f32 on the device; the factor is
         NaN when the norm is not finite.  out[1:] is AdamW.step's grad_scale."""
-        with _on(self._device):
-            out = torch.empty(2, dtype=torch.float32, device=self._device)
-            ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self._device)
-            check(L.load().zg_grad_norm(_FLOATS[self.grads[0].dtype], len(self.grads), self._ptrs,
-                                        self._sizes, float(max_norm), out.data_ptr(),
-                                        ws.data_ptr(), self._ws_bytes, _stream(out)))
+        index = self._device.index
+        with _on(index):
+            stream = _raw_stream(index)
+            out = self.grads[0].new_empty(2, dtype=torch.float32)
+            ws = _scratch(index, stream, self._ws_bytes)
+            check(L.load().zg_grad_norm(self._type, len(self._sizes), self._ptrs, self._sizes,
+                                        max_norm, out.data_ptr(), ws.data_ptr(), self._ws_bytes,
+                                        stream))
         return out

@@ -34,6 +34,18 @@ def host(t):
     return t.view(torch.uint8).numpy() if t.dtype == torch.float8_e4m3fn else t.float().numpy()
 
 
+def check_weight(got, want, p0, steps, kind):
+    """With 8-bit moments a step's change of the weight is a quotient of approximate
+    instructions: the root within 2^-22 of itself, the reciprocal 2^-23, the product
+    2^-24, under 2^-21 of the change; the change is at most what the weight moved plus
+    decay (counted once more as slack).  Each step then rounds the weight to `kind`,
+    half a step (2^-24 of it for f32), and may round to the other neighbour."""
+    moved = np.abs(want - p0) + 1e-3 * np.abs(p0) + 1e-2
+    half = max(torch.finfo(kind).eps / 2, 2.0 ** -24)
+    bound = steps * (2.0 ** -21 * moved + 2 * half * np.abs(want))
+    assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
+
+
 class Case:
     """Tensors of `sizes` with moments as after some steps, on the GPU and as float32 copies."""
 
@@ -41,7 +53,7 @@ class Case:
         def on_gpu(x, dtype=None):  # `offset` elements past an aligned address
             t = cuda(np.concatenate([np.zeros(offset, x.dtype), x]), dtype)
             return t[offset:]
-        self.bits, self.kind = bits, TYPES[kind]
+        self.bits, self.kind, self.steps = bits, TYPES[kind], 0
         self.p0 = [normal(n, 10 + i, 0.05) for i, n in enumerate(sizes)]
         self.params = [on_gpu(p, TYPES[kind]) for p in self.p0]
         self.master = [on_gpu(p) for p in self.p0] if master else None
@@ -70,6 +82,7 @@ class Case:
     def follow(self, step, s=None):
         """One step of the restatement; 16-bit weights without a master are rounded."""
         new = []
+        self.steps += 1
         for (p, m, v, ms, vs), g in zip(self.ref, self.g0):
             p, m, v, ms, vs = R.step_f32(p, m, v, g, step, s=s, bits=self.bits, ms=ms, vs=vs, **REF)
             if self.master is None:
@@ -79,9 +92,19 @@ class Case:
 
     def check(self):
         for i, (p, m, v, ms, vs) in enumerate(self.ref):
-            if self.master is not None:
-                np.testing.assert_array_equal(host(self.master[i]), p)
-            np.testing.assert_array_equal(host(self.params[i]), host(torch.from_numpy(p).to(self.kind)))
+            w = self.master if self.master is not None else self.params
+            if self.bits == 8:
+                check_weight(host(w[i]), p, self.p0[i], self.steps,
+                             torch.float32 if self.master else self.kind)
+                # 16-bit weights beside a master are its rounding
+                if self.master is not None:
+                    np.testing.assert_array_equal(host(self.params[i]),
+                                                  host(self.master[i].to(self.kind)))
+            else:
+                if self.master is not None:
+                    np.testing.assert_array_equal(host(self.master[i]), p)
+                np.testing.assert_array_equal(host(self.params[i]),
+                                              host(torch.from_numpy(p).to(self.kind)))
             np.testing.assert_array_equal(host(self.state["exp_avg"][i]), m)
             np.testing.assert_array_equal(host(self.state["exp_avg_sq"][i]), v)
             if self.bits == 8:
@@ -235,7 +258,7 @@ def test_adamw_captured(bits):
         new = []
         for (p, m, v, ms, vs), g in zip(c.ref, c.g0):
             new.append(R.step_f32(p, m, v, g, t, s=0.5, bits=bits, ms=ms, vs=vs, **{**REF, "lr": lr64}))
-        c.ref = new
+        c.ref, c.steps = new, t
     torch.cuda.synchronize()
     c.check()
 

@@ -107,6 +107,7 @@ struct Factors {
     float step_size;       // lr / (1 - b1^t)
     float root;            // 1 / sqrt(1 - b2^t)
     float eps, decay;      // decay: 1 - lr wd
+    float one;             // 1
 };
 
 struct DeviceHyper {  // values a captured graph reads anew at each replay
@@ -145,62 +146,165 @@ __device__ __forceinline__ int tensor_of(const Table<CAP, Tensor>& tab, uint32_t
     return lo;
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    return x;
+// Two f32 in a register pair: Blackwell's packed f32 units round each half as the
+// scalar operations do, at half the instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack(F2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// a + b as a 1 + b.  The 1 is a value the compiler does not know: it contracts a
+// packed product and a packed sum into one rounding, .rn or not.
+__device__ __forceinline__ F2 add2(F2 a, F2 b, F2 one) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(one), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 both(float a) { return pack(a, a); }
+
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
 }
 
-// The scale of a block whose largest magnitude is `top` (finite), and its inverse.
-__device__ __forceinline__ float block_scale(float top, float& inv) {
-    if (!(top > 0.0f)) {
-        inv = 0.0f;
-        return 0.0f;
+template <class T>
+__device__ __forceinline__ F2 widen(const T (&x)[8], int i) {
+    return pack(Elem<T>::get(x[2 * i]), Elem<T>::get(x[2 * i + 1]));
+}
+// Eight codes of a lane as two words of four: one load of a word in the vector form.
+__device__ __forceinline__ void load_codes(const uint8_t* x, bool vec, int lane, int64_t left,
+                                           uint32_t (&w)[2]) {
+    if (vec) {
+        w[0] = *reinterpret_cast<const uint32_t*>(x + 4 * lane);
+        w[1] = *reinterpret_cast<const uint32_t*>(x + 128 + 4 * lane);
+    } else {
+        w[0] = w[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = 32 * i + lane;
+            if (e < left) w[i / 4] |= static_cast<uint32_t>(x[e]) << (i % 4 * 8);
+        }
     }
+}
+__device__ __forceinline__ void store_codes(uint8_t* x, bool vec, int lane, int64_t left,
+                                            const uint32_t (&w)[2]) {
+    if (vec) {
+        *reinterpret_cast<uint32_t*>(x + 4 * lane) = w[0];
+        *reinterpret_cast<uint32_t*>(x + 128 + 4 * lane) = w[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = 32 * i + lane;
+            if (e < left) x[e] = static_cast<uint8_t>(w[i / 4] >> (i % 4 * 8));
+        }
+    }
+}
+// Codes 2 i and 2 i + 1 of the eight.
+__device__ __forceinline__ F2 decode(const uint32_t (&w)[2], int i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+        static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    return pack(f.x, f.y);
+}
+__device__ __forceinline__ void encode(uint32_t (&w)[2], int i, float2 y) {
+    const uint32_t c = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+    w[i / 2] = i % 2 ? w[i / 2] | (c << 16) : c;
+}
+
+// The scale of a block whose largest magnitude is `top`, and its inverse.
+__device__ __forceinline__ float block_scale(float top, float& inv) {
+    inv = 0.0f;
+    if (!(top > 0.0f)) return top;  // zero, or NaN
     const float s = fmaxf(__fmul_rn(top, 1.0f / 448.0f), 0x1p-126f);
     inv = __frcp_rn(s);
+    return top < INFINITY ? s : __int_as_float(0x7fc00000);
+}
+
+__device__ __forceinline__ float warp_top(float top) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+
+// Eight m of a block as codes, and the block's scale.
+__device__ __forceinline__ float encode_m(const F2 (&m)[4], uint32_t (&codes)[2]) {
+    float top = 0.0f, inv;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack(m[i]);
+        top = max_nan(top, max_nan(f.x, f.y));
+    }
+    const float s = block_scale(warp_top(top), inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) encode(codes, i, unpack(mul2(m[i], both(inv))));
     return s;
 }
 
-struct E4M3 {
-    __device__ static float get(uint8_t c) {
-        return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-    }
-    __device__ static uint8_t put(float x) {
-        return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-    }
-};
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
-// Stores eight f32 of a block as codes with one scale; `floor_code`: values
-// above zero keep at least the smallest code.
-__device__ __forceinline__ void store_8bit(uint8_t* codes, float* scale, bool vec, int lane,
-                                           int64_t left, const float (&x)[8], float floor_code) {
-    float top = 0.0f;
-    bool finite = true;
+// Eight roots of a block as codes, from v and r, the roots to within three units of
+// the last place (sqrt.approx: one or two): codes are those of the correctly rounded
+// root.  The root of the largest v is taken exactly, and so is that of a value
+// whose quotient y by the scale lies within eight units of a point where e4m3's
+// rounding turns (the low 20 bits at one half), or among the subnormal codes.
+__device__ __forceinline__ float encode_root(const F2 (&v)[4], const F2 (&r)[4],
+                                             uint32_t (&codes)[2]) {
+    float top = 0.0f, inv;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        top = fmaxf(top, fabsf(x[i]));
-        finite = finite && isfinite(x[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack(v[i]);
+        top = max_nan(top, max_nan(f.x, f.y));
     }
-    top = warp_max(top);
-    finite = __all_sync(0xffffffffu, finite);
-    float inv, s = block_scale(top, inv);
-    uint8_t q[8];
+    const float s = block_scale(__fsqrt_rn(warp_top(top)), inv);
+    float2 y[4];
+    uint32_t close = 0xffffffffu;  // distance to the nearest turn, least of the eight
+    float low = 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float y = __fmul_rn(x[i], inv);
-        if (x[i] > 0.0f) y = fmaxf(y, floor_code);
-        q[i] = E4M3::put(y);
+    for (int i = 0; i < 4; ++i) {
+        y[i] = unpack(mul2(r[i], both(inv)));
+        low = fminf(low, fminf(y[i].x, y[i].y));
+        close = min(close, (__float_as_uint(y[i].x) - 0x7fff8u) << 12);
+        close = min(close, (__float_as_uint(y[i].y) - 0x7fff8u) << 12);
     }
-    if (!finite) s = __int_as_float(0x7fc00000);
-    if (lane == 0) *scale = s;
-    store8<uint8_t>(codes, vec, lane, left, q);
+    if (low < 0x1p-6f || close <= (16u << 12)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack(v[i]);
+            y[i].x = __fmul_rn(__fsqrt_rn(f.x), inv);
+            y[i].y = __fmul_rn(__fsqrt_rn(f.y), inv);
+            if (f.x > 0.0f) y[i].x = fmaxf(y[i].x, 0x1p-9f);
+            if (f.y > 0.0f) y[i].y = fmaxf(y[i].y, 0x1p-9f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) encode(codes, i, y[i]);
+    return s;
 }
 
 // What bounds it: HBM.  f32 weights, gradients and moments move 28 bytes per
-// element, 16-bit weights with a master and 8-bit moments 16.1.
+// element, 16-bit weights with a master and 8-bit moments 16.1; the latter are
+// as near to the issue rate: roots and quotients are then the approximate
+// instructions (a quotient is within 2 units of its last place, on a change of the
+// weight that is small beside it; the roots' codes are exact, see encode_root).
 template <class P, class G, int BITS, int CAP>
-__global__ void __launch_bounds__(kOptThreads)
+__global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
     adamw_kernel(const __grid_constant__ Table<CAP, zg_adamw_tensor> tab, int64_t chunk, Factors f,
                  const zg_adamw_hyper hyper, const DeviceHyper dev) {
     const int i = tensor_of(tab, blockIdx.x);
@@ -239,57 +343,75 @@ __global__ void __launch_bounds__(kOptThreads)
     for (int64_t b = begin + warp * kBlockElems; b < end; b += kTurnElems) {
         const int64_t left = end - b;
         const bool vec = aligned && left >= kBlockElems;
-        P pv[8];
         G gv[8];
-        float w[8], m[8], v[8];
+        P pv[8];
+        float wv[8], mv[8], vv[8];
+        uint32_t mc[2], vc[2];
+        float ms = 0.0f, vs = 0.0f;
         load8<G>(g + b, vec, lane, left, gv);
-        if (master) {
-            load8<float>(master + b, vec, lane, left, w);
-        } else {
-            load8<P>(p + b, vec, lane, left, pv);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = Elem<P>::get(pv[e]);
-        }
+        if (master) load8<float>(master + b, vec, lane, left, wv);
+        else load8<P>(p + b, vec, lane, left, pv);
         if (BITS == 32) {
-            load8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, m);
-            load8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, v);
+            load8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, mv);
+            load8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, vv);
         } else {
-            uint8_t mc[8], vc[8];
-            load8<uint8_t>(static_cast<uint8_t*>(t.exp_avg) + b, vec, lane, left, mc);
-            load8<uint8_t>(static_cast<uint8_t*>(t.exp_avg_sq) + b, vec, lane, left, vc);
-            const float ms = t.exp_avg_scale[b / kBlockElems];
-            const float vs = t.exp_avg_sq_scale[b / kBlockElems];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                m[e] = __fmul_rn(E4M3::get(mc[e]), ms);
-                const float r = __fmul_rn(E4M3::get(vc[e]), vs);
-                v[e] = __fmul_rn(r, r);
-            }
+            load_codes(static_cast<uint8_t*>(t.exp_avg) + b, vec, lane, left, mc);
+            load_codes(static_cast<uint8_t*>(t.exp_avg_sq) + b, vec, lane, left, vc);
+            ms = t.exp_avg_scale[b / kBlockElems];
+            vs = t.exp_avg_sq_scale[b / kBlockElems];
         }
-        float r[8];
+        F2 m[4], v[4], r[4], w[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float ge = __fmul_rn(Elem<G>::get(gv[e]), gscale);
-            m[e] = __fadd_rn(__fmul_rn(m[e], f.b1), __fmul_rn(ge, f.c1));
-            v[e] = __fadd_rn(__fmul_rn(v[e], f.b2), __fmul_rn(__fmul_rn(ge, f.c2), ge));
-            r[e] = __fsqrt_rn(v[e]);
-            const float den = __fadd_rn(__fmul_rn(r[e], f.root), f.eps);
-            w[e] = __fsub_rn(__fmul_rn(w[e], f.decay),
-                             __fdiv_rn(__fmul_rn(m[e], f.step_size), den));
-            pv[e] = Elem<P>::put(w[e]);
+        for (int e = 0; e < 4; ++e) {
+            const F2 ge = mul2(widen(gv, e), both(gscale));
+            if (BITS == 32) {
+                m[e] = widen(mv, e);
+                v[e] = widen(vv, e);
+            } else {
+                m[e] = mul2(decode(mc, e), both(ms));
+                v[e] = mul2(decode(vc, e), both(vs));
+                v[e] = mul2(v[e], v[e]);
+            }
+            m[e] = add2(mul2(m[e], both(f.b1)), mul2(ge, both(f.c1)), both(f.one));
+            v[e] = add2(mul2(v[e], both(f.b2)), mul2(mul2(ge, both(f.c2)), ge), both(f.one));
+            const float2 v2 = unpack(v[e]);
+            r[e] = BITS == 32 ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
+                              : pack(sqrt_approx(v2.x), sqrt_approx(v2.y));
+            const float2 den = unpack(add2(mul2(r[e], both(f.root)), both(f.eps), both(f.one)));
+            const float2 num = unpack(mul2(m[e], both(-f.step_size)));
+            const F2 quot = BITS == 32
+                                ? pack(__fdiv_rn(num.x, den.x), __fdiv_rn(num.y, den.y))
+                                : pack(__fdividef(num.x, den.x), __fdividef(num.y, den.y));
+            w[e] = add2(mul2(master ? widen(wv, e) : widen(pv, e), both(f.decay)), quot,
+                        both(f.one));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 w2 = unpack(w[e]);
+            wv[2 * e] = w2.x, wv[2 * e + 1] = w2.y;
+            pv[2 * e] = Elem<P>::put(w2.x), pv[2 * e + 1] = Elem<P>::put(w2.y);
         }
         store8<P>(p + b, vec, lane, left, pv);
-        if (master) store8<float>(master + b, vec, lane, left, w);
+        if (master) store8<float>(master + b, vec, lane, left, wv);
         if (BITS == 32) {
-            store8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, m);
-            store8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 m2 = unpack(m[e]), v2 = unpack(v[e]);
+                mv[2 * e] = m2.x, mv[2 * e + 1] = m2.y;
+                vv[2 * e] = v2.x, vv[2 * e + 1] = v2.y;
+            }
+            store8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, mv);
+            store8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, vv);
         } else {
-            // lanes past a tensor's end hold zeros, which change no block's maximum,
+            // elements past a tensor's end are zeros, which change no block's maximum,
             // except that 0 / (0 + eps) may be NaN: only w sees that, and is not stored
-            store_8bit(static_cast<uint8_t*>(t.exp_avg) + b, t.exp_avg_scale + b / kBlockElems,
-                       vec, lane, left, m, -448.0f);
-            store_8bit(static_cast<uint8_t*>(t.exp_avg_sq) + b,
-                       t.exp_avg_sq_scale + b / kBlockElems, vec, lane, left, r, 0x1p-9f);
+            const float new_ms = encode_m(m, mc), new_vs = encode_root(v, r, vc);
+            store_codes(static_cast<uint8_t*>(t.exp_avg) + b, vec, lane, left, mc);
+            store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + b, vec, lane, left, vc);
+            if (lane == 0) {
+                t.exp_avg_scale[b / kBlockElems] = new_ms;
+                t.exp_avg_sq_scale[b / kBlockElems] = new_vs;
+            }
         }
     }
 }
@@ -524,6 +646,7 @@ extern "C" int zg_adamw(uint32_t param_dtype, uint32_t grad_dtype, int state_bit
     c.f.b2 = static_cast<float>(h->beta2);
     c.f.c2 = static_cast<float>(1.0 - h->beta2);
     c.f.eps = static_cast<float>(h->eps);
+    c.f.one = 1.0f;
     schedule(c.f, lr_dev ? 0.0 : h->lr, h->beta1, h->beta2, h->weight_decay,
              step_dev ? 1.0 : static_cast<double>(h->step));
     c.chunk = chunk_elems(total);

@@ -184,6 +184,18 @@ template <class T>
 __device__ __forceinline__ F2 widen(const T (&x)[8], int i) {
     return pack(Elem<T>::get(x[2 * i]), Elem<T>::get(x[2 * i + 1]));
 }
+// Copies a whole block's `Bytes` (256 elements) into shared memory, asynchronously.
+template <int Bytes>
+__device__ __forceinline__ void fetch(uint8_t* to, const void* from, int lane) {
+#pragma unroll
+    for (int i = 0; i < (Bytes + 511) / 512; ++i)
+        if (Bytes >= 512 || lane < Bytes / 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             smem_u32(to) + i * 512 + lane * 16),
+                         "l"(static_cast<const uint8_t*>(from) + i * 512 + lane * 16)
+                         : "memory");
+}
+
 // Eight codes of a lane as two words of four: one load of a word in the vector form.
 __device__ __forceinline__ void load_codes(const uint8_t* x, bool vec, int lane, int64_t left,
                                            uint32_t (&w)[2]) {
@@ -253,11 +265,20 @@ __device__ __forceinline__ float encode_m(const F2 (&m)[4], uint32_t (&codes)[2]
     return s;
 }
 
+// Both flush subnormals: a v below 2^-126 gives root 0 (see kTinyEps), and a
+// denominator, at least 2^-75 or zero, is none.
 __device__ __forceinline__ float sqrt_approx(float x) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// With eps this small the root of a subnormal v counts: exact roots then.
+constexpr float kTinyEps = 1e-12f;
 
 // Eight roots of a block as codes, from v and r, the roots to within three units of
 // the last place (sqrt.approx: one or two): codes are those of the correctly rounded
@@ -334,32 +355,68 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
     const G* g = static_cast<const G*>(t.grad);
     float* master = static_cast<float*>(t.master);
     const bool aligned =
-        ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(P) - 1)) |
-         (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) |
-         (reinterpret_cast<uintptr_t>(master) & 15) |
-         ((reinterpret_cast<uintptr_t>(t.exp_avg) | reinterpret_cast<uintptr_t>(t.exp_avg_sq)) &
-          (BITS == 8 ? 3 : 15))) == 0;
+        ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) |
+          reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(t.exp_avg) |
+          reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & 15) == 0;
 
-    for (int64_t b = begin + warp * kBlockElems; b < end; b += kTurnElems) {
+    // Whole blocks of aligned tensors come through shared memory: the next one is on
+    // its way while this one is worked on, at no cost in registers.
+    constexpr int kMoment = BITS == 32 ? 4 : 1;
+    constexpr int kG = kBlockElems * sizeof(G), kW = kBlockElems * 4, kM = kBlockElems * kMoment;
+    __shared__ __align__(16) uint8_t ring[kOptThreads / 32][kG + kW + 2 * kM];
+    uint8_t* in_g = ring[warp];
+    uint8_t *in_w = in_g + kG, *in_m = in_w + kW, *in_v = in_m + kM;
+    auto whole = [&](int64_t b) { return aligned && end - b >= kBlockElems; };
+    float next_ms = 0.0f, next_vs = 0.0f;
+    auto ask = [&](int64_t b) {
+        if (b >= end) return;
+        if (BITS == 8) {
+            next_ms = t.exp_avg_scale[b / kBlockElems];
+            next_vs = t.exp_avg_sq_scale[b / kBlockElems];
+        }
+        if (!whole(b)) return;
+        fetch<kG>(in_g, g + b, lane);
+        if (master) fetch<kW>(in_w, master + b, lane);
+        else fetch<kBlockElems * sizeof(P)>(in_w, p + b, lane);
+        fetch<kM>(in_m, static_cast<uint8_t*>(t.exp_avg) + b * kMoment, lane);
+        fetch<kM>(in_v, static_cast<uint8_t*>(t.exp_avg_sq) + b * kMoment, lane);
+    };
+
+    const bool exact_roots = f.eps < kTinyEps;
+    int64_t b = begin + warp * kBlockElems;
+    ask(b);
+    for (; b < end; b += kTurnElems) {
         const int64_t left = end - b;
-        const bool vec = aligned && left >= kBlockElems;
+        const bool vec = whole(b);
         G gv[8];
         P pv[8];
         float wv[8], mv[8], vv[8];
         uint32_t mc[2], vc[2];
-        float ms = 0.0f, vs = 0.0f;
-        load8<G>(g + b, vec, lane, left, gv);
-        if (master) load8<float>(master + b, vec, lane, left, wv);
-        else load8<P>(p + b, vec, lane, left, pv);
-        if (BITS == 32) {
-            load8<float>(static_cast<float*>(t.exp_avg) + b, vec, lane, left, mv);
-            load8<float>(static_cast<float*>(t.exp_avg_sq) + b, vec, lane, left, vv);
-        } else {
-            load_codes(static_cast<uint8_t*>(t.exp_avg) + b, vec, lane, left, mc);
-            load_codes(static_cast<uint8_t*>(t.exp_avg_sq) + b, vec, lane, left, vc);
-            ms = t.exp_avg_scale[b / kBlockElems];
-            vs = t.exp_avg_sq_scale[b / kBlockElems];
-        }
+        const float ms = next_ms, vs = next_vs;
+        auto take = [&](bool v, const G* gb, const float* wb, const P* pb, const uint8_t* mb,
+                        const uint8_t* vb) {
+            load8<G>(gb, v, lane, left, gv);
+            if (master) load8<float>(wb, v, lane, left, wv);
+            else load8<P>(pb, v, lane, left, pv);
+            if (BITS == 32) {
+                load8<float>(reinterpret_cast<const float*>(mb), v, lane, left, mv);
+                load8<float>(reinterpret_cast<const float*>(vb), v, lane, left, vv);
+            } else {
+                load_codes(mb, v, lane, left, mc);
+                load_codes(vb, v, lane, left, vc);
+            }
+        };
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        if (vec)
+            take(true, reinterpret_cast<const G*>(in_g), reinterpret_cast<const float*>(in_w),
+                 reinterpret_cast<const P*>(in_w), in_m, in_v);
+        else
+            take(false, g + b, master + b, p + b,
+                 static_cast<uint8_t*>(t.exp_avg) + b * kMoment,
+                 static_cast<uint8_t*>(t.exp_avg_sq) + b * kMoment);
+        __syncwarp();
+        ask(b + kTurnElems);
         F2 m[4], v[4], r[4], w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -375,13 +432,13 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
             m[e] = add2(mul2(m[e], both(f.b1)), mul2(ge, both(f.c1)), both(f.one));
             v[e] = add2(mul2(v[e], both(f.b2)), mul2(mul2(ge, both(f.c2)), ge), both(f.one));
             const float2 v2 = unpack(v[e]);
-            r[e] = BITS == 32 ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
+            r[e] = BITS == 32 || exact_roots ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
                               : pack(sqrt_approx(v2.x), sqrt_approx(v2.y));
             const float2 den = unpack(add2(mul2(r[e], both(f.root)), both(f.eps), both(f.one)));
             const float2 num = unpack(mul2(m[e], both(-f.step_size)));
             const F2 quot = BITS == 32
                                 ? pack(__fdiv_rn(num.x, den.x), __fdiv_rn(num.y, den.y))
-                                : pack(__fdividef(num.x, den.x), __fdividef(num.y, den.y));
+                                : pack(num.x * rcp_approx(den.x), num.y * rcp_approx(den.y));
             w[e] = add2(mul2(master ? widen(wv, e) : widen(pv, e), both(f.decay)), quot,
                         both(f.one));
         }
@@ -443,7 +500,6 @@ template <class G, int CAP>
 __global__ void __launch_bounds__(kOptThreads)
     norm_partial_kernel(const __grid_constant__ Table<CAP, NormTensor> tab, int64_t chunk,
                         double* partial) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t chunks = tab.first[tab.count];
     double sum = 0.0;
     for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -451,15 +507,32 @@ __global__ void __launch_bounds__(kOptThreads)
         const G* g = static_cast<const G*>(tab.t[i].g);
         const int64_t begin = static_cast<int64_t>(c - tab.first[i]) * chunk;
         const int64_t end = min(static_cast<int64_t>(tab.t[i].n), begin + chunk);
-        const bool aligned = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
-        for (int64_t b = begin + warp * kBlockElems; b < end; b += kTurnElems) {
-            G gv[8];
-            load8<G>(g + b, aligned && end - b >= kBlockElems, lane, end - b, gv);
+        auto add = [&](G x) {
+            const double d = static_cast<double>(Elem<G>::get(x));
+            sum = fma(d, d, sum);
+        };
+        if ((reinterpret_cast<uintptr_t>(g + begin) & 15) == 0) {
+            // 16-byte loads, four in flight a thread
+            constexpr int kPer = 16 / sizeof(G), kFlight = 4;
+            const int n = static_cast<int>(end - begin), pieces = n / kPer;
+            const uint4* from = reinterpret_cast<const uint4*>(g + begin);
+            for (int at = threadIdx.x; at < pieces; at += kFlight * kOptThreads) {
+                uint4 q[kFlight];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const double x = static_cast<double>(Elem<G>::get(gv[e]));
-                sum = fma(x, x, sum);
+                for (int u = 0; u < kFlight; ++u)
+                    q[u] = at + u * kOptThreads < pieces ? __ldcs(from + at + u * kOptThreads)
+                                                         : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    G x[kPer];
+                    __builtin_memcpy(x, &q[u], 16);
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) add(x[e]);
+                }
             }
+            if (threadIdx.x < n - pieces * kPer) add(g[begin + pieces * kPer + threadIdx.x]);
+        } else {
+            for (int64_t at = begin + threadIdx.x; at < end; at += kOptThreads) add(g[at]);
         }
     }
     sum = block_sum(sum);
@@ -498,8 +571,8 @@ int sm_count() {
 constexpr int kSmallTable = 32;
 constexpr int kLargeTable = 440;
 
-// Elements per chunk: whole turns of a CTA, about four chunks for each of the
-// 8 CTAs an SM holds when there is that much work, else as little as one turn.
+// Elements per chunk: whole turns of a CTA, up to eight when that leaves thirty
+// chunks for each SM, else as little as one.
 int64_t chunk_elems(uint64_t total) {
     const uint64_t want = total / (static_cast<uint64_t>(sm_count()) * 32);
     const uint64_t turns = std::min<uint64_t>(std::max<uint64_t>(want / kTurnElems, 1), 8);

@@ -171,6 +171,16 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ P
     }
 }
 
+void shape_y(const FfCall& c, FfProduct& p) { p.M = c.m, p.N = c.d, p.k[0] = c.f, p.ldc = c.d; }
+void shape_dx(const FfCall& c, FfProduct& p) {
+    p.M = c.m, p.N = c.k, p.k[0] = p.k[1] = c.f, p.ldc = c.k;
+}
+void shape_dw(const FfCall& c, FfProduct (&p)[3]) {  // dWg, dWu, dWd
+    for (FfProduct& q : p) q.k[0] = c.m;
+    p[0].M = p[1].M = c.k, p[0].N = p[1].N = c.f, p[0].ldc = p[1].ldc = c.f;
+    p[2].M = c.f, p[2].N = c.d, p[2].ldc = c.d;
+}
+
 // Workspace: h, then for the backward pass dg and du, [m, f] each; then padded
 // copies of the 16-bit inputs that need them.
 enum { kX, kWg, kWu, kWd, kDy, kInputs };
@@ -179,6 +189,7 @@ struct FfLayout {
     uint64_t plane, total;
     bool pad[kInputs];
     uint64_t at[kInputs];
+    uint64_t parts;  // of split sums; the launches that use it follow one another
 };
 FfLayout ff_layout(const FfCall& c) {
     FfLayout l;
@@ -190,6 +201,13 @@ FfLayout ff_layout(const FfCall& c) {
         l.pad[i] = c.size == 2 && cols[i] % 8 != 0 && (c.backward || i != kDy);
         l.at[i] = l.total;
         if (l.pad[i]) l.total += round_up(rows[i] * round_up(cols[i], 8) * c.size, 256);
+    }
+    l.parts = l.total;
+    if (c.size == 2) {
+        FfProduct y, dx, dw[3];
+        shape_y(c, y), shape_dx(c, dx), shape_dw(c, dw);
+        l.total += c.backward ? std::max(ff_split_bytes(&dx, 1), ff_split_bytes(dw, 3))
+                              : ff_split_bytes(&y, 1);
     }
     return l;
 }
@@ -408,8 +426,9 @@ int check_pointers(std::initializer_list<const void*> in, std::initializer_list<
     return ZG_OK;
 }
 
-int products(const FfCall& c, FfEpilogue epi, const FfProduct* p, int count, cudaStream_t s) {
-    if (c.size == 2) return ff_pair(c.dtype, epi, c.act, p, count, s);
+int products(const FfCall& c, FfEpilogue epi, const FfProduct* p, int count, void* parts,
+             cudaStream_t s) {
+    if (c.size == 2) return ff_pair(c.dtype, epi, c.act, p, count, static_cast<float*>(parts), s);
     int rc = ZG_OK;
     for (int i = 0; i < count && !rc; ++i) rc = ff_simt(c.dtype, epi, c.act, p[i], s);
     return rc;
@@ -461,13 +480,14 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
     p.c = workspace, p.ldc = l.ld_f;
     p.pre_g = pre_gate, p.pre_u = pre_up;
     const bool few = c.size == 2 && m <= kFfRows;
-    if ((rc = few ? ff_rows(dtype, true, act, p, s) : products(c, kFfGated, &p, 1, s))) return rc;
-    FfProduct q;  // y
-    q.M = m, q.N = d, q.k[0] = f;
+    void* parts = static_cast<uint8_t*>(workspace) + l.parts;
+    if ((rc = few ? ff_rows(dtype, true, act, p, s) : products(c, kFfGated, &p, 1, nullptr, s))) return rc;
+    FfProduct q;
+    shape_y(c, q);
     q.a[0] = {workspace, l.ld_f, false};
     q.b[0] = {in[kWd].p, in[kWd].ld, true};
-    q.c = y, q.ldc = d;
-    return few ? ff_rows(dtype, false, act, q, s) : products(c, kFfStore, &q, 1, s);
+    q.c = y;
+    return few ? ff_rows(dtype, false, act, q, s) : products(c, kFfStore, &q, 1, parts, s);
 }
 
 extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,
@@ -515,23 +535,21 @@ extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, in
     p.b[0] = {in[kWd].p, in[kWd].ld, false};
     p.c = dg, p.c2 = du, p.c3 = h, p.ldc = l.ld_f;
     p.pre_g = const_cast<float*>(pre_gate), p.pre_u = const_cast<float*>(pre_up);
-    if ((rc = products(c, kFfSlope, &p, 1, s))) return rc;
-    FfProduct q;  // dx
-    q.M = m, q.N = k, q.k[0] = q.k[1] = f;
+    if ((rc = products(c, kFfSlope, &p, 1, nullptr, s))) return rc;
+    FfProduct q;
+    shape_dx(c, q);
     q.a[0] = {dg, l.ld_f, false};
     q.b[0] = {in[kWg].p, in[kWg].ld, false};
     q.a[1] = {du, l.ld_f, false};
     q.b[1] = {in[kWu].p, in[kWu].ld, false};
-    q.c = dx, q.ldc = k;
-    if ((rc = products(c, kFfStore, &q, 1, s))) return rc;
-    FfProduct w[3];  // dWg, dWu, dWd
-    for (int i = 0; i < 3; ++i) w[i].k[0] = m;
-    w[0].M = w[1].M = k, w[0].N = w[1].N = f, w[0].ldc = w[1].ldc = f;
+    q.c = dx;
+    if ((rc = products(c, kFfStore, &q, 1, ws + l.parts, s))) return rc;
+    FfProduct w[3];
+    shape_dw(c, w);
     w[0].a[0] = w[1].a[0] = {in[kX].p, in[kX].ld, true};
     w[0].b[0] = {dg, l.ld_f, true}, w[0].c = dw_gate;
     w[1].b[0] = {du, l.ld_f, true}, w[1].c = dw_up;
-    w[2].M = f, w[2].N = d, w[2].ldc = d;
     w[2].a[0] = {h, l.ld_f, true};
     w[2].b[0] = {in[kDy].p, in[kDy].ld, true}, w[2].c = dw_down;
-    return products(c, kFfStore, w, 3, s);
+    return products(c, kFfStore, w, 3, ws + l.parts, s);
 }

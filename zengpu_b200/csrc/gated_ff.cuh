@@ -97,14 +97,35 @@ struct FfProduct {
     float* pre_u = nullptr;
 };
 
+// Launches a kernel that may start while the one before it in the stream still runs
+// (it calls griddepcontrol.wait before it touches memory).
+template <class... Params, class... Args>
+int launch_dependent(const char* what, void (*kernel)(Params...), unsigned grid, unsigned threads,
+                     size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
 // Plain CUDA-core product for any layout, f32 sums (gated_ff.cu).
 int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
 
 // 16-bit tensors on the tensor cores (gated_ff_tc.cu): `count` products of one
 // epilogue in one launch (at most three).  Operands: 16-byte aligned, pitch a
-// multiple of 8.
+// multiple of 8.  kFfStore: ff_splits says into how many parts the sums are split,
+// for which `parts` holds ff_split_bytes; ldc is N then.
+int ff_splits(const FfProduct* products, int count);
+uint64_t ff_split_bytes(const FfProduct* products, int count);
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
-            cudaStream_t s);
+            float* parts, cudaStream_t s);
 
 // The forward products for up to kFfRows rows of 16-bit tensors (gated_ff_rows.cu):
 // `gated` as kFfGated, else as kFfStore of one product, launched right behind the

@@ -28,7 +28,10 @@
 // whole sum: its additions truncate, about n / 16 2^-24 of the result for n terms,
 // which at n = 12288 is 5e-5, a tenth of half an f16 step.  Two accumulators: a
 // tile's epilogue overlaps the next tile's MMAs.  When the last wave would keep
-// at most half of the pairs busy its tiles run as two column halves.
+// at most half of the pairs busy its tiles run as two column halves.  Products of
+// few tiles and a long sum are split along it into f32 parts, which a second kernel
+// adds up in order.  Each kernel is launched while the one before it drains
+// (programmatic dependent launch) and waits for it before it touches memory.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -55,7 +58,7 @@ constexpr int kStageCount[3] = {5, 5, 4};
 template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
 constexpr int kBlock32 = 32 * kPitch<float>;
 constexpr int kBlock16 = 32 * kPitch<__half>;
-constexpr int kTurnBytes[3] = {kBlock16, kBlock32, kBlock16 + 2 * kBlock32};
+constexpr int kTurnBytes[3] = {kBlock32, kBlock32, kBlock16 + 2 * kBlock32};
 constexpr int smem_bytes(int epi) {
     return kStageCount[epi] * kStageBytes + kEpiWarps * kTurnBytes[epi] + 1024 /*align*/ +
            256 /*bars*/;
@@ -63,6 +66,7 @@ constexpr int smem_bytes(int epi) {
 static_assert(smem_bytes(2) <= 232448, "shared memory of an SM");
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxProblems = 3;
+constexpr int kPairsSold = 74;  // SM pairs of a B200: what split sums are dealt out for
 
 struct alignas(64) PairProblem {
     CUtensorMap a[2], b[2];
@@ -76,7 +80,9 @@ struct alignas(64) PairProblem {
     int nkb[2];  // stages of the two sums
     int a_mn, b_mn;
     int vec_c, vec_pre;
-    int tiles;  // of this problem and those before it
+    int splits;     // of the sum; with more than one, parts[s] = c, planes of M x ldp f32
+    int64_t plane;  // elements of one
+    int tiles;      // of this problem and those before it, each split counted
 };
 
 struct PairArgs {
@@ -121,6 +127,7 @@ __device__ __forceinline__ void raster(int tile, int mt, int nt, int& mi, int& n
 struct Unit {
     const PairProblem* p;
     int m0, n0, width;  // width: columns of D in TMEM, 256 or 128
+    int part, kb0, kb1;
 };
 template <int EPI>
 __device__ __forceinline__ Unit unit_of(const PairArgs& args, int u) {
@@ -130,11 +137,16 @@ __device__ __forceinline__ Unit unit_of(const PairArgs& args, int u) {
     while (i + 1 < args.count && tile >= args.p[i].tiles) ++i;
     const PairProblem& p = args.p[i];
     constexpr int cols = EPI == kFfGated ? 128 : 256;  // columns of the output
-    int mi, ni;
-    raster(tile - (i ? args.p[i - 1].tiles : 0), (p.M + 255) / 256, (p.N + cols - 1) / cols, mi,
-           ni);
+    const int mt = (p.M + 255) / 256, nt = (p.N + cols - 1) / cols;
+    const int t = tile - (i ? args.p[i - 1].tiles : 0);
     Unit w;
     w.p = &p;
+    w.part = EPI == kFfStore ? t / (mt * nt) : 0;
+    const int nkb = p.nkb[0] + p.nkb[1];
+    w.kb0 = nkb * w.part / p.splits;
+    w.kb1 = nkb * (w.part + 1) / p.splits;
+    int mi, ni;
+    raster(t - w.part * mt * nt, mt, nt, mi, ni);
     w.m0 = mi * 256;
     w.n0 = ni * cols + (half ? ((u - args.full_units) & 1) * (cols / 2) : 0);
     w.width = half ? 128 : 256;
@@ -245,6 +257,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // after the allocation: a dependent CTA must not hold TMEM that this grid waits for
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // what the kernel before this one wrote may be read from here on
+    asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -257,8 +273,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int b_rows = w.width / 2;
                 // gated: CTA 0 takes Wg's columns, CTA 1 the same columns of Wu
                 const int b0 = EPI == kFfGated ? w.n0 : w.n0 + b_rows * static_cast<int>(rank);
-                const int nkb = p.nkb[0] + p.nkb[1];
-                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
                     const int s = it % kStages;
                     if (!mbar_wait_bounded(&empty[s], ((it / kStages) & 1) ^ 1, args.status,
                                            kErrFfProducer)) {
@@ -299,8 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 const uint32_t idesc = instr_desc<T>(w.width, p.a_mn, p.b_mn);
                 const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-                const int nkb = p.nkb[0] + p.nkb[1];
-                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
                     const int s = it % kStages;
                     if (!mbar_wait_bounded(&full[s], (it / kStages) & 1, args.status, kErrFfMma)) {
                         ok = false;
@@ -312,7 +326,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < kBK / 16; ++i)
                         mma_f16_ss_pair(d_tmem, smem_desc(a + i * a_step, kBoxBytes),
                                         smem_desc(b + i * b_step, kBoxBytes), idesc,
-                                        (kb | i) != 0);
+                                        kb != w.kb0 || i != 0);
                     mma_commit_pair(&empty[s], 0x3);
                 }
                 if (ok) mma_commit_pair(&acc_full[buf], 0x3);
@@ -361,7 +375,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int64_t at = row0 * p.ldc + col, pre = row0 * p.N + col;
                 T* c = static_cast<T*>(p.c) + at;
                 auto f = [](uint32_t x) { return __uint_as_float(x); };
-                if (EPI == kFfStore) {
+                if (EPI == kFfStore && p.splits > 1) {
+                    store_block<float>(static_cast<float*>(p.c) + w.part * p.plane + at, p.ldc, rows,
+                                       cols, true, r, turn, lane);
+                } else if (EPI == kFfStore) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
                     store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
@@ -431,6 +448,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
+// Adds up the parts of split sums, in order, and rounds: four elements a thread.
+struct SumArgs {
+    struct {
+        const float* part;
+        void* c;
+        int64_t plane, groups;  // groups of this matrix and those before it
+        int N, ldp;
+    } m[kMaxProblems];
+    int count, splits;
+};
+template <class T>
+__global__ void __launch_bounds__(256) ff_sum_kernel(const __grid_constant__ SumArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+         g < a.m[a.count - 1].groups; g += step) {
+        int i = 0;
+        while (g >= a.m[i].groups) ++i;
+        const auto& m = a.m[i];
+        const int64_t at = (g - (i ? a.m[i - 1].groups : 0)) * 4;
+        const int64_t row = at / m.ldp;
+        const int col = static_cast<int>(at - row * m.ldp);
+        float4 sum = __ldcs(reinterpret_cast<const float4*>(m.part + at));
+        for (int s = 1; s < a.splits; ++s) {
+            const float4 x = __ldcs(reinterpret_cast<const float4*>(m.part + s * m.plane + at));
+            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+        }
+        T* c = static_cast<T*>(m.c) + row * m.N + col;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (m.N % 4 == 0 && (reinterpret_cast<uintptr_t>(m.c) & 7) == 0) {
+            T t[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = FfElem<T>::put(v[e]);
+            uint2 q;
+            __builtin_memcpy(&q, t, 8);
+            *reinterpret_cast<uint2*>(c) = q;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < m.N) c[e] = FfElem<T>::put(v[e]);
+        }
+    }
+}
+
 // ---- host ----------------------------------------------------------------------
 int sm_pairs() {
     int dev = 0, sms = 148;
@@ -459,9 +520,8 @@ int launch(const PairArgs& args, int units, cudaStream_t s) {
         if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     }
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
-    ff_pair_kernel<EPI, ACT, T><<<2 * std::min(units, sm_pairs()), kThreads, smem_bytes(EPI), s>>>(
-        args);
-    return cuda_status(cudaGetLastError(), "gated_ff");
+    return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T>, 2 * std::min(units, sm_pairs()),
+                            kThreads, smem_bytes(EPI), s, args);
 }
 
 template <class T>
@@ -483,12 +543,37 @@ int launch_epi(FfEpilogue epi, int act, const PairArgs& a, int units, cudaStream
 
 }  // namespace
 
+int ff_splits(const FfProduct* products, int count) {
+    int64_t tiles = 0;
+    int nkb = 1 << 30;
+    for (int i = 0; i < count; ++i) {
+        const FfProduct& f = products[i];
+        tiles += static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256);
+        nkb = std::min(nkb, (f.k[0] + kBK - 1) / kBK + (f.k[1] + kBK - 1) / kBK);
+    }
+    return static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>({4, kPairsSold / std::max<int64_t>(tiles, 1), nkb / 8})));
+}
+
+uint64_t ff_split_bytes(const FfProduct* products, int count) {
+    const int splits = ff_splits(products, count);
+    if (splits == 1) return 0;
+    uint64_t elems = 0;
+    for (int i = 0; i < count; ++i)
+        elems += static_cast<uint64_t>(products[i].M) * ((products[i].N + 3) / 4 * 4);
+    return elems * splits * 4;
+}
+
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
-            cudaStream_t s) {
+            float* parts, cudaStream_t s) {
     PairArgs args;
     std::memset(&args, 0, sizeof(args));
     args.count = count;
     int rc = status_word(&args.status), tiles = 0;
+    const int splits = epi == kFfStore ? ff_splits(products, count) : 1;
+    SumArgs sum;
+    sum.count = count, sum.splits = splits;
+    int64_t groups = 0;
     const int cols = epi == kFfGated ? 128 : 256;
     for (int i = 0; i < count && !rc; ++i) {
         const FfProduct& f = products[i];
@@ -500,12 +585,21 @@ int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, 
         p.vec_c = f.ldc % 8 == 0 && aligned16(f.c) && aligned16(f.c2) && aligned16(f.c3);
         p.vec_pre = f.N % 4 == 0 && aligned16(f.pre_g) && aligned16(f.pre_u);
         for (int seg = 0; seg < 2; ++seg) p.nkb[seg] = (f.k[seg] + kBK - 1) / kBK;
+        p.splits = splits;
+        if (splits > 1) {  // f32 parts first
+            const int ldp = (f.N + 3) / 4 * 4;
+            p.plane = static_cast<int64_t>(f.M) * ldp;
+            groups += p.plane / 4;
+            sum.m[i] = {parts, f.c, p.plane, groups, f.N, ldp};
+            p.c = parts, p.ldc = ldp;
+            parts += p.plane * splits;
+        }
         rc = operand_map(&p.a[0], dtype, f.a[0], f.M, f.k[0]);
         if (!rc) rc = operand_map(&p.b[0], dtype, f.b[0], f.N, f.k[0]);
         if (!rc && f.k[1]) rc = operand_map(&p.a[1], dtype, f.a[1], f.M, f.k[1]);
         if (!rc && f.b[1].p) rc = operand_map(&p.b[1], dtype, f.b[1], f.N, f.k[1] ? f.k[1] : f.k[0]);
         const int64_t total =
-            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + cols - 1) / cols);
+            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + cols - 1) / cols) * splits;
         if (total > (1 << 29)) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many tiles");
         p.tiles = tiles = static_cast<int>(total);
     }
@@ -514,8 +608,13 @@ int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, 
     args.split = rem > 0 && 2 * rem <= pairs ? 2 : 1;
     args.full_units = args.split > 1 ? tiles - rem : tiles;
     const int units = args.full_units + (tiles - args.full_units) * args.split;
-    return dtype == ZG_DTYPE_BF16 ? launch_epi<__nv_bfloat16>(epi, act, args, units, s)
-                                  : launch_epi<__half>(epi, act, args, units, s);
+    rc = dtype == ZG_DTYPE_BF16 ? launch_epi<__nv_bfloat16>(epi, act, args, units, s)
+                                : launch_epi<__half>(epi, act, args, units, s);
+    if (rc || splits == 1) return rc;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((groups + 255) / 256, 148 * 16));
+    return dtype == ZG_DTYPE_BF16
+               ? launch_dependent("gated_ff sum", ff_sum_kernel<__nv_bfloat16>, grid, 256, 0, s, sum)
+               : launch_dependent("gated_ff sum", ff_sum_kernel<__half>, grid, 256, 0, s, sum);
 }
 
 }  // namespace zg

@@ -513,6 +513,36 @@ int zg_grad_norm(uint32_t grad_dtype, uint32_t count, const void *const *grads,
                  const uint64_t *sizes, double max_norm, float *out, void *workspace,
                  uint64_t workspace_bytes, void *stream);
 
+/* ---- The same on arrays (layer 2), as GemmKernel and Level1Kernels methods: checks,
+ * pools and GpuOnly residency as for sgemm and saxpy there.  Arrays are F32, BF16
+ * or F16 (one dtype per call for the block; `k`'s mode is read for F32).
+ *   gated_ff           out [m, d] from the pool; pre_gate, pre_up (both or neither
+ *                      NULL): f32 [m, f] from the pool, for the backward pass
+ *   gated_ff_backward  dx, dw_gate, dw_up, dw_down from the pool
+ *   adamw              `count` arrays of each kind, in place: moments f32, or U8 codes
+ *                      with their scales [ceil(n / 256)] f32 (else NULL); master
+ *                      NULL or f32; norm_scale NULL or what grad_norm returned.  No
+ *                      buffer may be bound twice, gradients aside.
+ *   grad_norm          out f32 [2] from the pool: norm, clip factor */
+int zg_gemm_gated_ff(const zg_gemm_kernel *k, zg_device *dev, zg_pool *pool, int act,
+                     const zg_device_array *x, const zg_device_array *w_gate,
+                     const zg_device_array *w_up, const zg_device_array *w_down,
+                     zg_device_array *out, zg_device_array *pre_gate, zg_device_array *pre_up);
+int zg_gemm_gated_ff_backward(const zg_gemm_kernel *k, zg_device *dev, zg_pool *pool, int act,
+                              const zg_device_array *dy, const zg_device_array *x,
+                              const zg_device_array *w_gate, const zg_device_array *w_up,
+                              const zg_device_array *w_down, const zg_device_array *pre_gate,
+                              const zg_device_array *pre_up, zg_device_array *dx,
+                              zg_device_array *dw_gate, zg_device_array *dw_up,
+                              zg_device_array *dw_down);
+int zg_level1_adamw(zg_device *dev, uint32_t count, const zg_device_array *params,
+                    const zg_device_array *grads, const zg_device_array *master,
+                    const zg_device_array *exp_avg, const zg_device_array *exp_avg_sq,
+                    const zg_device_array *exp_avg_scale, const zg_device_array *exp_avg_sq_scale,
+                    const zg_adamw_hyper *h, const zg_device_array *norm_scale);
+int zg_level1_grad_norm(zg_device *dev, zg_pool *pool, uint32_t count,
+                        const zg_device_array *grads, double max_norm, zg_device_array *out);
+
 /* Name of the main kernel zg_sgemm_f32 / zg_sgemm_packed launch for
  * (mode, m, n, k) on the current device ("" for an unknown mode or an empty
  * output), for reports and profiler filters.  The tensor-core modes take the

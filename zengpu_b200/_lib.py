@@ -201,6 +201,14 @@ SIGNATURES: dict[str, tuple] = {
     "zg_grad_norm_workspace_bytes": (_u64, [_u32]),
     "zg_grad_norm": (_i, [_u32, _u32, C.POINTER(_vp), C.POINTER(_u64), C.c_double, _vp, _vp, _u64,
                           _vp]),
+    "zg_gemm_gated_ff": (_i, [C.POINTER(CGemmKernel), _vp, _vp, _i] +
+                         [C.POINTER(CDeviceArray)] * 7),
+    "zg_gemm_gated_ff_backward": (_i, [C.POINTER(CGemmKernel), _vp, _vp, _i] +
+                                  [C.POINTER(CDeviceArray)] * 11),
+    "zg_level1_adamw": (_i, [_vp, _u32] + [C.POINTER(CDeviceArray)] * 7 +
+                        [C.POINTER(AdamWHyper), C.POINTER(CDeviceArray)]),
+    "zg_level1_grad_norm": (_i, [_vp, _vp, _u32, C.POINTER(CDeviceArray), C.c_double,
+                                 C.POINTER(CDeviceArray)]),
     "zg_kernel_status": (_i, [C.POINTER(_u32)]),
     "zg_sgemm_kernel_name": (C.c_char_p, [_i, _i, _i, _i]),
     "zg_bchain_create": (_i, [_i, _i, _i, _i, C.POINTER(_vp), C.POINTER(C.c_uint8)]),

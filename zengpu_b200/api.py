@@ -588,8 +588,44 @@ class GemmKernel:
         del ka, kb, kc, kbias
 
 
+    def gated_ff(self, device: CudaDevice, pool: BufferPool, x: DeviceArray, w_gate: DeviceArray,
+                 w_up: DeviceArray, w_down: DeviceArray, act: Activation = Activation.SILU,
+                 save: bool = False):
+        """(act(x @ w_gate) * (x @ w_up)) @ w_down; save=True returns (y, (pre_gate,
+        pre_up)) for gated_ff_backward.  F32 (in this kernel's mode), F16 or Bf16."""
+        out = [L.CDeviceArray() for _ in range(3 if save else 1)]
+        refs = [C.byref(o) for o in out] + [None] * (3 - len(out))
+        check(self._lib.zg_gemm_gated_ff(C.byref(self._k), device.raw, pool.raw, int(act),
+                                         C.byref(x._c), C.byref(w_gate._c), C.byref(w_up._c),
+                                         C.byref(w_down._c), *refs))
+        y, *saved = map(DeviceArray, out)
+        return (y, tuple(saved)) if save else y
+
+    def gated_ff_backward(self, device: CudaDevice, pool: BufferPool, dy: DeviceArray,
+                          x: DeviceArray, w_gate: DeviceArray, w_up: DeviceArray,
+                          w_down: DeviceArray, saved: Sequence[DeviceArray],
+                          act: Activation = Activation.SILU) -> tuple[DeviceArray, ...]:
+        """(dx, dw_gate, dw_up, dw_down) for dy, the gradient of gated_ff's y."""
+        out = [L.CDeviceArray() for _ in range(4)]
+        pre_gate, pre_up = saved
+        check(self._lib.zg_gemm_gated_ff_backward(
+            C.byref(self._k), device.raw, pool.raw, int(act), C.byref(dy._c), C.byref(x._c),
+            C.byref(w_gate._c), C.byref(w_up._c), C.byref(w_down._c), C.byref(pre_gate._c),
+            C.byref(pre_up._c), *[C.byref(o) for o in out]))
+        return tuple(map(DeviceArray, out))
+
+
+def _arrays(arrays: Sequence[DeviceArray] | None, count: int, name: str):
+    if arrays is None:
+        return None
+    if len(arrays) != count:
+        raise ValueError(f"{name}: {len(arrays)} arrays, expected {count}")
+    return (L.CDeviceArray * max(count, 1))(*[a._c for a in arrays])
+
+
 class Level1Kernels:
-    """saxpy / sscal, in place (zengpu-blas/src/level1.rs:51-139)."""
+    """saxpy / sscal, in place (zengpu-blas/src/level1.rs:51-139), and the steps over
+    many arrays: adamw, grad_norm."""
 
     def __init__(self, device: CudaDevice):
         self._lib = L.load()
@@ -603,6 +639,35 @@ class Level1Kernels:
 
     def sscal(self, device: CudaDevice, pool: BufferPool, alpha: float, x: DeviceArray) -> None:
         check(self._lib.zg_level1_sscal(device.raw, float(alpha), C.byref(x._c)))
+
+    def adamw(self, device: CudaDevice, params: Sequence[DeviceArray],
+              grads: Sequence[DeviceArray], exp_avg: Sequence[DeviceArray],
+              exp_avg_sq: Sequence[DeviceArray], step: int, lr: float = 1e-3, beta1: float = 0.9,
+              beta2: float = 0.999, eps: float = 1e-8, weight_decay: float = 0.01,
+              master: Sequence[DeviceArray] | None = None,
+              scales: tuple[Sequence[DeviceArray], Sequence[DeviceArray]] | None = None,
+              norm_scale: DeviceArray | None = None) -> None:
+        """One AdamW step over all arrays, in place (zg_level1_adamw).  Moments: F32, or
+        U8 codes with `scales`, their two lists of F32 arrays (one value for each 256
+        elements).  norm_scale: grad_norm's result."""
+        n = len(params)
+        ms, vs = scales if scales is not None else (None, None)
+        hyper = L.AdamWHyper(lr, beta1, beta2, eps, weight_decay, step)
+        check(self._lib.zg_level1_adamw(
+            device.raw, n, _arrays(params, n, "params"), _arrays(grads, n, "grads"),
+            _arrays(master, n, "master"), _arrays(exp_avg, n, "exp_avg"),
+            _arrays(exp_avg_sq, n, "exp_avg_sq"), _arrays(ms, n, "scales"),
+            _arrays(vs, n, "scales"), C.byref(hyper),
+            C.byref(norm_scale._c) if norm_scale is not None else None))
+
+    def grad_norm(self, device: CudaDevice, pool: BufferPool, grads: Sequence[DeviceArray],
+                  max_norm: float) -> DeviceArray:
+        """[norm, min(1, max_norm / norm)] over all arrays, F32 [2] from the pool."""
+        out = L.CDeviceArray()
+        check(self._lib.zg_level1_grad_norm(device.raw, pool.raw, len(grads),
+                                            _arrays(grads, len(grads), "grads"), float(max_norm),
+                                            C.byref(out)))
+        return DeviceArray(out)
 
 
 class Blas:

@@ -1526,6 +1526,289 @@ extern "C" int zg_level1_sscal(zg_device* dev, float alpha, const zg_device_arra
 }
 
 // ======================================================================
+// Gated feed-forward block, AdamW and gradient norm on arrays
+// ======================================================================
+
+namespace zg {
+namespace {
+
+// An operand of these ops: live, of `dtype`, `rank` sizes as given, and in a buffer
+// that holds it.
+int array_ptr(zg_device* dev, const zg_device_array* a, uint32_t dtype, uint32_t rank,
+              const uint32_t* shape, const char* op, const char* name, void** p) {
+    int rc = check_array(a, op);
+    if (rc) return rc;
+    if (a->dtype != dtype)
+        return set_error(ZG_ERR_DISPATCH, "%s: %s is %s, expected %s", op, name,
+                         dtype_name(a->dtype), dtype_name(dtype));
+    zg_device_array want = *a;
+    want.rank = rank;
+    for (uint32_t i = 0; i < rank; ++i) want.shape[i] = shape[i];
+    if (!same_shape(a, &want))
+        return set_error(ZG_ERR_DISPATCH, "%s: %s has shape %s, expected %s", op, name,
+                         shape_str(a).c_str(), shape_str(&want).c_str());
+    Buffer* b = dev->buffers.get(a->buffer);
+    if (!b) return stale(op, a->buffer, dev->buffers.current_gen(a->buffer.index));
+    uint32_t n = 0;
+    if (!array_len(a, &n) || static_cast<uint64_t>(n) * dtype_size(dtype) > b->len)
+        return set_error(ZG_ERR_DISPATCH, "%s: %s of shape %s exceeds its buffer", op, name,
+                         shape_str(a).c_str());
+    *p = b->ptr;
+    return ZG_OK;
+}
+
+// Output arrays of one call: given back to the pool if the call fails.
+struct PoolOutputs {
+    zg_pool* pool;
+    std::vector<zg_device_array*> got;
+    int alloc(uint32_t rows, uint32_t cols, uint32_t dtype, zg_device_array* out) {
+        const uint32_t shape[2] = {rows, cols};
+        const int rc = zg_pool_alloc(pool, shape, 2, dtype, out);
+        if (rc == ZG_OK) got.push_back(out);
+        return rc;
+    }
+    int fail(int rc) {
+        for (zg_device_array* a : got) zg_pool_free(pool, a);
+        return rc;
+    }
+};
+
+// Queues nothing more: waits unless the results are GpuOnly (see dispatch_deferred).
+int finish_op(zg_device* dev, bool deferred) {
+    if (deferred) {
+        dev->status_unchecked = true;
+        return ZG_OK;
+    }
+    return finish_sync(dev, true);
+}
+
+struct FfShapes {
+    uint32_t m, k, f, d, dtype;
+};
+
+// Shapes of x [m, k], w_gate [k, f] and w_down [f, d]; the rest is checked against them.
+int ff_shapes(const zg_device_array* x, const zg_device_array* w_gate,
+              const zg_device_array* w_down, const char* op, FfShapes* s) {
+    int rc;
+    for (const zg_device_array* a : {x, w_gate, w_down}) {
+        if ((rc = check_array(a, op))) return rc;
+        if (a->rank != 2)
+            return set_error(ZG_ERR_DISPATCH, "%s: expected 2D arrays, got shape %s", op,
+                             shape_str(a).c_str());
+        for (uint32_t i = 0; i < 2; ++i)
+            if (a->shape[i] > 0x7fffffffu)
+                return set_error(ZG_ERR_DISPATCH, "%s: dimension exceeds 2^31-1", op);
+    }
+    *s = {x->shape[0], x->shape[1], w_gate->shape[1], w_down->shape[1], x->dtype};
+    if (s->dtype != ZG_DTYPE_F32 && s->dtype != ZG_DTYPE_F16 && s->dtype != ZG_DTYPE_BF16)
+        return set_error(ZG_ERR_DISPATCH, "%s: f32, f16 and bf16 are supported, got %s", op,
+                         dtype_name(s->dtype));
+    return ZG_OK;
+}
+
+}  // namespace
+}  // namespace zg
+
+extern "C" int zg_gemm_gated_ff(const zg_gemm_kernel* k, zg_device* dev, zg_pool* pool, int act,
+                                const zg_device_array* x, const zg_device_array* w_gate,
+                                const zg_device_array* w_up, const zg_device_array* w_down,
+                                zg_device_array* out, zg_device_array* pre_gate,
+                                zg_device_array* pre_up) {
+    const char* op = "gated_ff";
+    if (!k || !dev || !pool || !out || (pre_gate == nullptr) != (pre_up == nullptr))
+        return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
+    FfShapes s;
+    int rc = ff_shapes(x, w_gate, w_down, op, &s);
+    if (rc) return rc;
+    std::lock_guard<std::recursive_mutex> lk(dev->mu);
+    if ((rc = set_device(dev))) return rc;
+    void *px, *pg, *pu, *pd, *py, *pre[2] = {nullptr, nullptr};
+    const uint32_t xs[2] = {s.m, s.k}, gs[2] = {s.k, s.f}, ds[2] = {s.f, s.d}, ys[2] = {s.m, s.d},
+                   ps[2] = {s.m, s.f};
+    if ((rc = array_ptr(dev, x, s.dtype, 2, xs, op, "x", &px)) ||
+        (rc = array_ptr(dev, w_gate, s.dtype, 2, gs, op, "w_gate", &pg)) ||
+        (rc = array_ptr(dev, w_up, s.dtype, 2, gs, op, "w_up", &pu)) ||
+        (rc = array_ptr(dev, w_down, s.dtype, 2, ds, op, "w_down", &pd)))
+        return rc;
+    const uint64_t ws = zg_gated_ff_workspace_bytes(s.dtype, k->mode, s.m, s.k, s.f, s.d, 0);
+    if ((rc = ensure_workspace(dev, ws))) return rc;
+    PoolOutputs outs{pool, {}};
+    if ((rc = outs.alloc(s.m, s.d, s.dtype, out)) ||
+        (pre_gate && ((rc = outs.alloc(s.m, s.f, ZG_DTYPE_F32, pre_gate)) ||
+                      (rc = outs.alloc(s.m, s.f, ZG_DTYPE_F32, pre_up)))) ||
+        (rc = array_ptr(dev, out, s.dtype, 2, ys, op, "out", &py)) ||
+        (pre_gate && ((rc = array_ptr(dev, pre_gate, ZG_DTYPE_F32, 2, ps, op, "pre_gate", &pre[0])) ||
+                      (rc = array_ptr(dev, pre_up, ZG_DTYPE_F32, 2, ps, op, "pre_up", &pre[1])))))
+        return outs.fail(rc);
+    if ((rc = zg_gated_ff(s.dtype, k->mode, act, s.m, s.k, s.f, s.d, px, pg, pu, pd, py,
+                          static_cast<float*>(pre[0]), static_cast<float*>(pre[1]), dev->workspace,
+                          dev->workspace_bytes, dev->stream))) {
+        cudaStreamSynchronize(dev->stream);
+        return outs.fail(rc);
+    }
+    return finish_op(dev, pool->memory == ZG_MEMORY_GPU_ONLY);
+}
+
+extern "C" int zg_gemm_gated_ff_backward(
+    const zg_gemm_kernel* k, zg_device* dev, zg_pool* pool, int act, const zg_device_array* dy,
+    const zg_device_array* x, const zg_device_array* w_gate, const zg_device_array* w_up,
+    const zg_device_array* w_down, const zg_device_array* pre_gate, const zg_device_array* pre_up,
+    zg_device_array* dx, zg_device_array* dw_gate, zg_device_array* dw_up,
+    zg_device_array* dw_down) {
+    const char* op = "gated_ff_backward";
+    if (!k || !dev || !pool || !dx || !dw_gate || !dw_up || !dw_down)
+        return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
+    FfShapes s;
+    int rc = ff_shapes(x, w_gate, w_down, op, &s);
+    if (rc) return rc;
+    std::lock_guard<std::recursive_mutex> lk(dev->mu);
+    if ((rc = set_device(dev))) return rc;
+    void *px, *pg, *pu, *pd, *pdy, *pre[2], *po[4];
+    const uint32_t xs[2] = {s.m, s.k}, gs[2] = {s.k, s.f}, ds[2] = {s.f, s.d}, ys[2] = {s.m, s.d},
+                   ps[2] = {s.m, s.f};
+    if ((rc = array_ptr(dev, dy, s.dtype, 2, ys, op, "dy", &pdy)) ||
+        (rc = array_ptr(dev, x, s.dtype, 2, xs, op, "x", &px)) ||
+        (rc = array_ptr(dev, w_gate, s.dtype, 2, gs, op, "w_gate", &pg)) ||
+        (rc = array_ptr(dev, w_up, s.dtype, 2, gs, op, "w_up", &pu)) ||
+        (rc = array_ptr(dev, w_down, s.dtype, 2, ds, op, "w_down", &pd)) ||
+        (rc = array_ptr(dev, pre_gate, ZG_DTYPE_F32, 2, ps, op, "pre_gate", &pre[0])) ||
+        (rc = array_ptr(dev, pre_up, ZG_DTYPE_F32, 2, ps, op, "pre_up", &pre[1])))
+        return rc;
+    const uint64_t ws = zg_gated_ff_workspace_bytes(s.dtype, k->mode, s.m, s.k, s.f, s.d, 1);
+    if ((rc = ensure_workspace(dev, ws))) return rc;
+    PoolOutputs outs{pool, {}};
+    zg_device_array* o[4] = {dx, dw_gate, dw_up, dw_down};
+    const uint32_t* shapes[4] = {xs, gs, gs, ds};
+    for (int i = 0; i < 4; ++i)
+        if ((rc = outs.alloc(shapes[i][0], shapes[i][1], s.dtype, o[i])) ||
+            (rc = array_ptr(dev, o[i], s.dtype, 2, shapes[i], op, "output", &po[i])))
+            return outs.fail(rc);
+    if ((rc = zg_gated_ff_backward(s.dtype, k->mode, act, s.m, s.k, s.f, s.d, pdy, px, pg, pu, pd,
+                                   static_cast<float*>(pre[0]), static_cast<float*>(pre[1]), po[0],
+                                   po[1], po[2], po[3], dev->workspace, dev->workspace_bytes,
+                                   dev->stream))) {
+        cudaStreamSynchronize(dev->stream);
+        return outs.fail(rc);
+    }
+    return finish_op(dev, pool->memory == ZG_MEMORY_GPU_ONLY);
+}
+
+extern "C" int zg_level1_adamw(zg_device* dev, uint32_t count, const zg_device_array* params,
+                               const zg_device_array* grads, const zg_device_array* master,
+                               const zg_device_array* exp_avg, const zg_device_array* exp_avg_sq,
+                               const zg_device_array* exp_avg_scale,
+                               const zg_device_array* exp_avg_sq_scale, const zg_adamw_hyper* h,
+                               const zg_device_array* norm_scale) {
+    const char* op = "adamw";
+    if (!dev || !h || (count && (!params || !grads || !exp_avg || !exp_avg_sq)))
+        return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
+    if (count == 0) return ZG_OK;
+    int rc;
+    const uint32_t state = exp_avg[0].dtype;
+    if (state != ZG_DTYPE_F32 && state != ZG_DTYPE_U8)
+        return set_error(ZG_ERR_DISPATCH, "%s: moments are f32, or u8 codes, got %s", op,
+                         dtype_name(state));
+    if (state == ZG_DTYPE_U8 && (!exp_avg_scale || !exp_avg_sq_scale))
+        return set_error(ZG_ERR_DISPATCH, "%s: moments in u8 codes need their scales", op);
+    std::lock_guard<std::recursive_mutex> lk(dev->mu);
+    if ((rc = set_device(dev))) return rc;
+    std::vector<zg_adamw_tensor> t(count);
+    std::vector<uint32_t> written, read;
+    bool deferred = true;
+    for (uint32_t i = 0; i < count; ++i) {
+        const zg_device_array& p = params[i];
+        if ((rc = check_array(&p, op))) return rc;
+        uint32_t n = 0;
+        if (!array_len(&p, &n)) return set_error(ZG_ERR_DISPATCH, "%s: length overflows u32", op);
+        const uint32_t blocks = n / ZG_ADAMW_BLOCK + (n % ZG_ADAMW_BLOCK != 0);
+        t[i] = {};
+        t[i].n = n;
+        void *g = nullptr, *ms = nullptr, *vs = nullptr;
+        if ((rc = array_ptr(dev, &p, params[0].dtype, p.rank, p.shape, op, "weight", &t[i].param)) ||
+            (rc = array_ptr(dev, &grads[i], grads[0].dtype, p.rank, p.shape, op, "gradient", &g)) ||
+            (rc = array_ptr(dev, &exp_avg[i], state, p.rank, p.shape, op, "exp_avg", &t[i].exp_avg)) ||
+            (rc = array_ptr(dev, &exp_avg_sq[i], state, p.rank, p.shape, op, "exp_avg_sq",
+                            &t[i].exp_avg_sq)) ||
+            (master && (rc = array_ptr(dev, &master[i], ZG_DTYPE_F32, p.rank, p.shape, op, "master",
+                                       &t[i].master))))
+            return rc;
+        t[i].grad = g;
+        if (state == ZG_DTYPE_U8) {
+            if ((rc = array_ptr(dev, &exp_avg_scale[i], ZG_DTYPE_F32, 1, &blocks, op,
+                                "exp_avg_scale", &ms)) ||
+                (rc = array_ptr(dev, &exp_avg_sq_scale[i], ZG_DTYPE_F32, 1, &blocks, op,
+                                "exp_avg_sq_scale", &vs)))
+                return rc;
+            t[i].exp_avg_scale = static_cast<float*>(ms);
+            t[i].exp_avg_sq_scale = static_cast<float*>(vs);
+        }
+        if (n) {
+            read.push_back(grads[i].buffer.index);
+            for (const zg_device_array* a : {&p, &exp_avg[i], &exp_avg_sq[i]})
+                written.push_back(a->buffer.index);
+            if (master) written.push_back(master[i].buffer.index);
+            if (state == ZG_DTYPE_U8) {
+                written.push_back(exp_avg_scale[i].buffer.index);
+                written.push_back(exp_avg_sq_scale[i].buffer.index);
+            }
+        }
+        deferred = deferred && buffer_memory(dev, p.buffer) == ZG_MEMORY_GPU_ONLY;
+    }
+    std::sort(written.begin(), written.end());
+    bool twice = std::adjacent_find(written.begin(), written.end()) != written.end();
+    for (uint32_t g : read) twice = twice || std::binary_search(written.begin(), written.end(), g);
+    if (twice) return set_error(ZG_ERR_DISPATCH, "%s: one buffer is bound twice", op);
+    const float* scale = nullptr;
+    if (norm_scale) {
+        const uint32_t two = 2;
+        void* p = nullptr;
+        if ((rc = array_ptr(dev, norm_scale, ZG_DTYPE_F32, 1, &two, op, "norm_scale", &p))) return rc;
+        scale = static_cast<const float*>(p) + 1;
+    }
+    if ((rc = zg_adamw(params[0].dtype, grads[0].dtype, state == ZG_DTYPE_U8 ? 8 : 32, count,
+                       t.data(), h, nullptr, nullptr, scale, dev->stream)))
+        return rc;
+    return deferred ? ZG_OK : finish_sync(dev, false);
+}
+
+extern "C" int zg_level1_grad_norm(zg_device* dev, zg_pool* pool, uint32_t count,
+                                   const zg_device_array* grads, double max_norm,
+                                   zg_device_array* out) {
+    const char* op = "grad_norm";
+    if (!dev || !pool || !out || (count && !grads))
+        return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
+    int rc;
+    std::lock_guard<std::recursive_mutex> lk(dev->mu);
+    if ((rc = set_device(dev))) return rc;
+    std::vector<const void*> ptrs(count);
+    std::vector<uint64_t> sizes(count);
+    for (uint32_t i = 0; i < count; ++i) {
+        if ((rc = check_array(&grads[i], op))) return rc;
+        uint32_t n = 0;
+        void* p = nullptr;
+        if ((rc = array_ptr(dev, &grads[i], grads[0].dtype, grads[i].rank, grads[i].shape, op,
+                            "gradient", &p)))
+            return rc;
+        array_len(&grads[i], &n);
+        ptrs[i] = p;
+        sizes[i] = n;
+    }
+    const uint64_t ws = zg_grad_norm_workspace_bytes(count);
+    if ((rc = ensure_workspace(dev, ws))) return rc;
+    const uint32_t two = 2;
+    if ((rc = zg_pool_alloc(pool, &two, 1, ZG_DTYPE_F32, out))) return rc;
+    void* po = nullptr;
+    if ((rc = array_ptr(dev, out, ZG_DTYPE_F32, 1, &two, op, "out", &po)) ||
+        (rc = zg_grad_norm(count ? grads[0].dtype : ZG_DTYPE_F32, count, ptrs.data(), sizes.data(),
+                           max_norm, static_cast<float*>(po), dev->workspace, dev->workspace_bytes,
+                           dev->stream))) {
+        zg_pool_free(pool, out);
+        return rc;
+    }
+    return pool->memory == ZG_MEMORY_GPU_ONLY ? ZG_OK : finish_sync(dev, false);
+}
+
+// ======================================================================
 // Pipelined GEMM on host arrays
 // ======================================================================
 

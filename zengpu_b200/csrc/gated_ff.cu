@@ -291,7 +291,7 @@ struct Planes {
     }
     void gemm(const OperandView& a, const OperandView& b, int M, int N, int K, float* out) {
         if (ws && !rc)
-            rc = gemm_run({c.mode, a, b}, M, N, K, 1.0f, out, N, nullptr, 0, s, nullptr, true);
+            rc = gemm_run({c.mode, a, b}, M, N, K, 1.0f, out, N, nullptr, 0, s);
     }
 };
 
@@ -348,8 +348,76 @@ struct F32Tensors {
     float *pre_g, *pre_u, *y, *dx, *dwg, *dwu, *dwd;
 };
 
+// TF32X3 runs on the block's own kernels (gated_ff_f32.cu); the other modes, which
+// are chosen for speed over accuracy or for comparison, on sgemm's.
+FfOperand operand(const OperandView& v) { return {v.p, v.ld, false}; }
+
+uint64_t tf32x3_forward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s,
+                        int* rc) {
+    Planes p{c, ws, 0, s};
+    const OperandView x = p.of(t.x, c.m, c.k, false), wg = p.of(t.wg, c.f, c.k, true),
+                      wu = p.of(t.wu, c.f, c.k, true), wd = p.of(t.wd, c.d, c.f, true),
+                      h = gemm_carve_planes(p.take(gemm_planes_bytes(c.mode, c.m, c.f)), c.mode,
+                                            c.m, c.f);
+    // counted without pre-activations given: the case that takes more
+    float* pre[2] = {ws && t.pre_g ? t.pre_g : p.matrix(c.m, c.f),
+                     ws && t.pre_g ? t.pre_u : p.matrix(c.m, c.f)};
+    FfProduct gu[2], y;
+    for (int i = 0; i < 2; ++i) {
+        gu[i].M = c.m, gu[i].N = gu[i].ldc = c.f, gu[i].k[0] = c.k;
+        gu[i].a[0] = operand(x), gu[i].b[0] = operand(i ? wu : wg), gu[i].c = pre[i];
+    }
+    shape_y(c, y);
+    y.a[0] = operand(h), y.b[0] = operand(wd), y.c = t.y;
+    float* parts = static_cast<float*>(
+        p.take(std::max(ff_f32_split_bytes(gu, 2), ff_f32_split_bytes(&y, 1))));
+    if (ws && !p.rc) p.rc = ff_f32(gu, 2, parts, s);
+    if (ws && !p.rc) p.rc = ff_f32_act(c.act, pre[0], pre[1], c.m, c.f, operand(h), s);
+    if (ws && !p.rc) p.rc = ff_f32(&y, 1, parts, s);
+    *rc = p.rc;
+    return p.used;
+}
+
+uint64_t tf32x3_backward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s,
+                         int* rc) {
+    Planes p{c, ws, 0, s};
+    const OperandView dy = p.of(t.dy, c.m, c.d, false), wd = p.of(t.wd, c.f, c.d, false),
+                      w = p.beside(t.wg, t.wu, c.k, c.f), xt = p.of(t.x, c.k, c.m, true),
+                      dyt = p.of(t.dy, c.d, c.m, true);
+    OperandView dg = gemm_carve_planes(nullptr, c.mode, c.m, c.f), du = dg;
+    dg.ld = du.ld = 2 * dg.ld;
+    dg.p = p.take(static_cast<uint64_t>(c.m) * dg.ld * 4);
+    du.p = static_cast<float*>(dg.p) + (ws ? dg.ld / 2 : 0);
+    FfOperand turned[3];  // dg, du, h
+    for (FfOperand& o : turned)
+        o = operand(gemm_carve_planes(p.take(gemm_planes_bytes(c.mode, c.f, c.m)), c.mode, c.f, c.m));
+    float* dh = p.matrix(c.m, c.f);
+    FfProduct h, dx, dw[3];
+    h.M = c.m, h.N = h.ldc = c.f, h.k[0] = c.d;
+    h.a[0] = operand(dy), h.b[0] = operand(wd), h.c = dh;
+    shape_dx(c, dx), shape_dw(c, dw);
+    dx.k[0] = 2 * gemm_planes_k(c.mode, c.f), dx.k[1] = 0;
+    dx.a[0] = operand(dg), dx.b[0] = operand(w), dx.c = t.dx;
+    dw[0].a[0] = dw[1].a[0] = operand(xt);
+    dw[0].b[0] = turned[0], dw[0].c = t.dwg;
+    dw[1].b[0] = turned[1], dw[1].c = t.dwu;
+    dw[2].a[0] = turned[2], dw[2].b[0] = operand(dyt), dw[2].c = t.dwd;
+    float* parts = static_cast<float*>(
+        p.take(std::max({ff_f32_split_bytes(&h, 1), ff_f32_split_bytes(&dx, 1),
+                         ff_f32_split_bytes(dw, 3)})));
+    if (ws && !p.rc) p.rc = ff_f32(&h, 1, parts, s);
+    if (ws && !p.rc)
+        p.rc = ff_f32_slope(c.act, t.pre_g, t.pre_u, dh, c.m, c.f, operand(dg), operand(du),
+                            turned, s);
+    if (ws && !p.rc) p.rc = ff_f32(&dx, 1, parts, s);
+    if (ws && !p.rc) p.rc = ff_f32(dw, 3, parts, s);
+    *rc = p.rc;
+    return p.used;
+}
+
 // Runs the pass; with ws null only counts the workspace it takes.
 uint64_t f32_forward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s, int* rc) {
+    if (c.mode == ZG_GEMM_TF32X3) return tf32x3_forward(c, t, ws, s, rc);
     Planes p{c, ws, 0, s};
     // counted without pre-activations given: the case that takes more
     float* g = ws && t.pre_g ? t.pre_g : p.matrix(c.m, c.f);
@@ -366,6 +434,7 @@ uint64_t f32_forward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStre
 }
 
 uint64_t f32_backward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cudaStream_t s, int* rc) {
+    if (c.mode == ZG_GEMM_TF32X3) return tf32x3_backward(c, t, ws, s, rc);
     Planes p{c, ws, 0, s};
     float *dg = p.matrix(c.m, c.f), *du = p.matrix(c.m, c.f), *h = p.matrix(c.m, c.f);
     p.gemm(p.of(t.dy, c.m, c.d, false), p.of(t.wd, c.f, c.d, false), c.m, c.f, c.d, dg);  // dh
@@ -398,7 +467,7 @@ int check_call(FfCall& c, const char* what) {
 }
 
 uint64_t ff_workspace(const FfCall& c) {
-    if (!f32_tensor(c)) return ff_layout(c).total;
+    if (!f32_tensor(c) || (!c.backward && c.m <= kFfRowsF32)) return ff_layout(c).total;
     int rc;
     return c.backward ? f32_backward(c, {}, nullptr, nullptr, &rc)
                       : f32_forward(c, {}, nullptr, nullptr, &rc);
@@ -460,7 +529,7 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
                          "gated_ff: pre_gate and pre_up are both null or both 16-byte aligned");
     if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff"))) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (f32_tensor(c)) {
+    if (f32_tensor(c) && m > kFfRowsF32) {
         F32Tensors t{};
         t.x = static_cast<const float*>(x), t.wg = static_cast<const float*>(w_gate);
         t.wu = static_cast<const float*>(w_up), t.wd = static_cast<const float*>(w_down);
@@ -479,15 +548,18 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
     p.b[1] = {in[kWu].p, in[kWu].ld, true};
     p.c = workspace, p.ldc = l.ld_f;
     p.pre_g = pre_gate, p.pre_u = pre_up;
-    const bool few = c.size == 2 && m <= kFfRows;
     void* parts = static_cast<uint8_t*>(workspace) + l.parts;
-    if ((rc = few ? ff_rows(dtype, true, act, p, s) : products(c, kFfGated, &p, 1, nullptr, s))) return rc;
+    const bool few = m <= (c.size == 2 ? kFfRows : kFfRowsF32);
+    auto rows = [&](bool gated, const FfProduct& f) {
+        return c.size == 2 ? ff_rows(dtype, gated, act, f, s) : ff_rows_f32(gated, act, f, s);
+    };
+    if ((rc = few ? rows(true, p) : products(c, kFfGated, &p, 1, nullptr, s))) return rc;
     FfProduct q;
     shape_y(c, q);
     q.a[0] = {workspace, l.ld_f, false};
     q.b[0] = {in[kWd].p, in[kWd].ld, true};
     q.c = y;
-    return few ? ff_rows(dtype, false, act, q, s) : products(c, kFfStore, &q, 1, parts, s);
+    return few ? rows(false, q) : products(c, kFfStore, &q, 1, parts, s);
 }
 
 extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f, int d,

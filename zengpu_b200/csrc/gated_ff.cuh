@@ -127,10 +127,26 @@ uint64_t ff_split_bytes(const FfProduct* products, int count);
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
             float* parts, cudaStream_t s);
 
+// f32 tensors in the TF32X3 mode (gated_ff_f32.cu), operands as planes (sgemm_tc.cu,
+// k-major, ld in floats), k[0] the sum's length; kFfStore only, parts as ff_pair's.
+int ff_f32_splits(const FfProduct* products, int count);
+uint64_t ff_f32_split_bytes(const FfProduct* products, int count);
+int ff_f32(const FfProduct* products, int count, float* parts, cudaStream_t s);
+// h = act(g) u as planes [m, n]; dg and du as planes, and dg, du and h transposed.
+int ff_f32_act(int act, const float* g, const float* u, int m, int n, const FfOperand& h,
+               cudaStream_t s);
+int ff_f32_slope(int act, const float* g, const float* u, const float* dh, int m, int n,
+                 const FfOperand& dg, const FfOperand& du, const FfOperand (&turned)[3],
+                 cudaStream_t s);
+
 // The forward products for up to kFfRows rows of 16-bit tensors (gated_ff_rows.cu):
 // `gated` as kFfGated, else as kFfStore of one product, launched right behind the
 // gated one whose result it reads.
 constexpr int kFfRows = 128;
 int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& product, cudaStream_t s);
+
+// The same for f32 tensors, on the CUDA cores (gated_ff_rows_f32.cu).
+constexpr int kFfRowsF32 = 64;
+int ff_rows_f32(bool gated, int act, const FfProduct& product, cudaStream_t s);
 
 }  // namespace zg

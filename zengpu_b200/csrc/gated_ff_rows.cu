@@ -62,18 +62,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t mine, uint32_t rank)
     return v;
 }
 
-__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
-        " {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-
 __host__ __device__ constexpr uint32_t tmem_columns(int n) {
     return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
 }
@@ -217,8 +205,8 @@ __global__ void __launch_bounds__(kRowsThreads)
             for (int r0 = 0; r0 < ROWS; r0 += 16) {
                 if (r0 >= args.M) break;
                 uint32_t g[16], u[16];
-                tmem_ld_16(lanes + r0, g);
-                if (GATED) tmem_ld_16(lanes + ROWS + r0, u);
+                tmem_ld_32x32b_x16(lanes + r0, g);
+                if (GATED) tmem_ld_32x32b_x16(lanes + ROWS + r0, u);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     finish(r0 + i, n0 + column, __uint_as_float(g[i]),
@@ -237,7 +225,7 @@ __global__ void __launch_bounds__(kRowsThreads)
                 for (int r0 = 0; r0 < ROWS; r0 += 16) {
                     if (r0 >= args.M) break;
                     uint32_t v[16];
-                    tmem_ld_16(lanes + w * ROWS + r0, v);
+                    tmem_ld_32x32b_x16(lanes + w * ROWS + r0, v);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         part[(w * ROWS + r0 + i) * kColumns + column] = __uint_as_float(v[i]);

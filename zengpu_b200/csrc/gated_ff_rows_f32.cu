@@ -1,0 +1,246 @@
+// gated_ff_rows_f32.cu - the forward products of the gated feed-forward block for
+// few rows of f32 tensors, on the CUDA cores: every weight is read once, as it lies
+// (any size, any pitch), where the tensor-core modes would first write it out again
+// as operand planes.  Every mode takes this form for up to kFfRowsF32 rows; its sums
+// are plain f32 FMAs.
+//
+// A CTA takes 128 columns of W (of Wg and of Wu for the gated product) and a part of
+// the sum; the CTAs of a cluster share the columns and split the sum.  Weights and
+// the transposed piece of x come through a ring of stages of 16 of the sum
+// (cp.async, 16 bytes where the pitch allows it, else 4).  A lane holds four columns;
+// the eight warps are dealt out to groups of eight rows and, where there are fewer,
+// to parts of the stage: 8 rows x 4 columns x 2 products a thread, 64 FMAs for four
+// 16-byte reads of shared memory.  Partial results meet in shared memory, across the
+// cluster as in gated_ff_rows.cu, in a fixed order.
+//
+// Up to 16 rows the weights' 4 bytes each bound it; beyond, the f32 pipe (8 rows a
+// weight take 16 cycles of an SM's 128 lanes for 1 KB of weights, which HBM delivers
+// in 44).
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "gated_ff.cuh"
+
+namespace zg {
+namespace {
+
+constexpr int kRThreads = 256, kRWarps = 8, kRCols = 128, kRStep = 16, kRStages = 5;
+
+struct RowsF32Args {
+    const float* x;
+    const float* w[2];
+    float* c;
+    float* pre_g;
+    float* pre_u;
+    int64_t ldx, ldw, ldc;
+    int M, N, K;
+    int vec;  // w: 16-byte aligned rows
+};
+
+__device__ __forceinline__ void copy16(uint32_t to, const float* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from),
+                 "r"(in ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const float* from, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from),
+                 "r"(in ? 4 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ float4 ld_rank(uint32_t mine, uint32_t rank) {
+    float4 v;
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(mine), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
+
+// ROWS: 8, 16, 32 or 64.
+template <bool GATED, int ACT, int ROWS>
+__global__ void __launch_bounds__(kRThreads)
+    ff_rows_f32_kernel(const RowsF32Args a) {
+    constexpr int kMats = GATED ? 2 : 1;
+    constexpr int kRowGroups = ROWS / 8, kSumGroups = kRWarps / kRowGroups;
+    constexpr int kWFloats = kMats * kRStep * kRCols, kXFloats = kRStep * ROWS;
+    constexpr int kStageFloats = kWFloats + kXFloats;
+    extern __shared__ float4 ring4[];
+    float* ring = reinterpret_cast<float*>(ring4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = gridDim.x, rank = blockIdx.x;
+    const int n0 = blockIdx.y * kRCols;
+    const int steps = (a.K + kRStep - 1) / kRStep;
+    const int s0 = static_cast<int>(static_cast<int64_t>(steps) * rank / split);
+    const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / split);
+    const int row0 = warp % kRowGroups * 8, part = warp / kRowGroups;
+
+    auto load = [&](int step) {
+        if (step < s1) {
+            const uint32_t st = smem_u32(ring + (step - s0) % kRStages * kStageFloats);
+            const int k0 = step * kRStep;
+            if (a.vec) {
+#pragma unroll
+                for (int j = threadIdx.x; j < kWFloats / 4; j += kRThreads) {
+                    const int w = j / (kRStep * kRCols / 4), k = j / (kRCols / 4) % kRStep;
+                    const int c = j % (kRCols / 4) * 4;
+                    const bool in = k0 + k < a.K && n0 + c < a.N;
+                    copy16(st + j * 16, in ? a.w[w] + (k0 + k) * a.ldw + n0 + c : a.w[0], in);
+                }
+            } else {
+                for (int j = threadIdx.x; j < kWFloats; j += kRThreads) {
+                    const int w = j / (kRStep * kRCols), k = j / kRCols % kRStep;
+                    const int c = j % kRCols;
+                    const bool in = k0 + k < a.K && n0 + c < a.N;
+                    copy4(st + j * 4, in ? a.w[w] + (k0 + k) * a.ldw + n0 + c : a.w[0], in);
+                }
+            }
+            for (int j = threadIdx.x; j < kXFloats; j += kRThreads) {
+                const int k = j % kRStep, r = j / kRStep;
+                const bool in = k0 + k < a.K && r < a.M;
+                copy4(st + (kWFloats + k * ROWS + r) * 4, in ? a.x + r * a.ldx + k0 + k : a.x, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    float acc[kMats][8][4] = {};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = 0; i < kRStages - 1; ++i) load(s0 + i);
+    for (int step = s0; step < s1; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRStages - 2) : "memory");
+        __syncthreads();  // the stage has landed, and the one before it is free
+        load(step + kRStages - 1);
+        const float* st = ring + (step - s0) % kRStages * kStageFloats;
+#pragma unroll 4
+        for (int i = 0; i < kRStep / kSumGroups; ++i) {
+            const int k = part + i * kSumGroups;
+            float x[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 v =
+                    *reinterpret_cast<const float4*>(st + kWFloats + k * ROWS + row0 + 4 * h);
+                x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+            }
+#pragma unroll
+            for (int w = 0; w < kMats; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(st + (w * kRStep + k) * kRCols +
+                                                                  lane * 4);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    acc[w][r][0] = fmaf(x[r], v.x, acc[w][r][0]);
+                    acc[w][r][1] = fmaf(x[r], v.y, acc[w][r][1]);
+                    acc[w][r][2] = fmaf(x[r], v.z, acc[w][r][2]);
+                    acc[w][r][3] = fmaf(x[r], v.w, acc[w][r][3]);
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    // partial results [sum group][product][row][column] take the ring's place
+#pragma unroll
+    for (int w = 0; w < kMats; ++w)
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            *reinterpret_cast<float4*>(ring + ((part * kMats + w) * ROWS + row0 + r) * kRCols +
+                                       lane * 4) =
+                make_float4(acc[w][r][0], acc[w][r][1], acc[w][r][2], acc[w][r][3]);
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    const uint32_t at = smem_u32(ring) + lane * 16;
+    for (int row = rank + split * warp; row < a.M; row += split * kRWarps) {
+        float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f), u = g;
+        for (int p = 0; p < split; ++p)
+#pragma unroll
+            for (int q = 0; q < kSumGroups; ++q) {
+                const float4 v = ld_rank(at + (q * kMats * ROWS + row) * kRCols * 4, p);
+                g.x += v.x, g.y += v.y, g.z += v.z, g.w += v.w;
+                if (GATED) {
+                    const float4 z = ld_rank(at + ((q * kMats + 1) * ROWS + row) * kRCols * 4, p);
+                    u.x += z.x, u.y += z.y, u.z += z.z, u.w += z.w;
+                }
+            }
+        const float gs[4] = {g.x, g.y, g.z, g.w}, us[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int col = n0 + lane * 4 + e;
+            if (col >= a.N) break;
+            if (GATED && a.pre_g) {
+                const int64_t pre = static_cast<int64_t>(row) * a.N + col;
+                a.pre_g[pre] = gs[e];
+                a.pre_u[pre] = us[e];
+            }
+            a.c[row * a.ldc + col] = GATED ? activate<ACT, false>(gs[e]).a * us[e] : gs[e];
+        }
+    }
+    if (split > 1) cluster_sync();  // nobody leaves while its memory is read
+}
+
+template <bool GATED, int ACT, int ROWS>
+int launch_rows(const RowsF32Args& a, cudaStream_t s) {
+    constexpr int kMats = GATED ? 2 : 1;
+    constexpr int kSmem = std::max(kRStages * (kMats * kRStep * kRCols + kRStep * ROWS),
+                                   kMats * 8 * kRWarps * kRCols) * 4;
+    const int tiles = (a.N + kRCols - 1) / kRCols, steps = (a.K + kRStep - 1) / kRStep;
+    int split = 1;
+    // two CTAs of an SM, a few stages for each part of the sum at least
+    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= steps) split *= 2;
+    auto kernel = ff_rows_f32_kernel<GATED, ACT, ROWS>;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    }
+    if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, tiles);
+    cfg.blockDim = dim3(kRThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), "gated_ff rows");
+}
+
+template <bool GATED, int ACT>
+int launch_rows_n(const RowsF32Args& a, cudaStream_t s) {
+    if (a.M <= 8) return launch_rows<GATED, ACT, 8>(a, s);
+    if (a.M <= 16) return launch_rows<GATED, ACT, 16>(a, s);
+    if (a.M <= 32) return launch_rows<GATED, ACT, 32>(a, s);
+    return launch_rows<GATED, ACT, 64>(a, s);
+}
+
+}  // namespace
+
+int ff_rows_f32(bool gated, int act, const FfProduct& f, cudaStream_t s) {
+    RowsF32Args a{};
+    a.x = static_cast<const float*>(f.a[0].p), a.ldx = f.a[0].ld;
+    a.w[0] = static_cast<const float*>(f.b[0].p), a.w[1] = static_cast<const float*>(f.b[1].p);
+    a.ldw = f.b[0].ld;
+    a.c = static_cast<float*>(f.c), a.ldc = f.ldc;
+    a.pre_g = f.pre_g, a.pre_u = f.pre_u;
+    a.M = f.M, a.N = f.N, a.K = f.k[0];
+    a.vec = a.ldw % 4 == 0 &&
+            ((reinterpret_cast<uintptr_t>(a.w[0]) | reinterpret_cast<uintptr_t>(a.w[1])) & 15) == 0;
+    if (!gated) return launch_rows_n<false, ZG_ACT_RELU>(a, s);
+    switch (act) {
+        case ZG_ACT_SILU: return launch_rows_n<true, ZG_ACT_SILU>(a, s);
+        case ZG_ACT_GELU: return launch_rows_n<true, ZG_ACT_GELU>(a, s);
+        case ZG_ACT_GELU_TANH: return launch_rows_n<true, ZG_ACT_GELU_TANH>(a, s);
+        default: return launch_rows_n<true, ZG_ACT_RELU>(a, s);
+    }
+}
+
+}  // namespace zg

@@ -37,7 +37,7 @@
 #include <cstdint>
 #include <cstring>
 
-#include "gated_ff.cuh"
+#include "gated_ff_pair.cuh"
 #include "zg_gemm_internal.h"
 
 namespace zg {
@@ -51,11 +51,6 @@ constexpr int kStageBytes = 2 * kOperandBytes; // A and B: 32 KB per CTA
 // Stages: five; dh's epilogue, which also holds blocks of g and u, leaves room for
 // four.
 constexpr int kStageCount[3] = {5, 5, 4};
-// An epilogue warp turns blocks of 32 x 32 between "a row per lane" (TMEM) and
-// "neighbours along a row" (memory) through shared memory of its own, with rows of
-// 144 bytes (f32) or 80 (16 bits): an odd number of 16-byte pieces, so that accesses
-// of either kind meet no bank twice.
-template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
 constexpr int kBlock32 = 32 * kPitch<float>;
 constexpr int kBlock16 = 32 * kPitch<__half>;
 constexpr int kTurnBytes[3] = {kBlock32, kBlock32, kBlock16 + 2 * kBlock32};
@@ -65,8 +60,6 @@ constexpr int smem_bytes(int epi) {
 }
 static_assert(smem_bytes(2) <= 232448, "shared memory of an SM");
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxProblems = 3;
-constexpr int kPairsSold = 74;  // SM pairs of a B200: what split sums are dealt out for
 
 struct alignas(64) PairProblem {
     CUtensorMap a[2], b[2];
@@ -115,14 +108,6 @@ __device__ __forceinline__ void load_operand(uint8_t* smem, const CUtensorMap* m
         tma_load_2d_pair(smem + b * 128, map, mn ? r0 + b : i0, mn ? i0 : r0 + b, bar);
 }
 
-// Grouped raster, as the f32 kernels' (eight row tiles before the next column).
-__device__ __forceinline__ void raster(int tile, int mt, int nt, int& mi, int& ni) {
-    const int group = tile / (8 * nt), first = group * 8;
-    const int gm = min(mt - first, 8), r = tile - group * 8 * nt;
-    mi = first + r % gm;
-    ni = r / gm;
-}
-
 // A unit of work: a tile, or a column half of one of the last tiles.
 struct Unit {
     const PairProblem* p;
@@ -160,35 +145,6 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
     uint32_t w;
     __builtin_memcpy(&w, t, 4);
     return w;
-}
-
-// Stores a warp's 32 x 32 block of T, row `lane` in the words of v, at `dst` (its
-// row 0, column 0); `rows` and `cols` of it lie inside the matrix.  vec: 16-byte
-// pieces of rows; otherwise (odd pitch or base) one element a lane, neighbours
-// side by side.
-template <class T>
-__device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int cols, bool vec,
-                                            const uint32_t (&v)[8 * sizeof(T)], uint8_t* turn,
-                                            int lane) {
-    constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer, kTurnPitch = kPitch<T>;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-        *reinterpret_cast<uint4*>(turn + lane * kTurnPitch + i * 16) =
-            make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    __syncwarp();
-    if (vec) {
-#pragma unroll
-        for (int j = 0; j < kPieces; ++j) {
-            const int r = (j * 32 + lane) / kPieces, piece = lane % kPieces;
-            if (r < rows && piece * kPer < cols)
-                *reinterpret_cast<uint4*>(dst + r * ld + piece * kPer) =
-                    *reinterpret_cast<const uint4*>(turn + r * kTurnPitch + piece * 16);
-        }
-    } else if (lane < cols) {
-        for (int r = 0; r < rows; ++r)
-            dst[r * ld + lane] = reinterpret_cast<const T*>(turn + r * kTurnPitch)[lane];
-    }
 }
 
 // The reverse for f32, asynchronous: copies the block's rows into `turn`, zeros
@@ -448,77 +404,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
-// Adds up the parts of split sums, in order, and rounds: four elements a thread.
-struct SumArgs {
-    struct {
-        const float* part;
-        void* c;
-        int64_t plane, groups;  // groups of this matrix and those before it
-        int N, ldp;
-    } m[kMaxProblems];
-    int count, splits;
-};
-template <class T>
-__global__ void __launch_bounds__(256) ff_sum_kernel(const __grid_constant__ SumArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-    for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-         g < a.m[a.count - 1].groups; g += step) {
-        int i = 0;
-        while (g >= a.m[i].groups) ++i;
-        const auto& m = a.m[i];
-        const int64_t at = (g - (i ? a.m[i - 1].groups : 0)) * 4;
-        const int64_t row = at / m.ldp;
-        const int col = static_cast<int>(at - row * m.ldp);
-        float4 sum = __ldcs(reinterpret_cast<const float4*>(m.part + at));
-        for (int s = 1; s < a.splits; ++s) {
-            const float4 x = __ldcs(reinterpret_cast<const float4*>(m.part + s * m.plane + at));
-            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-        }
-        T* c = static_cast<T*>(m.c) + row * m.N + col;
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        if (m.N % 4 == 0 && (reinterpret_cast<uintptr_t>(m.c) & 7) == 0) {
-            T t[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = FfElem<T>::put(v[e]);
-            uint2 q;
-            __builtin_memcpy(&q, t, 8);
-            *reinterpret_cast<uint2*>(c) = q;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < m.N) c[e] = FfElem<T>::put(v[e]);
-        }
-    }
-}
-
 // ---- host ----------------------------------------------------------------------
-int sm_pairs() {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return std::max((sms > 0 ? sms : 148) / 2, 1);
-}
-
 // An operand as 64 x 64 boxes: inner dimension along the memory.
 int operand_map(CUtensorMap* map, uint32_t dtype, const FfOperand& o, int rows, int sum) {
     return encode_16bit_map(map, dtype, o.p, o.mn ? rows : sum, o.mn ? sum : rows, o.ld, kBox, kBox);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 template <int EPI, int ACT, class T>
 int launch(const PairArgs& args, int units, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
-    if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(ff_pair_kernel<EPI, ACT, T>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 smem_bytes(EPI));
-        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-    }
+    const cudaError_t e = allow_smem(ff_pair_kernel<EPI, ACT, T>, smem_bytes(EPI), done);
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
     return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T>, 2 * std::min(units, sm_pairs()),
                             kThreads, smem_bytes(EPI), s, args);
@@ -543,25 +438,10 @@ int launch_epi(FfEpilogue epi, int act, const PairArgs& a, int units, cudaStream
 
 }  // namespace
 
-int ff_splits(const FfProduct* products, int count) {
-    int64_t tiles = 0;
-    int nkb = 1 << 30;
-    for (int i = 0; i < count; ++i) {
-        const FfProduct& f = products[i];
-        tiles += static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256);
-        nkb = std::min(nkb, (f.k[0] + kBK - 1) / kBK + (f.k[1] + kBK - 1) / kBK);
-    }
-    return static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>({4, kPairsSold / std::max<int64_t>(tiles, 1), nkb / 8})));
-}
+int ff_splits(const FfProduct* products, int count) { return splits_of(products, count, kBK); }
 
 uint64_t ff_split_bytes(const FfProduct* products, int count) {
-    const int splits = ff_splits(products, count);
-    if (splits == 1) return 0;
-    uint64_t elems = 0;
-    for (int i = 0; i < count; ++i)
-        elems += static_cast<uint64_t>(products[i].M) * ((products[i].N + 3) / 4 * 4);
-    return elems * splits * 4;
+    return split_bytes(products, count, ff_splits(products, count));
 }
 
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,

@@ -88,14 +88,6 @@ constexpr uint32_t kTmemCols = 512;              // two BN-column accumulators
 
 // Per-scheme stage geometry: every operand row of a stage is 128 bytes (BK
 // values of k: 32 f32 for TF32, 16 interleaved split values otherwise).
-// S = 5 is TF32X3 (S = 2) with accumulators drained every 64 of k instead of 512:
-// 24 truncating additions between roundings to nearest instead of 192, for callers
-// that chain products (the gated feed-forward block) and want f32's own accuracy.
-// A chunk's MMAs take about 3000 cycles, its drain 500 beside them, so the speed is
-// the same.
-template <int S>
-constexpr int kChunkK = S == 5 ? 64 : 512;
-
 template <int S>
 struct TcCfg {
     static constexpr int BK = (S == 1 || S == 4) ? 32 : 16;  // k per stage
@@ -108,7 +100,7 @@ struct TcCfg {
     // k-blocks per TMEM accumulation chunk: 512 of k for the split modes
     // (keeps the accumulator's truncation error near 3e-6 relative); TF32
     // (tolerance 5e-3) accumulates the whole k range in TMEM.
-    static constexpr int KB_PER_CHUNK = S >= 2 ? kChunkK<S> / BK : (1 << 30);
+    static constexpr int KB_PER_CHUNK = S >= 2 ? 512 / BK : (1 << 30);
 };
 
 struct TcMaps {
@@ -184,7 +176,7 @@ __device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t stage_base
     for (int kk = 0; kk < (S == 1 ? 4 : 2); ++kk) {
         // K = 8 per tf32 MMA: 32 bytes along the swizzled row
         const uint32_t ko = kk * 32;
-        if (S == 2 || S == 5) {
+        if (S == 2) {
             mma_tf32_ss(d_tmem, d(a + 64 + ko), d(b + ko), kIdescTf32, acc);
             acc = 1u;
             mma_tf32_ss(d_tmem, d(a + ko), d(b + 64 + ko), kIdescTf32, 1u);
@@ -410,7 +402,7 @@ struct PairCfg {
     static constexpr int B_BYTES = 128 * 128;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;  // 32 KB
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*bars*/;
-    static constexpr int KB_PER_CHUNK = S >= 2 ? kChunkK<S> / BK : (1 << 30);
+    static constexpr int KB_PER_CHUNK = S >= 2 ? 512 / BK : (1 << 30);
 };
 
 constexpr uint32_t kIdescShapePair =
@@ -450,7 +442,7 @@ __device__ __forceinline__ void issue_stage_pair(uint32_t d_tmem, uint32_t stage
 #pragma unroll
     for (int kk = 0; kk < (S == 1 ? 4 : 2); ++kk) {
         const uint32_t ko = kk * 32;
-        if (S == 2 || S == 5) {
+        if (S == 2) {
             mma_tf32_ss_pair(d_tmem, d(a + 64 + ko), d(b + ko), idesc_tf32, acc);
             acc = 1u;
             mma_tf32_ss_pair(d_tmem, d(a + ko), d(b + 64 + ko), idesc_tf32, 1u);
@@ -1223,7 +1215,7 @@ int gemm_prep_b_signal(int mode, int K, int N, const float* B, int64_t ldb,
 }
 
 int gemm_run(const GemmOperands& op, int M, int N, int K, float alpha, float* C, int64_t ldc,
-             const float* bias, int relu, cudaStream_t s, const GemmGate* gate, bool fine) {
+             const float* bias, int relu, cudaStream_t s, const GemmGate* gate) {
     if (gate && gate->flags && op.mode == ZG_GEMM_SIMT_FP32)
         return set_error(ZG_ERR_DISPATCH, "sgemm: the arrival gate needs a tensor-core mode");
     switch (op.mode) {
@@ -1232,9 +1224,7 @@ int gemm_run(const GemmOperands& op, int M, int N, int K, float alpha, float* C,
                                      static_cast<const float*>(op.b.p), op.b.ld, C, ldc, bias,
                                      relu, s);
         case ZG_GEMM_TF32: return run_tc<1>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);
-        case ZG_GEMM_TF32X3:
-            if (fine) return run_tc<5>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);
-            return run_tc<2>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);
+        case ZG_GEMM_TF32X3: return run_tc<2>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);
         case ZG_GEMM_TF32_BF16X2:
             return run_tc<3>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);
         case ZG_GEMM_BF16X3: return run_tc<4>(op, M, N, K, alpha, C, ldc, bias, relu, s, gate);

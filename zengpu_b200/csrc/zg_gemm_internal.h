@@ -80,9 +80,7 @@ struct GemmGate {
 
 // C[M x N, pitch ldc] = epilogue(alpha * A @ B) on prepared operands; `gate`
 // (tensor-core modes only) holds back B loads until their chunk has arrived.
-// `fine`: TF32X3 drains its accumulators every 64 of k instead of every 512.
 int gemm_run(const GemmOperands& op, int M, int N, int K, float alpha, float* C, int64_t ldc,
-             const float* bias, int relu, cudaStream_t s, const GemmGate* gate = nullptr,
-             bool fine = false);
+             const float* bias, int relu, cudaStream_t s, const GemmGate* gate = nullptr);
 
 }  // namespace zg

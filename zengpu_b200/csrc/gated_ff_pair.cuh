@@ -112,7 +112,7 @@ inline int sm_pairs() {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Into how many parts products of few 256 x 256 tiles split their sums, stages of
-// `step`: as many as the SM pairs take, four at most, eight stages each at least.
+// `step`: as many as the SM pairs take, sixteen at most, four stages each at least.
 inline int splits_of(const FfProduct* products, int count, int step) {
     int64_t tiles = 0;
     int nkb = 1 << 30;
@@ -122,7 +122,7 @@ inline int splits_of(const FfProduct* products, int count, int step) {
         nkb = std::min(nkb, (f.k[0] + step - 1) / step + (f.k[1] + step - 1) / step);
     }
     return static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>({4, kPairsSold / std::max<int64_t>(tiles, 1), nkb / 8})));
+        std::max<int64_t>(1, std::min<int64_t>({16, kPairsSold / std::max<int64_t>(tiles, 1), nkb / 4})));
 }
 inline uint64_t split_bytes(const FfProduct* products, int count, int splits) {
     if (splits == 1) return 0;

@@ -4,7 +4,7 @@
 //
 // The weights take the MMA's M side: D^T[128 columns of W x rows of x] = W^T x^T, so
 // a tile wastes nothing on missing rows: the MMA's N is the rows rounded up to
-// 16, 32, 64 or 128.  W is read as it lies (mn-major, see gated_ff_tc.cu), x or h as
+// 16, 32 or 64.  W is read as it lies (mn-major, see gated_ff_tc.cu), x or h as
 // the k-major B operand.  The gated product holds two accumulators, of Wg and Wu.
 //
 // A CTA takes 128 columns and a part of the sum; the CTAs of a cluster share the
@@ -63,7 +63,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t mine, uint32_t rank)
 }
 
 __host__ __device__ constexpr uint32_t tmem_columns(int n) {
-    return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256;
+    return n <= 32 ? 32 : n <= 64 ? 64 : 128;
 }
 
 // GATED: c = act(x Wg) * (x Wu), and the two products to pre_g, pre_u unless null.
@@ -313,8 +313,7 @@ template <bool GATED, int ACT, class T>
 int launch_rows_n(RowsArgs& a, cudaStream_t s) {
     if (a.M <= 16) return launch_rows<GATED, ACT, T, 16>(a, s);
     if (a.M <= 32) return launch_rows<GATED, ACT, T, 32>(a, s);
-    if (a.M <= 64) return launch_rows<GATED, ACT, T, 64>(a, s);
-    return launch_rows<GATED, ACT, T, 128>(a, s);
+    return launch_rows<GATED, ACT, T, 64>(a, s);
 }
 
 template <class T>
@@ -335,7 +334,7 @@ int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& f, cudaStream_
     std::memset(&args, 0, sizeof(args));
     args.c = f.c, args.ldc = f.ldc, args.pre_g = f.pre_g, args.pre_u = f.pre_u;
     args.M = f.M, args.N = f.N, args.nkb = (f.k[0] + kSumStep - 1) / kSumStep;
-    const int rows = f.M <= 16 ? 16 : f.M <= 32 ? 32 : f.M <= 64 ? 64 : 128;
+    const int rows = f.M <= 16 ? 16 : f.M <= 32 ? 32 : 64;
     int rc = status_word(&args.status);
     for (int w = 0; w < (gated ? 2 : 1) && !rc; ++w)
         rc = encode_16bit_map(&args.w[w], dtype, f.b[w].p, f.N, f.k[0], f.b[w].ld, 64, kSumStep);

@@ -6,11 +6,11 @@
 //
 // A CTA takes 128 columns of W (of Wg and of Wu for the gated product) and a part of
 // the sum; the CTAs of a cluster share the columns and split the sum.  Weights and
-// the transposed piece of x come through a ring of stages of 16 of the sum
-// (cp.async, 16 bytes where the pitch allows it, else 4).  A lane holds four columns;
-// the eight warps are dealt out to groups of eight rows and, where there are fewer,
-// to parts of the stage: 8 rows x 4 columns x 2 products a thread, 64 FMAs for four
-// 16-byte reads of shared memory.  Partial results meet in shared memory, across the
+// the piece of x come through a ring of stages of 32 of the sum (cp.async, 16 bytes
+// where the pitch allows it, else 4).  A lane holds four columns; the eight warps are
+// dealt out to groups of eight rows (of 1, 2 or 4, up to that many) and, where those are
+// fewer, to parts of the stage: 8 rows x 4 columns x 2 products a thread, 64 FMAs for four 16-byte reads of shared
+// memory (two of them the eight rows' x, four of the sum at a time).  Partial results meet in shared memory, across the
 // cluster as in gated_ff_rows.cu, in a fixed order.
 //
 // Up to 16 rows the weights' 4 bytes each bound it; beyond, the f32 pipe (8 rows a
@@ -25,7 +25,10 @@
 namespace zg {
 namespace {
 
-constexpr int kRThreads = 256, kRWarps = 8, kRCols = 128, kRStep = 16, kRStages = 5;
+constexpr int kRThreads = 256, kRWarps = 8, kRCols = 128, kRStep = 32;
+constexpr int kXPitch = kRStep + 4;  // floats of a row of x in a stage
+// About 100 KB of weights in flight, two CTAs to an SM.
+__host__ __device__ constexpr int ring_stages(int mats) { return mats == 2 ? 3 : 5; }
 
 struct RowsF32Args {
     const float* x;
@@ -35,7 +38,7 @@ struct RowsF32Args {
     float* pre_u;
     int64_t ldx, ldw, ldc;
     int M, N, K;
-    int vec;  // w: 16-byte aligned rows
+    int vec_w, vec_x;  // 16-byte aligned rows
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const float* from, bool in) {
@@ -59,14 +62,15 @@ __device__ __forceinline__ float4 ld_rank(uint32_t mine, uint32_t rank) {
     return v;
 }
 
-// ROWS: 8, 16, 32 or 64.
+// ROWS: 1, 2, 4, 8, 16 or 32.
 template <bool GATED, int ACT, int ROWS>
-__global__ void __launch_bounds__(kRThreads)
-    ff_rows_f32_kernel(const RowsF32Args a) {
+__global__ void __launch_bounds__(kRThreads, 2)
+    ff_rows_f32_kernel(const __grid_constant__ RowsF32Args a) {
     constexpr int kMats = GATED ? 2 : 1;
-    constexpr int kRowGroups = ROWS / 8, kSumGroups = kRWarps / kRowGroups;
-    constexpr int kWFloats = kMats * kRStep * kRCols, kXFloats = kRStep * ROWS;
-    constexpr int kStageFloats = kWFloats + kXFloats;
+    constexpr int kOwn = ROWS < 8 ? ROWS : 8;  // rows of a warp
+    constexpr int kRowGroups = ROWS / kOwn, kSumGroups = kRWarps / kRowGroups;
+    constexpr int kStages = ring_stages(kMats);
+    constexpr int kWFloats = kMats * kRStep * kRCols, kStageFloats = kWFloats + ROWS * kXPitch;
     extern __shared__ float4 ring4[];
     float* ring = reinterpret_cast<float*>(ring4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -75,68 +79,87 @@ __global__ void __launch_bounds__(kRThreads)
     const int steps = (a.K + kRStep - 1) / kRStep;
     const int s0 = static_cast<int>(static_cast<int64_t>(steps) * rank / split);
     const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / split);
-    const int row0 = warp % kRowGroups * 8, part = warp / kRowGroups;
+    const int row0 = warp % kRowGroups * kOwn, part = warp / kRowGroups;
 
     auto load = [&](int step) {
         if (step < s1) {
-            const uint32_t st = smem_u32(ring + (step - s0) % kRStages * kStageFloats);
+            const uint32_t st = smem_u32(ring + (step - s0) % kStages * kStageFloats);
             const int k0 = step * kRStep;
-            if (a.vec) {
 #pragma unroll
-                for (int j = threadIdx.x; j < kWFloats / 4; j += kRThreads) {
-                    const int w = j / (kRStep * kRCols / 4), k = j / (kRCols / 4) % kRStep;
-                    const int c = j % (kRCols / 4) * 4;
-                    const bool in = k0 + k < a.K && n0 + c < a.N;
-                    copy16(st + j * 16, in ? a.w[w] + (k0 + k) * a.ldw + n0 + c : a.w[0], in);
-                }
-            } else {
-                for (int j = threadIdx.x; j < kWFloats; j += kRThreads) {
-                    const int w = j / (kRStep * kRCols), k = j / kRCols % kRStep;
-                    const int c = j % kRCols;
-                    const bool in = k0 + k < a.K && n0 + c < a.N;
-                    copy4(st + j * 4, in ? a.w[w] + (k0 + k) * a.ldw + n0 + c : a.w[0], in);
+            for (int w = 0; w < kMats; ++w) {
+                const float* from = w ? a.w[1] : a.w[0];
+                const uint32_t to = st + w * kRStep * kRCols * 4;
+                if (a.vec_w) {
+#pragma unroll
+                    for (int i = 0; i < kRStep * kRCols / 4 / kRThreads; ++i) {
+                        const int k = i * (kRThreads * 4 / kRCols) + threadIdx.x / (kRCols / 4);
+                        const int c = threadIdx.x % (kRCols / 4) * 4;
+                        const bool in = k0 + k < a.K && n0 + c < a.N;
+                        copy16(to + (k * kRCols + c) * 4,
+                               in ? from + (k0 + k) * a.ldw + n0 + c : from, in);
+                    }
+                } else {
+#pragma unroll 4
+                    for (int i = 0; i < kRStep * kRCols / kRThreads; ++i) {
+                        const int k = i * (kRThreads / kRCols) + threadIdx.x / kRCols;
+                        const int c = threadIdx.x % kRCols;
+                        const bool in = k0 + k < a.K && n0 + c < a.N;
+                        copy4(to + (k * kRCols + c) * 4,
+                              in ? from + (k0 + k) * a.ldw + n0 + c : from, in);
+                    }
                 }
             }
-            for (int j = threadIdx.x; j < kXFloats; j += kRThreads) {
-                const int k = j % kRStep, r = j / kRStep;
-                const bool in = k0 + k < a.K && r < a.M;
-                copy4(st + (kWFloats + k * ROWS + r) * 4, in ? a.x + r * a.ldx + k0 + k : a.x, in);
+            const uint32_t to = st + kWFloats * 4;
+            if (a.vec_x) {
+                for (int j = threadIdx.x; j < ROWS * (kRStep / 4); j += kRThreads) {
+                    const int r = j / (kRStep / 4), k = j % (kRStep / 4) * 4;
+                    const bool in = k0 + k < a.K && r < a.M;
+                    copy16(to + (r * kXPitch + k) * 4, in ? a.x + r * a.ldx + k0 + k : a.x, in);
+                }
+            } else {
+                for (int j = threadIdx.x; j < ROWS * kRStep; j += kRThreads) {
+                    const int r = j / kRStep, k = j % kRStep;
+                    const bool in = k0 + k < a.K && r < a.M;
+                    copy4(to + (r * kXPitch + k) * 4, in ? a.x + r * a.ldx + k0 + k : a.x, in);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
-    float acc[kMats][8][4] = {};
+    float acc[kMats][kOwn][4] = {};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = 0; i < kRStages - 1; ++i) load(s0 + i);
+    for (int i = 0; i < kStages - 1; ++i) load(s0 + i);
     for (int step = s0; step < s1; ++step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kRStages - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncthreads();  // the stage has landed, and the one before it is free
-        load(step + kRStages - 1);
-        const float* st = ring + (step - s0) % kRStages * kStageFloats;
-#pragma unroll 4
-        for (int i = 0; i < kRStep / kSumGroups; ++i) {
-            const int k = part + i * kSumGroups;
-            float x[8];
+        load(step + kStages - 1);
+        const float* st = ring + (step - s0) % kStages * kStageFloats;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+        for (int i = 0; i < kRStep / 4 / kSumGroups; ++i) {
+            const int k = (part + i * kSumGroups) * 4;
+            float x[kOwn][4];
+#pragma unroll
+            for (int r = 0; r < kOwn; ++r) {
                 const float4 v =
-                    *reinterpret_cast<const float4*>(st + kWFloats + k * ROWS + row0 + 4 * h);
-                x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+                    *reinterpret_cast<const float4*>(st + kWFloats + (row0 + r) * kXPitch + k);
+                x[r][0] = v.x, x[r][1] = v.y, x[r][2] = v.z, x[r][3] = v.w;
             }
 #pragma unroll
-            for (int w = 0; w < kMats; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(st + (w * kRStep + k) * kRCols +
-                                                                  lane * 4);
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    acc[w][r][0] = fmaf(x[r], v.x, acc[w][r][0]);
-                    acc[w][r][1] = fmaf(x[r], v.y, acc[w][r][1]);
-                    acc[w][r][2] = fmaf(x[r], v.z, acc[w][r][2]);
-                    acc[w][r][3] = fmaf(x[r], v.w, acc[w][r][3]);
+                for (int w = 0; w < kMats; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(
+                        st + (w * kRStep + k + e) * kRCols + lane * 4);
+#pragma unroll
+                    for (int r = 0; r < kOwn; ++r) {
+                        acc[w][r][0] = fmaf(x[r][e], v.x, acc[w][r][0]);
+                        acc[w][r][1] = fmaf(x[r][e], v.y, acc[w][r][1]);
+                        acc[w][r][2] = fmaf(x[r][e], v.z, acc[w][r][2]);
+                        acc[w][r][3] = fmaf(x[r][e], v.w, acc[w][r][3]);
+                    }
                 }
-            }
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -145,7 +168,7 @@ __global__ void __launch_bounds__(kRThreads)
 #pragma unroll
     for (int w = 0; w < kMats; ++w)
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < kOwn; ++r)
             *reinterpret_cast<float4*>(ring + ((part * kMats + w) * ROWS + row0 + r) * kRCols +
                                        lane * 4) =
                 make_float4(acc[w][r][0], acc[w][r][1], acc[w][r][2], acc[w][r][3]);
@@ -183,12 +206,12 @@ __global__ void __launch_bounds__(kRThreads)
 template <bool GATED, int ACT, int ROWS>
 int launch_rows(const RowsF32Args& a, cudaStream_t s) {
     constexpr int kMats = GATED ? 2 : 1;
-    constexpr int kSmem = std::max(kRStages * (kMats * kRStep * kRCols + kRStep * ROWS),
-                                   kMats * 8 * kRWarps * kRCols) * 4;
+    constexpr int kSmem = std::max(ring_stages(kMats) * (kMats * kRStep * kRCols + ROWS * kXPitch),
+                                   kMats * std::min(ROWS, 8) * kRWarps * kRCols) * 4;
     const int tiles = (a.N + kRCols - 1) / kRCols, steps = (a.K + kRStep - 1) / kRStep;
     int split = 1;
     // two CTAs of an SM, a few stages for each part of the sum at least
-    while (split < 8 && 2 * split * tiles <= 2 * 148 && 8 * split <= steps) split *= 2;
+    while (split < 8 && 2 * split * tiles <= 2 * 148 && 6 * split <= steps) split *= 2;
     auto kernel = ff_rows_f32_kernel<GATED, ACT, ROWS>;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
@@ -216,10 +239,12 @@ int launch_rows(const RowsF32Args& a, cudaStream_t s) {
 
 template <bool GATED, int ACT>
 int launch_rows_n(const RowsF32Args& a, cudaStream_t s) {
+    if (a.M <= 1) return launch_rows<GATED, ACT, 1>(a, s);
+    if (a.M <= 2) return launch_rows<GATED, ACT, 2>(a, s);
+    if (a.M <= 4) return launch_rows<GATED, ACT, 4>(a, s);
     if (a.M <= 8) return launch_rows<GATED, ACT, 8>(a, s);
     if (a.M <= 16) return launch_rows<GATED, ACT, 16>(a, s);
-    if (a.M <= 32) return launch_rows<GATED, ACT, 32>(a, s);
-    return launch_rows<GATED, ACT, 64>(a, s);
+    return launch_rows<GATED, ACT, 32>(a, s);
 }
 
 }  // namespace
@@ -232,7 +257,8 @@ int ff_rows_f32(bool gated, int act, const FfProduct& f, cudaStream_t s) {
     a.c = static_cast<float*>(f.c), a.ldc = f.ldc;
     a.pre_g = f.pre_g, a.pre_u = f.pre_u;
     a.M = f.M, a.N = f.N, a.K = f.k[0];
-    a.vec = a.ldw % 4 == 0 &&
+    a.vec_x = a.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+    a.vec_w = a.ldw % 4 == 0 &&
             ((reinterpret_cast<uintptr_t>(a.w[0]) | reinterpret_cast<uintptr_t>(a.w[1])) & 15) == 0;
     if (!gated) return launch_rows_n<false, ZG_ACT_RELU>(a, s);
     switch (act) {

@@ -443,13 +443,15 @@ int zg_fill_normal_f32(float *x, uint64_t n, uint64_t seed, void *stream);
  * or F16, 16-byte aligned.  Sums are f32.  BF16 and F16 run on the tensor cores
  * as they are (mode is not read); h = act(x w_gate) * (x w_up), and in the
  * backward pass the gradients of the two products, are rounded once to the
- * dtype, as operands of the next product.  F32 runs in `mode` (ZG_GEMM_*), with
- * f32 throughout.
+ * dtype, as operands of the next product.  F32 runs in `mode` (ZG_GEMM_*): TF32X3
+ * with sums that end within 1e-6 of float64 (relative Frobenius norm, two chained
+ * products), the other tensor-core modes at sgemm's accuracy for each product,
+ * SIMT_FP32 in plain f32; a forward pass of up to 32 rows is plain f32 in every mode.
  *     pre_gate, pre_up: f32 [m, f], written by the forward pass when both are
  * given (x w_gate and x w_up before the activation), read by the backward pass.
  *     workspace: zg_gated_ff_workspace_bytes(...), 256-byte aligned, not shared by
  * calls that may overlap.  m = 0 computes nothing (the weights' gradients are
- * zero); k, f, d are at least 1.  Outputs must not overlap inputs. */
+ * zero); k, f, d are at least 1; no size exceeds 2^28.  Outputs must not overlap inputs. */
 #define ZG_ACT_SILU 0      /* g / (1 + e^-g) */
 #define ZG_ACT_GELU 1      /* g Phi(g) */
 #define ZG_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
@@ -484,7 +486,7 @@ int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f,
  * not finite gets a NaN scale.
  *     step_dev, lr_dev: device scalars that replace h->step and h->lr (NULL:
  * the host's), read by the kernel, so that a captured step can be replayed with
- * new ones.  grad_scale_dev: device scalar s (NULL: 1); when it is not finite
+ * new ones; a *step_dev below 1 changes nothing.  grad_scale_dev: device scalar s (NULL: 1); when it is not finite
  * the call changes nothing.  The tensors of a call must not overlap. */
 #define ZG_ADAMW_BLOCK 256
 typedef struct zg_adamw_tensor {

@@ -263,6 +263,13 @@ def test_adamw_captured(bits):
     c.check()
 
 
+def test_adamw_device_step_below_one_changes_nothing():
+    c = Case([300])
+    for step in (0, -3):
+        c.opt.step(torch.full((1,), step, dtype=torch.int64, device="cuda"), **HYPER)
+    c.check()
+
+
 def test_adamw_refusals():
     p, g = torch.zeros(8, device="cuda"), torch.zeros(8, device="cuda")
     opt = K.AdamW([p], [g])

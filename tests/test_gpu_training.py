@@ -4,6 +4,9 @@ DeviceArrays, eager and as one captured graph."""
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -17,6 +20,7 @@ from zengpu_b200 import Activation, kernels as K
 
 pytestmark = pytest.mark.gpu
 
+ROOT = Path(__file__).resolve().parents[1]
 NAMES = ("dw_gate", "dw_up", "dw_down")
 
 
@@ -215,3 +219,36 @@ def test_device_array_refusals(device, pool):
         level1.grad_norm(device, pool, [alloc(4, dtype=zg.DType.I32)], 1.0)
     with pytest.raises(ValueError):
         level1.adamw(device, [p], [g, g], [m], [v], 1)
+
+
+FIRST = """
+import torch
+from zengpu_b200 import kernels as K
+x, wg, wu, wd, dy = (torch.randn(s, device="cuda").to({kind}) * 0.1
+                     for s in ((m, 64), (64, 136), (64, 136), (136, 64), (m, 64)))
+grads = [torch.empty_like(w) for w in (wg, wu, wd)]
+opt, norm = K.AdamW([w.clone() for w in (wg, wu, wd)], grads, state_bits=8), K.GradNorm(grads)
+torch.cuda.synchronize()
+def run():
+    y, saved = K.gated_ff(x, wg, wu, wd, save=True)
+    K.gated_ff_backward(dy, x, wg, wu, wd, saved, out=(None, *grads))
+    opt.step(1, grad_scale=norm.clip_scale(1.0)[1:])
+    return y
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = run()
+y.zero_()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, K.gated_ff(x, wg, wu, wd)) and K.kernel_status() == 0
+"""
+
+
+@pytest.mark.parametrize("kind,m", [("torch.bfloat16", 5), ("torch.float16", 300),
+                                    ("torch.float32", 5), ("torch.float32", 300)])
+def test_first_call_of_a_process_may_be_captured(kind, m):
+    """Kernels load and attributes are set at the first call; a capture takes that too."""
+    code = FIRST.replace("{kind}", kind).replace("(m, 64)", f"({m}, 64)")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import types
 
 import pytest
 
@@ -29,7 +30,7 @@ def ff_backward(ptrs=None, ws=FAKE, nbytes=1 << 20, **kw):
 
 def test_gated_ff_refusals():
     for bad in (dict(dtype=I32), dict(act=4), dict(act=-1), dict(dtype=F32, mode=5), dict(m=-1),
-                dict(k=0), dict(f=-3), dict(d=0), dict(ws=None), dict(nbytes=16), dict(ws=FAKE + 8),
+                dict(k=0), dict(f=-3), dict(d=0), dict(f=(1 << 28) + 1), dict(ws=None), dict(nbytes=16), dict(ws=FAKE + 8),
                 dict(pre=(FAKE, None)), dict(ptrs=[FAKE + 2] + [FAKE] * 4)):
         assert ff(**bad) == DISPATCH, bad
         assert L.last_error(), bad
@@ -98,6 +99,9 @@ def test_python_refuses_cpu_tensors():
     x = torch.zeros(2, 4)
     with pytest.raises(ValueError):
         K.gated_ff(x, torch.zeros(4, 6), torch.zeros(4, 6), torch.zeros(6, 4))
+    with pytest.raises(ValueError, match="exceed"):
+        K._ff_sizes(types.SimpleNamespace(is_cuda=True, dtype=torch.bfloat16, shape=(1 << 33, 4),
+                                          dim=lambda: 2), torch.zeros(4, 6), torch.zeros(6, 4))
     with pytest.raises(ValueError):
         K.AdamW([x], [x.clone()])
     with pytest.raises(ValueError):

@@ -14,11 +14,12 @@ namespace zg {
 namespace {
 
 // ---- CUDA-core product ------------------------------------------------------------
-// 64 x 64 of D per CTA, 4 x 4 per thread (twice for the gated pair), operands
-// through shared memory 16 of the sum at a time.  f32 throughout.
+// The SIMT_FP32 mode: 64 x 64 of D per CTA, 4 x 4 per thread (twice for the gated
+// pair), operands of any layout through shared memory 16 of the sum at a time.  f32
+// throughout; bound by the f32 pipe, of which it reaches a quarter (18 TFLOP/s on a
+// 2048 x 1024 x 4096 training pass): the mode is the accuracy anchor, not a fast path.
 constexpr int kTile = 64, kStep = 16;
 
-template <class T>
 __device__ __forceinline__ void load_panel(float (&sh)[kStep][kTile + 4], const FfOperand& o,
                                            int rows, int r0, int k, int i0) {
     // the thread order follows the operand's contiguous direction
@@ -26,23 +27,23 @@ __device__ __forceinline__ void load_panel(float (&sh)[kStep][kTile + 4], const 
         const int r = o.mn ? e % kTile : e / kStep, i = o.mn ? e / kTile : e % kStep;
         float v = 0.0f;
         if (r0 + r < rows && i0 + i < k)
-            v = FfElem<T>::get(static_cast<const T*>(
-                o.p)[o.mn ? (i0 + i) * o.ld + r0 + r : (r0 + r) * o.ld + i0 + i]);
+            v = static_cast<const float*>(
+                o.p)[o.mn ? (i0 + i) * o.ld + r0 + r : (r0 + r) * o.ld + i0 + i];
         sh[i][r] = v;
     }
 }
 
-template <class T, int EPI, int ACT>
+template <int EPI, int ACT>
 __global__ void __launch_bounds__(256) ff_simt_kernel(const FfProduct p) {
     __shared__ float sa[kStep][kTile + 4], sb[2][kStep][kTile + 4];
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
+    const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     float acc[2][4][4] = {};
     for (int seg = 0; seg < (EPI == kFfStore ? 2 : 1); ++seg) {
         for (int i0 = 0; i0 < p.k[seg]; i0 += kStep) {
-            load_panel<T>(sa, p.a[seg], p.M, m0, p.k[seg], i0);
-            load_panel<T>(sb[0], p.b[seg], p.N, n0, p.k[seg], i0);
-            if (EPI == kFfGated) load_panel<T>(sb[1], p.b[1], p.N, n0, p.k[0], i0);
+            load_panel(sa, p.a[seg], p.M, m0, p.k[seg], i0);
+            load_panel(sb[0], p.b[seg], p.N, n0, p.k[seg], i0);
+            if (EPI == kFfGated) load_panel(sb[1], p.b[1], p.N, n0, p.k[0], i0);
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
@@ -72,10 +73,10 @@ __global__ void __launch_bounds__(256) ff_simt_kernel(const FfProduct p) {
             if (col >= p.N) break;
             const int64_t at = row * p.ldc + col, pre = row * p.N + col;
             const float x = acc[0][r][c];
-            if (EPI == kFfStore) static_cast<T*>(p.c)[at] = FfElem<T>::put(x);
+            if (EPI == kFfStore) static_cast<float*>(p.c)[at] = x;
             if (EPI == kFfGated) {
                 const float u = acc[1][r][c];
-                static_cast<T*>(p.c)[at] = FfElem<T>::put(activate<ACT, sizeof(T) == 2>(x).a * u);
+                static_cast<float*>(p.c)[at] = activate<ACT, false>(x).a * u;
                 if (p.pre_g) {
                     p.pre_g[pre] = x;
                     p.pre_u[pre] = u;
@@ -83,45 +84,35 @@ __global__ void __launch_bounds__(256) ff_simt_kernel(const FfProduct p) {
             }
             if (EPI == kFfSlope) {
                 const float u = p.pre_u[pre];
-                const ActValue v = activate<ACT, sizeof(T) == 2>(p.pre_g[pre]);
-                static_cast<T*>(p.c)[at] = FfElem<T>::put(x * u * v.slope);
-                static_cast<T*>(p.c2)[at] = FfElem<T>::put(x * v.a);
-                static_cast<T*>(p.c3)[at] = FfElem<T>::put(v.a * u);
+                const ActValue v = activate<ACT, false>(p.pre_g[pre]);
+                static_cast<float*>(p.c)[at] = x * u * v.slope;
+                static_cast<float*>(p.c2)[at] = x * v.a;
+                static_cast<float*>(p.c3)[at] = v.a * u;
             }
         }
     }
 }
 
-template <class T, int EPI>
+template <int EPI>
 int launch_simt(int act, const FfProduct& p, cudaStream_t s) {
-    const dim3 grid((p.N + kTile - 1) / kTile, (p.M + kTile - 1) / kTile);
-    if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many rows");
+    const dim3 grid((p.M + kTile - 1) / kTile, (p.N + kTile - 1) / kTile);
+    if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many columns");
     switch (EPI == kFfStore ? ZG_ACT_RELU : act) {
-        case ZG_ACT_SILU: ff_simt_kernel<T, EPI, ZG_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
-        case ZG_ACT_GELU: ff_simt_kernel<T, EPI, ZG_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
-        case ZG_ACT_GELU_TANH: ff_simt_kernel<T, EPI, ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
-        default: ff_simt_kernel<T, EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
+        case ZG_ACT_SILU: ff_simt_kernel<EPI, ZG_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
+        case ZG_ACT_GELU: ff_simt_kernel<EPI, ZG_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
+        case ZG_ACT_GELU_TANH: ff_simt_kernel<EPI, ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
+        default: ff_simt_kernel<EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
     }
     return cuda_status(cudaGetLastError(), "gated_ff");
 }
 
-template <class T>
-int launch_simt_epi(FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s) {
-    switch (epi) {
-        case kFfStore: return launch_simt<T, kFfStore>(act, p, s);
-        case kFfGated: return launch_simt<T, kFfGated>(act, p, s);
-        default: return launch_simt<T, kFfSlope>(act, p, s);
-    }
-}
-
 }  // namespace
 
-int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s) {
-    if (p.M == 0 || p.N == 0) return ZG_OK;
-    switch (dtype) {
-        case ZG_DTYPE_F32: return launch_simt_epi<float>(epi, act, p, s);
-        case ZG_DTYPE_BF16: return launch_simt_epi<__nv_bfloat16>(epi, act, p, s);
-        default: return launch_simt_epi<__half>(epi, act, p, s);
+int ff_simt(FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s) {
+    switch (epi) {
+        case kFfStore: return launch_simt<kFfStore>(act, p, s);
+        case kFfGated: return launch_simt<kFfGated>(act, p, s);
+        default: return launch_simt<kFfSlope>(act, p, s);
     }
 }
 
@@ -162,11 +153,21 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ P
         const int64_t row = at / t.ld;
         const int col = static_cast<int>(at - row * t.ld);
         const uint16_t* src = t.src + row * t.cols + col;
-        uint16_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = col + e < t.cols ? src[e] : 0;
         uint4 q;
-        __builtin_memcpy(&q, v, 16);
+        if (col + 8 > t.cols) {
+            uint16_t v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = col + e < t.cols ? src[e] : 0;
+            __builtin_memcpy(&q, v, 16);
+        } else if ((reinterpret_cast<uintptr_t>(src) & 2) == 0) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {  // three words inside, an element on either side
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(src + 1);
+            const uint32_t a = src[0], b = w[0], c = w[1], d = w[2], e = src[7];
+            q = make_uint4(a | (b << 16), (b >> 16) | (c << 16), (c >> 16) | (d << 16),
+                           (d >> 16) | (e << 16));
+        }
         *reinterpret_cast<uint4*>(t.dst + at) = q;
     }
 }
@@ -248,6 +249,11 @@ int place_inputs(const FfCall& c, const FfLayout& l, uint8_t* ws, const void* co
 // dx's two products are one GEMM over [dg | du] and [Wg | Wu], each padded to whole
 // k blocks with zeros.
 
+// The forward pass of few rows (gated_ff_rows.cu, gated_ff_rows_f32.cu), whose grids
+// take 65535 tiles of 128 columns.
+bool few_rows(const FfCall& c) {
+    return c.m <= (c.size == 2 ? kFfRows : kFfRowsF32) && std::max(c.f, c.d) <= 65535 * 128;
+}
 bool f32_tensor(const FfCall& c) { return c.size == 4 && c.mode != ZG_GEMM_SIMT_FP32; }
 
 struct Planes {
@@ -460,14 +466,16 @@ int check_call(FfCall& c, const char* what) {
         return set_error(ZG_ERR_DISPATCH, "%s: unknown activation %d", what, c.act);
     if (c.dtype == ZG_DTYPE_F32 && (c.mode < ZG_GEMM_SIMT_FP32 || c.mode > ZG_GEMM_BF16X3))
         return set_error(ZG_ERR_DISPATCH, "%s: unknown mode %d", what, c.mode);
-    if (c.m < 0 || c.k < 1 || c.f < 1 || c.d < 1)
+    constexpr int kMost = 1 << 28;  // tiles, planes and box coordinates stay within 32 bits
+    if (c.m < 0 || c.k < 1 || c.f < 1 || c.d < 1 || c.m > kMost || c.k > kMost || c.f > kMost ||
+        c.d > kMost)
         return set_error(ZG_ERR_DISPATCH, "%s: bad shape: %d rows, sizes %d, %d, %d", what, c.m,
                          c.k, c.f, c.d);
     return ZG_OK;
 }
 
 uint64_t ff_workspace(const FfCall& c) {
-    if (!f32_tensor(c) || (!c.backward && c.m <= kFfRowsF32)) return ff_layout(c).total;
+    if (!f32_tensor(c) || (!c.backward && few_rows(c))) return ff_layout(c).total;
     int rc;
     return c.backward ? f32_backward(c, {}, nullptr, nullptr, &rc)
                       : f32_forward(c, {}, nullptr, nullptr, &rc);
@@ -499,7 +507,7 @@ int products(const FfCall& c, FfEpilogue epi, const FfProduct* p, int count, voi
              cudaStream_t s) {
     if (c.size == 2) return ff_pair(c.dtype, epi, c.act, p, count, static_cast<float*>(parts), s);
     int rc = ZG_OK;
-    for (int i = 0; i < count && !rc; ++i) rc = ff_simt(c.dtype, epi, c.act, p[i], s);
+    for (int i = 0; i < count && !rc; ++i) rc = ff_simt(epi, c.act, p[i], s);
     return rc;
 }
 
@@ -529,7 +537,7 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
                          "gated_ff: pre_gate and pre_up are both null or both 16-byte aligned");
     if ((rc = check_workspace(c, workspace, workspace_bytes, "gated_ff"))) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (f32_tensor(c) && m > kFfRowsF32) {
+    if (f32_tensor(c) && !few_rows(c)) {
         F32Tensors t{};
         t.x = static_cast<const float*>(x), t.wg = static_cast<const float*>(w_gate);
         t.wu = static_cast<const float*>(w_up), t.wd = static_cast<const float*>(w_down);
@@ -549,7 +557,7 @@ extern "C" int zg_gated_ff(uint32_t dtype, int mode, int act, int m, int k, int 
     p.c = workspace, p.ldc = l.ld_f;
     p.pre_g = pre_gate, p.pre_u = pre_up;
     void* parts = static_cast<uint8_t*>(workspace) + l.parts;
-    const bool few = m <= (c.size == 2 ? kFfRows : kFfRowsF32);
+    const bool few = few_rows(c);
     auto rows = [&](bool gated, const FfProduct& f) {
         return c.size == 2 ? ff_rows(dtype, gated, act, f, s) : ff_rows_f32(gated, act, f, s);
     };

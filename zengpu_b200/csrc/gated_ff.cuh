@@ -115,8 +115,8 @@ int launch_dependent(const char* what, void (*kernel)(Params...), unsigned grid,
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
-// Plain CUDA-core product for any layout, f32 sums (gated_ff.cu).
-int ff_simt(uint32_t dtype, FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
+// Plain CUDA-core product of f32 tensors of any layout (gated_ff.cu).
+int ff_simt(FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
 
 // 16-bit tensors on the tensor cores (gated_ff_tc.cu): `count` products of one
 // epilogue in one launch (at most three).  Operands: 16-byte aligned, pitch a

@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(kActThreads) ff_planes_kernel(const ActArgs a)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ float tile[SLOPE ? kActCols / 32 : 1][SLOPE ? 3 : 1][32][33];
     const int lane = threadIdx.x & 31, block = threadIdx.x / 64, half = threadIdx.x / 32 & 1;
-    const int col = blockIdx.x * kActCols + block * 32 + lane;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 32;
+    const int col = blockIdx.y * kActCols + block * 32 + lane;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 32;
     const int kpad = (a.N + 15) / 16 * 16;
     float g[16], u[16], d[16];
 #pragma unroll
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kActThreads) ff_planes_kernel(const ActArgs a)
     const int m = static_cast<int>(row0) + lane;
 #pragma unroll 4
     for (int r = 0; r < 16; ++r) {
-        const int c = half * 16 + r, f = blockIdx.x * kActCols + block * 32 + c;
+        const int c = half * 16 + r, f = blockIdx.y * kActCols + block * 32 + c;
         if (f >= a.N || m >= mpad) continue;
 #pragma unroll
         for (int t = 0; t < 3; ++t)
@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(kActThreads) ff_planes_kernel(const ActArgs a)
 
 template <int ACT, bool SLOPE>
 int launch_planes(const ActArgs& a, cudaStream_t s) {
-    const dim3 grid((a.N + kActCols - 1) / kActCols, (a.M + 31) / 32);
-    if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many rows");
+    const dim3 grid((a.M + 31) / 32, (a.N + kActCols - 1) / kActCols);
+    if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many columns");
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -30,8 +30,7 @@ template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
 
 // Stores a warp's 32 x 32 block of T, row `lane` in the words of v, at `dst` (its
 // row 0, column 0); `rows` and `cols` of it lie inside the matrix.  vec: 16-byte
-// pieces of rows; otherwise (odd pitch or base) one element a lane, neighbours
-// side by side.
+// pieces of rows; otherwise (odd pitch or base) neighbours side by side.
 template <class T>
 __device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int cols, bool vec,
                                             const uint32_t (&v)[8 * sizeof(T)], uint8_t* turn,
@@ -50,6 +49,25 @@ __device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int co
             if (r < rows && piece * kPer < cols)
                 *reinterpret_cast<uint4*>(dst + r * ld + piece * kPer) =
                     *reinterpret_cast<const uint4*>(turn + r * kTurnPitch + piece * 16);
+        }
+    } else if (sizeof(T) == 2) {
+        // two rows a turn, 16 lanes each, in aligned words of two elements: 2 l and
+        // 2 l + 1, or in a row that starts inside a word one further, and then
+        // elements 0 and 31 alone
+        const int l = lane & 15;
+        for (int r = lane >> 4; r < rows; r += 2) {
+            T* to = dst + r * ld;
+            const T* from = reinterpret_cast<const T*>(turn + r * kTurnPitch);
+            const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1, e = 2 * l + odd;
+            if (e + 1 < min(cols, 32)) {
+                T pair[2] = {from[e], from[e + 1]};
+                uint32_t word;
+                __builtin_memcpy(&word, pair, 4);
+                *reinterpret_cast<uint32_t*>(to + e) = word;
+            } else if (e < cols) {
+                to[e] = from[e];
+            }
+            if (odd && l == 0 && cols > 0) to[0] = from[0];
         }
     } else if (lane < cols) {
         for (int r = 0; r < rows; ++r)

@@ -29,6 +29,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <algorithm>
+#include <exception>
 #include <mutex>
 #include <string>
 #include <thread>
@@ -1698,7 +1699,7 @@ extern "C" int zg_level1_adamw(zg_device* dev, uint32_t count, const zg_device_a
                                const zg_device_array* exp_avg, const zg_device_array* exp_avg_sq,
                                const zg_device_array* exp_avg_scale,
                                const zg_device_array* exp_avg_sq_scale, const zg_adamw_hyper* h,
-                               const zg_device_array* norm_scale) {
+                               const zg_device_array* norm_scale) try {
     const char* op = "adamw";
     if (!dev || !h || (count && (!params || !grads || !exp_avg || !exp_avg_sq)))
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
@@ -1769,11 +1770,13 @@ extern "C" int zg_level1_adamw(zg_device* dev, uint32_t count, const zg_device_a
                        t.data(), h, nullptr, nullptr, scale, dev->stream)))
         return rc;
     return deferred ? ZG_OK : finish_sync(dev, false);
+} catch (const std::exception& e) {  // the host ran out of memory for the tables
+    return set_error(ZG_ERR_BACKEND, "adamw: %s", e.what());
 }
 
 extern "C" int zg_level1_grad_norm(zg_device* dev, zg_pool* pool, uint32_t count,
                                    const zg_device_array* grads, double max_norm,
-                                   zg_device_array* out) {
+                                   zg_device_array* out) try {
     const char* op = "grad_norm";
     if (!dev || !pool || !out || (count && !grads))
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
@@ -1806,6 +1809,8 @@ extern "C" int zg_level1_grad_norm(zg_device* dev, zg_pool* pool, uint32_t count
         return rc;
     }
     return pool->memory == ZG_MEMORY_GPU_ONLY ? ZG_OK : finish_sync(dev, false);
+} catch (const std::exception& e) {
+    return set_error(ZG_ERR_BACKEND, "grad_norm: %s", e.what());
 }
 
 // ======================================================================

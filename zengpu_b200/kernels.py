@@ -249,7 +249,7 @@ def _ff_operand(name: str, t: torch.Tensor, shape: tuple[int, ...],
     if t.dtype is not like.dtype or t.device != like.device or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {like.dtype} tensor on {like.device}")
     # the kernels' copies start on 16-byte boundaries; a view that does not is copied
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
 
 
 def _ff_output(name: str, t: torch.Tensor | None, shape: tuple[int, ...],
@@ -267,7 +267,10 @@ def _ff_sizes(x: torch.Tensor, w_gate: torch.Tensor, w_down: torch.Tensor) -> tu
         raise ValueError("gated_ff: expected f32, bf16 or f16 CUDA tensors")
     if x.dim() != 2 or w_gate.dim() != 2 or w_down.dim() != 2:
         raise ValueError("gated_ff: expected 2-D tensors")
-    return *x.shape, w_gate.shape[1], w_down.shape[1]
+    sizes = (*x.shape, w_gate.shape[1], w_down.shape[1])
+    if max(sizes) > 1 << 28:
+        raise ValueError(f"gated_ff: sizes {sizes} exceed 2^28")
+    return sizes
 
 
 @functools.lru_cache(maxsize=1024)
@@ -326,7 +329,7 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
         w_up = _ff_operand("w_up", w_up, (k, f), x)
         w_down = _ff_operand("w_down", w_down, (f, d), x)
         pre = [_ff_output("saved", t, (m, f), x, torch.float32) for t in saved]
-        pre = [t if t.data_ptr() % 16 == 0 else t.clone() for t in pre]
+        pre = [t if t.data_ptr() % 16 == 0 else t.detach().clone() for t in pre]
         got = (_ff_output("dx", out[0], (m, k), x), _ff_output("dw_gate", out[1], (k, f), x),
                _ff_output("dw_up", out[2], (k, f), x), _ff_output("dw_down", out[3], (f, d), x))
         dt, stream = _FLOATS[x.dtype].value, _raw_stream(index)

@@ -97,11 +97,17 @@ template <int EPI>
 int launch_simt(int act, const FfProduct& p, cudaStream_t s) {
     const dim3 grid((p.M + kTile - 1) / kTile, (p.N + kTile - 1) / kTile);
     if (grid.y > 65535u) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many columns");
-    switch (EPI == kFfStore ? ZG_ACT_RELU : act) {
-        case ZG_ACT_SILU: ff_simt_kernel<EPI, ZG_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
-        case ZG_ACT_GELU: ff_simt_kernel<EPI, ZG_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
-        case ZG_ACT_GELU_TANH: ff_simt_kernel<EPI, ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
-        default: ff_simt_kernel<EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
+    if constexpr (EPI == kFfStore) {
+        ff_simt_kernel<EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p);
+    } else {
+        switch (act) {
+            case ZG_ACT_SILU: ff_simt_kernel<EPI, ZG_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
+            case ZG_ACT_GELU: ff_simt_kernel<EPI, ZG_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
+            case ZG_ACT_GELU_TANH:
+                ff_simt_kernel<EPI, ZG_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p);
+                break;
+            default: ff_simt_kernel<EPI, ZG_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
+        }
     }
     return cuda_status(cudaGetLastError(), "gated_ff");
 }

@@ -179,13 +179,11 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ P
 }
 
 void shape_y(const FfCall& c, FfProduct& p) { p.M = c.m, p.N = c.d, p.k[0] = c.f, p.ldc = c.d; }
-void shape_dx(const FfCall& c, FfProduct& p) {
-    p.M = c.m, p.N = c.k, p.k[0] = p.k[1] = c.f, p.ldc = c.k;
-}
-void shape_dw(const FfCall& c, FfProduct (&p)[3]) {  // dWg, dWu, dWd
-    for (FfProduct& q : p) q.k[0] = c.m;
-    p[0].M = p[1].M = c.k, p[0].N = p[1].N = c.f, p[0].ldc = p[1].ldc = c.f;
-    p[2].M = c.f, p[2].N = c.d, p[2].ldc = c.d;
+void shape_grads(const FfCall& c, FfProduct (&p)[4]) {  // dx, dWg, dWu, dWd
+    p[0].M = c.m, p[0].N = c.k, p[0].k[0] = p[0].k[1] = c.f, p[0].ldc = c.k;
+    for (int i = 1; i < 4; ++i) p[i].k[0] = c.m;
+    p[1].M = p[2].M = c.k, p[1].N = p[2].N = c.f, p[1].ldc = p[2].ldc = c.f;
+    p[3].M = c.f, p[3].N = c.d, p[3].ldc = c.d;
 }
 
 // Workspace: h, then for the backward pass dg and du, [m, f] each; then padded
@@ -196,7 +194,7 @@ struct FfLayout {
     uint64_t plane, total;
     bool pad[kInputs];
     uint64_t at[kInputs];
-    uint64_t parts;  // of split sums; the launches that use it follow one another
+    uint64_t parts;  // of split sums
 };
 FfLayout ff_layout(const FfCall& c) {
     FfLayout l;
@@ -211,10 +209,9 @@ FfLayout ff_layout(const FfCall& c) {
     }
     l.parts = l.total;
     if (c.size == 2) {
-        FfProduct y, dx, dw[3];
-        shape_y(c, y), shape_dx(c, dx), shape_dw(c, dw);
-        l.total += c.backward ? std::max(ff_split_bytes(&dx, 1), ff_split_bytes(dw, 3))
-                              : ff_split_bytes(&y, 1);
+        FfProduct y, grads[4];
+        shape_y(c, y), shape_grads(c, grads);
+        l.total += c.backward ? ff_split_bytes(grads, 4) : ff_split_bytes(&y, 1);
     }
     return l;
 }
@@ -404,25 +401,23 @@ uint64_t tf32x3_backward(const FfCall& c, const F32Tensors& t, uint8_t* ws, cuda
     for (FfOperand& o : turned)
         o = operand(gemm_carve_planes(p.take(gemm_planes_bytes(c.mode, c.f, c.m)), c.mode, c.f, c.m));
     float* dh = p.matrix(c.m, c.f);
-    FfProduct h, dx, dw[3];
+    FfProduct h, grads[4];
     h.M = c.m, h.N = h.ldc = c.f, h.k[0] = c.d;
     h.a[0] = operand(dy), h.b[0] = operand(wd), h.c = dh;
-    shape_dx(c, dx), shape_dw(c, dw);
-    dx.k[0] = 2 * gemm_planes_k(c.mode, c.f), dx.k[1] = 0;
-    dx.a[0] = operand(dg), dx.b[0] = operand(w), dx.c = t.dx;
-    dw[0].a[0] = dw[1].a[0] = operand(xt);
-    dw[0].b[0] = turned[0], dw[0].c = t.dwg;
-    dw[1].b[0] = turned[1], dw[1].c = t.dwu;
-    dw[2].a[0] = turned[2], dw[2].b[0] = operand(dyt), dw[2].c = t.dwd;
+    shape_grads(c, grads);
+    grads[0].k[0] = 2 * gemm_planes_k(c.mode, c.f), grads[0].k[1] = 0;
+    grads[0].a[0] = operand(dg), grads[0].b[0] = operand(w), grads[0].c = t.dx;
+    grads[1].a[0] = grads[2].a[0] = operand(xt);
+    grads[1].b[0] = turned[0], grads[1].c = t.dwg;
+    grads[2].b[0] = turned[1], grads[2].c = t.dwu;
+    grads[3].a[0] = turned[2], grads[3].b[0] = operand(dyt), grads[3].c = t.dwd;
     float* parts = static_cast<float*>(
-        p.take(std::max({ff_f32_split_bytes(&h, 1), ff_f32_split_bytes(&dx, 1),
-                         ff_f32_split_bytes(dw, 3)})));
+        p.take(std::max(ff_f32_split_bytes(&h, 1), ff_f32_split_bytes(grads, 4))));
     if (ws && !p.rc) p.rc = ff_f32(&h, 1, parts, s);
     if (ws && !p.rc)
         p.rc = ff_f32_slope(c.act, t.pre_g, t.pre_u, dh, c.m, c.f, operand(dg), operand(du),
                             turned, s);
-    if (ws && !p.rc) p.rc = ff_f32(&dx, 1, parts, s);
-    if (ws && !p.rc) p.rc = ff_f32(dw, 3, parts, s);
+    if (ws && !p.rc) p.rc = ff_f32(grads, 4, parts, s);
     *rc = p.rc;
     return p.used;
 }
@@ -622,20 +617,17 @@ extern "C" int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, in
     p.c = dg, p.c2 = du, p.c3 = h, p.ldc = l.ld_f;
     p.pre_g = const_cast<float*>(pre_gate), p.pre_u = const_cast<float*>(pre_up);
     if ((rc = products(c, kFfSlope, &p, 1, nullptr, s))) return rc;
-    FfProduct q;
-    shape_dx(c, q);
-    q.a[0] = {dg, l.ld_f, false};
-    q.b[0] = {in[kWg].p, in[kWg].ld, false};
-    q.a[1] = {du, l.ld_f, false};
-    q.b[1] = {in[kWu].p, in[kWu].ld, false};
-    q.c = dx;
-    if ((rc = products(c, kFfStore, &q, 1, ws + l.parts, s))) return rc;
-    FfProduct w[3];
-    shape_dw(c, w);
-    w[0].a[0] = w[1].a[0] = {in[kX].p, in[kX].ld, true};
-    w[0].b[0] = {dg, l.ld_f, true}, w[0].c = dw_gate;
-    w[1].b[0] = {du, l.ld_f, true}, w[1].c = dw_up;
-    w[2].a[0] = {h, l.ld_f, true};
-    w[2].b[0] = {in[kDy].p, in[kDy].ld, true}, w[2].c = dw_down;
-    return products(c, kFfStore, w, 3, ws + l.parts, s);
+    FfProduct w[4];
+    shape_grads(c, w);
+    w[0].a[0] = {dg, l.ld_f, false};
+    w[0].b[0] = {in[kWg].p, in[kWg].ld, false};
+    w[0].a[1] = {du, l.ld_f, false};
+    w[0].b[1] = {in[kWu].p, in[kWu].ld, false};
+    w[0].c = dx;
+    w[1].a[0] = w[2].a[0] = {in[kX].p, in[kX].ld, true};
+    w[1].b[0] = {dg, l.ld_f, true}, w[1].c = dw_gate;
+    w[2].b[0] = {du, l.ld_f, true}, w[2].c = dw_up;
+    w[3].a[0] = {h, l.ld_f, true};
+    w[3].b[0] = {in[kDy].p, in[kDy].ld, true}, w[3].c = dw_down;
+    return products(c, kFfStore, w, 4, ws + l.parts, s);
 }

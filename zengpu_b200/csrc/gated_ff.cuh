@@ -45,7 +45,8 @@ struct ActValue {
 };
 
 // FAST (16-bit tensors): __expf, whose error grows to 2^-18 relative at |g| = 30,
-// far below the rounding that follows; f32 tensors take expf and a true quotient.
+// far below the rounding that follows, and a published polynomial for erfc; f32
+// tensors take expf, erfcf and a true quotient.
 template <bool FAST>
 __device__ __forceinline__ float logistic(float x) {
     return FAST ? __frcp_rn(1.0f + __expf(-x)) : 1.0f / (1.0f + expf(-x));
@@ -58,10 +59,23 @@ __device__ __forceinline__ ActValue activate(float g) {
         const float s = logistic<FAST>(g);
         return {g * s, s * (1.0f + g * (1.0f - s))};
     }
+    if (ACT == ZG_ACT_GELU && FAST) {
+        // Abramowitz and Stegun 7.1.26: erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2) for z >= 0,
+        // t = 1 / (1 + 0.3275911 z), within 1.5e-7; z = |g| / sqrt 2 makes the exponential
+        // the density's
+        const float e = __expf(-0.5f * g * g);
+        const float t = __frcp_rn(fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.0f));
+        float p = fmaf(1.061405429f, t, -1.453152027f);
+        p = fmaf(p, t, 1.421413741f);
+        p = fmaf(p, t, -0.284496736f);
+        p = fmaf(p, t, 0.254829592f);
+        const float tail = 0.5f * p * t * e;  // Phi(-|g|)
+        const float c = g > 0.0f ? 1.0f - tail : tail;
+        return {g * c, fmaf(g * 0.39894228040143268f, e, c)};
+    }
     if (ACT == ZG_ACT_GELU) {
         const float c = 0.5f * erfcf(-0.70710678118654752f * g);
-        const float e = -0.5f * g * g;
-        return {g * c, c + g * 0.39894228040143268f * (FAST ? __expf(e) : expf(e))};
+        return {g * c, c + g * 0.39894228040143268f * expf(-0.5f * g * g)};
     }
     const float k = 0.79788456080286536f;
     const float q = k * (g + 0.044715f * g * g * g);
@@ -119,17 +133,15 @@ int launch_dependent(const char* what, void (*kernel)(Params...), unsigned grid,
 int ff_simt(FfEpilogue epi, int act, const FfProduct& p, cudaStream_t s);
 
 // 16-bit tensors on the tensor cores (gated_ff_tc.cu): `count` products of one
-// epilogue in one launch (at most three).  Operands: 16-byte aligned, pitch a
-// multiple of 8.  kFfStore: ff_splits says into how many parts the sums are split,
-// for which `parts` holds ff_split_bytes; ldc is N then.
-int ff_splits(const FfProduct* products, int count);
+// epilogue in one launch (at most four).  Operands: 16-byte aligned, pitch a multiple
+// of 8.  kFfStore: long sums of few tiles are split, for which `parts` holds
+// ff_split_bytes; ldc is N then.
 uint64_t ff_split_bytes(const FfProduct* products, int count);
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
             float* parts, cudaStream_t s);
 
 // f32 tensors in the TF32X3 mode (gated_ff_f32.cu), operands as planes (sgemm_tc.cu,
 // k-major, ld in floats), k[0] the sum's length; kFfStore only, parts as ff_pair's.
-int ff_f32_splits(const FfProduct* products, int count);
 uint64_t ff_f32_split_bytes(const FfProduct* products, int count);
 int ff_f32(const FfProduct* products, int count, float* parts, cudaStream_t s);
 // h = act(g) u as planes [m, n]; dg and du as planes, and dg, du and h transposed.

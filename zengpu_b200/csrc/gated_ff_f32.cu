@@ -40,6 +40,7 @@ struct alignas(64) F32Problem {
 struct F32Args {
     F32Problem p[kMaxProblems];
     int count;
+    Deal deal;
     uint32_t* status;
 };
 
@@ -87,8 +88,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
-    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-    const int units = args.p[args.count - 1].tiles;
+    const int pair = blockIdx.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -114,7 +114,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int u = pair; u < units && ok; u += npairs) {
+            for (int j = 0, u; ok && (u = unit_at(args.deal, pair, j)) >= 0; ++j) {
                 const F32Unit w = f32_unit(args, u);
                 const int half = 128 * static_cast<int>(rank);
                 for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
@@ -138,7 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (leader && lane == 0) {
             bool ok = true;
             int it = 0, n = 0;  // stages and chunks so far
-            for (int u = pair; u < units && ok; u += npairs) {
+            for (int j = 0, u; ok && (u = unit_at(args.deal, pair, j)) >= 0; ++j) {
                 const F32Unit w = f32_unit(args, u);
                 for (int kc = w.kb0; kc < w.kb1 && ok; kc += kChunk, ++n) {
                     const int buf = n & 1;
@@ -185,7 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint8_t* turn = turns + (warp - 2) * kTurnBytes;
         bool ok = true;
         int n = 0;
-        for (int u = pair; u < units && ok; u += npairs) {
+        for (int j = 0, u; ok && (u = unit_at(args.deal, pair, j)) >= 0; ++j) {
             const F32Unit w = f32_unit(args, u);
             const F32Problem& p = *w.p;
             float acc[64] = {};
@@ -348,10 +348,8 @@ int plane_map(CUtensorMap* map, const FfOperand& o, int rows, int nkb) {
 
 }  // namespace
 
-int ff_f32_splits(const FfProduct* products, int count) { return splits_of(products, count, 64); }
-
 uint64_t ff_f32_split_bytes(const FfProduct* products, int count) {
-    return split_bytes(products, count, ff_f32_splits(products, count));
+    return split_bytes(products, count, 64);
 }
 
 int ff_f32(const FfProduct* products, int count, float* parts, cudaStream_t s) {
@@ -359,28 +357,25 @@ int ff_f32(const FfProduct* products, int count, float* parts, cudaStream_t s) {
     std::memset(&args, 0, sizeof(args));
     args.count = count;
     int rc = status_word(&args.status), tiles = 0;
-    const int splits = ff_f32_splits(products, count);
+    int splits[kMaxProblems];
+    splits_of(products, count, 64, splits);
     SumArgs sum;
-    sum.count = count, sum.splits = splits;
-    int64_t groups = 0;
+    sum.count = 0;
     for (int i = 0; i < count && !rc; ++i) {
         const FfProduct& f = products[i];
         F32Problem& p = args.p[i];
-        p.M = f.M, p.N = f.N, p.nkb = (f.k[0] + kBK - 1) / kBK, p.splits = splits;
+        p.M = f.M, p.N = f.N, p.nkb = (f.k[0] + kBK - 1) / kBK, p.splits = splits[i];
         p.c = static_cast<float*>(f.c), p.ldc = f.ldc;
         p.vec_c = f.ldc % 4 == 0 && aligned16(f.c);
-        if (splits > 1) {
-            const int ldp = (f.N + 3) / 4 * 4;
-            p.plane = static_cast<int64_t>(f.M) * ldp;
-            groups += p.plane / 4;
-            sum.m[i] = {parts, f.c, p.plane, groups, f.N, ldp};
-            p.c = parts, p.ldc = ldp, p.vec_c = 1;
-            parts += p.plane * splits;
+        if (splits[i] > 1) {
+            p.c = parts, p.vec_c = 1;
+            add_parts(sum, f, splits[i], parts);
+            p.plane = sum.m[sum.count - 1].plane, p.ldc = sum.m[sum.count - 1].ldp;
         }
         rc = plane_map(&p.a, f.a[0], f.M, p.nkb);
         if (!rc) rc = plane_map(&p.b, f.b[0], f.N, p.nkb);
         const int64_t total =
-            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256) * splits;
+            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256) * splits[i];
         if (total > (1 << 29)) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many tiles");
         p.tiles = tiles = static_cast<int>(total);
     }
@@ -388,12 +383,11 @@ int ff_f32(const FfProduct* products, int count, float* parts, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(ff_f32_kernel, kSmem, done);
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
-    rc = launch_dependent("gated_ff", ff_f32_kernel, 2 * std::min(tiles, sm_pairs()), kThreads,
-                          kSmem, s, args);
-    if (rc || splits == 1) return rc;
-    return launch_dependent("gated_ff sum", ff_sum_kernel<float>,
-                            static_cast<unsigned>(std::min<int64_t>((groups + 255) / 256, 148 * 16)),
-                            256, 0, s, sum);
+    auto unit_time = [&](int i) { return args.p[i].nkb / splits[i] + 8; };  // in stages
+    args.deal = deal_of(tiles, sm_pairs(), args.p[0].tiles,
+                        count > 1 ? unit_time(0) / unit_time(1) : 0);
+    rc = launch_dependent("gated_ff", ff_f32_kernel, 2 * args.deal.pairs, kThreads, kSmem, s, args);
+    return rc ? rc : launch_sum<float>(sum, s);
 }
 
 int ff_f32_act(int act, const float* g, const float* u, int m, int n, const FfOperand& h,

@@ -11,7 +11,7 @@
 namespace zg {
 namespace {
 
-constexpr int kMaxProblems = 3;
+constexpr int kMaxProblems = 4;  // of a launch: dx and the three weights' gradients
 constexpr int kPairsSold = 74;  // SM pairs of a B200: what split sums are dealt out for
 
 // Grouped raster, as sgemm_tc.cu's (eight row tiles before the next column).
@@ -20,6 +20,30 @@ __device__ __forceinline__ void raster(int tile, int mt, int nt, int& mi, int& n
     const int gm = min(mt - first, 8), r = tile - group * 8 * nt;
     mi = first + r % gm;
     ni = r / gm;
+}
+
+// Which unit of work an SM pair takes in its turn j: its own remainder of the units,
+// unless the first `longs` of them take much longer than the others (dx's sum is 2 f
+// long, the weights' gradients' m).  Then the long ones are dealt out first, and the
+// pairs that got one less take `extra` short ones before the rest go around.
+struct Deal {
+    int units, pairs, longs, extra;
+};
+__device__ __forceinline__ int unit_at(const Deal& d, int pair, int j) {
+    const int over = d.longs % d.pairs;  // pairs with one long unit more
+    const int own = d.longs / d.pairs + (pair < over);
+    if (j < own) return pair + j * d.pairs;
+    j -= own;
+    int rest = d.longs;
+    if (over) {
+        if (pair >= over) {
+            if (j < d.extra) return rest + (pair - over) * d.extra + j;
+            j -= d.extra;
+        }
+        rest += d.extra * (d.pairs - over);
+    }
+    const int u = rest + (pair - over + d.pairs) % d.pairs + j * d.pairs;
+    return u < d.units ? u : -1;
 }
 
 // An epilogue warp turns blocks of 32 x 32 between "a row per lane" (TMEM) and
@@ -81,9 +105,9 @@ struct SumArgs {
         const float* part;
         void* c;
         int64_t plane, groups;  // groups of this matrix and those before it
-        int N, ldp;
+        int N, ldp, splits;
     } m[kMaxProblems];
-    int count, splits;
+    int count;
 };
 template <class T>
 __global__ void __launch_bounds__(256) ff_sum_kernel(const __grid_constant__ SumArgs a) {
@@ -98,7 +122,7 @@ __global__ void __launch_bounds__(256) ff_sum_kernel(const __grid_constant__ Sum
         const int64_t row = at / m.ldp;
         const int col = static_cast<int>(at - row * m.ldp);
         float4 sum = __ldcs(reinterpret_cast<const float4*>(m.part + at));
-        for (int s = 1; s < a.splits; ++s) {
+        for (int s = 1; s < m.splits; ++s) {
             const float4 x = __ldcs(reinterpret_cast<const float4*>(m.part + s * m.plane + at));
             sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
         }
@@ -129,25 +153,58 @@ inline int sm_pairs() {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Into how many parts products of few 256 x 256 tiles split their sums, stages of
-// `step`: as many as the SM pairs take, sixteen at most, four stages each at least.
-inline int splits_of(const FfProduct* products, int count, int step) {
-    int64_t tiles = 0;
-    int nkb = 1 << 30;
+// Into how many parts each product of a launch splits its sum, in stages of `step`:
+// as many as leave no unit with more than an SM pair's share of all the stages, but
+// sixteen at most, and four stages to a part at least.
+inline void splits_of(const FfProduct* products, int count, int step, int (&splits)[kMaxProblems]) {
+    int64_t tiles[kMaxProblems], nkb[kMaxProblems], all = 0;
     for (int i = 0; i < count; ++i) {
         const FfProduct& f = products[i];
-        tiles += static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256);
-        nkb = std::min(nkb, (f.k[0] + step - 1) / step + (f.k[1] + step - 1) / step);
+        tiles[i] = static_cast<int64_t>((f.M + 255) / 256) * ((f.N + 255) / 256);
+        nkb[i] = (f.k[0] + step - 1) / step + (f.k[1] + step - 1) / step;
+        all += tiles[i] * nkb[i];
     }
-    return static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>({16, kPairsSold / std::max<int64_t>(tiles, 1), nkb / 4})));
-}
-inline uint64_t split_bytes(const FfProduct* products, int count, int splits) {
-    if (splits == 1) return 0;
-    uint64_t elems = 0;
+    const int64_t share = std::max<int64_t>((all + kPairsSold - 1) / kPairsSold, 1);
     for (int i = 0; i < count; ++i)
-        elems += static_cast<uint64_t>(products[i].M) * ((products[i].N + 3) / 4 * 4);
-    return elems * splits * 4;
+        splits[i] = static_cast<int>(std::max<int64_t>(
+            1, std::min<int64_t>({16, (nkb[i] + share / 2) / share, nkb[i] / 4})));
+}
+inline uint64_t split_bytes(const FfProduct* products, int count, int step) {
+    int splits[kMaxProblems];
+    splits_of(products, count, step, splits);
+    uint64_t bytes = 0;
+    for (int i = 0; i < count; ++i)
+        if (splits[i] > 1)
+            bytes += static_cast<uint64_t>(products[i].M) * ((products[i].N + 3) / 4 * 4) *
+                     splits[i] * 4;
+    return bytes;
+}
+// Notes a split product for ff_sum_kernel; its parts begin at `parts`, which moves on.
+inline void add_parts(SumArgs& sum, const FfProduct& f, int splits, float*& parts) {
+    const int ldp = (f.N + 3) / 4 * 4;
+    const int64_t plane = static_cast<int64_t>(f.M) * ldp;
+    const int64_t before = sum.count ? sum.m[sum.count - 1].groups : 0;
+    sum.m[sum.count++] = {parts, f.c, plane, before + plane / 4, f.N, ldp, splits};
+    parts += plane * splits;
+}
+template <class T>
+int launch_sum(const SumArgs& sum, cudaStream_t s) {
+    if (!sum.count) return ZG_OK;
+    const int64_t groups = sum.m[sum.count - 1].groups;
+    return launch_dependent("gated_ff sum", ff_sum_kernel<T>,
+                            static_cast<unsigned>(std::min<int64_t>((groups + 255) / 256, 148 * 16)),
+                            256, 0, s, sum);
+}
+
+// The deal for `units`, of which the first `longs` take `ratio` times the others' time.
+inline Deal deal_of(int units, int pairs, int longs, int ratio) {
+    Deal d{units, std::min(units, pairs), 0, 0};
+    if (ratio >= 2 && longs < units) {
+        d.longs = longs;
+        const int less = d.pairs - longs % d.pairs;
+        d.extra = std::min(ratio, (units - longs) / less);
+    }
+    return d;
 }
 
 template <class Kernel>

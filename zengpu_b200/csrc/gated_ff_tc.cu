@@ -20,8 +20,8 @@
 // columns of Wu: one accumulator holds 128 columns of g beside 128 of u, the
 // epilogue threads find both for their row, and neither goes through memory.
 // dh's epilogue reads g and u and writes dg, du and h; dh itself stays in TMEM.
-// dx sums two products in one accumulator; the three weights' gradients share one
-// launch.
+// dx sums two products in one accumulator; it and the three weights' gradients share
+// one launch.
 //
 // Roles as in the f32 kernels (sgemm_tc.cu): warp 0 TMA, warp 1 MMA (CTA 0 of the
 // pair issues), warps 2-9 epilogue.  The f32 accumulator stays in TMEM over the
@@ -82,6 +82,7 @@ struct PairArgs {
     PairProblem p[kMaxProblems];
     int count;
     int full_units, split;
+    Deal deal;
     uint32_t* status;
 };
 
@@ -192,9 +193,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
-    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-    const int units =
-        args.full_units + (args.p[args.count - 1].tiles - args.full_units) * args.split;
+    const int pair = blockIdx.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -223,7 +222,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int u = pair; u < units && ok; u += npairs) {
+            for (int j = 0, u; ok && (u = unit_at(args.deal, pair, j)) >= 0; ++j) {
                 const Unit w = unit_of<EPI>(args, u);
                 const PairProblem& p = *w.p;
                 const int b_rows = w.width / 2;
@@ -256,8 +255,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // ---------------- MMA issuer (CTA 0) ----------------
         if (leader && lane == 0) {
             bool ok = true;
-            int it = 0, n = 0;
-            for (int u = pair; u < units && ok; u += npairs, ++n) {
+            int it = 0;
+            for (int n = 0, u; ok && (u = unit_at(args.deal, pair, n)) >= 0; ++n) {
                 const Unit w = unit_of<EPI>(args, u);
                 const PairProblem& p = *w.p;
                 const int buf = n & 1;
@@ -300,8 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t leader_empty1 = mapa_shared(&acc_empty[1], 0);
         uint8_t* turn = turns + (warp - 2) * kTurnBytes[EPI];
         uint8_t *turn_g = turn + kBlock16, *turn_u = turn_g + kBlock32;  // dh's epilogue
-        int n = 0;
-        for (int u = pair; u < units; u += npairs, ++n) {
+        for (int n = 0, u; (u = unit_at(args.deal, pair, n)) >= 0; ++n) {
             const Unit w = unit_of<EPI>(args, u);
             const PairProblem& p = *w.p;
             const int64_t row0 = w.m0 + 128 * static_cast<int>(rank) + q * 32;
@@ -411,37 +409,35 @@ int operand_map(CUtensorMap* map, uint32_t dtype, const FfOperand& o, int rows, 
 }
 
 template <int EPI, int ACT, class T>
-int launch(const PairArgs& args, int units, cudaStream_t s) {
+int launch(const PairArgs& args, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(ff_pair_kernel<EPI, ACT, T>, smem_bytes(EPI), done);
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
-    return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T>, 2 * std::min(units, sm_pairs()),
+    return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T>, 2 * args.deal.pairs,
                             kThreads, smem_bytes(EPI), s, args);
 }
 
 template <class T>
-int launch_epi(FfEpilogue epi, int act, const PairArgs& a, int units, cudaStream_t s) {
-    if (epi == kFfStore) return launch<kFfStore, ZG_ACT_RELU, T>(a, units, s);
+int launch_epi(FfEpilogue epi, int act, const PairArgs& a, cudaStream_t s) {
+    if (epi == kFfStore) return launch<kFfStore, ZG_ACT_RELU, T>(a, s);
     if (epi == kFfGated) switch (act) {
-            case ZG_ACT_SILU: return launch<kFfGated, ZG_ACT_SILU, T>(a, units, s);
-            case ZG_ACT_GELU: return launch<kFfGated, ZG_ACT_GELU, T>(a, units, s);
-            case ZG_ACT_GELU_TANH: return launch<kFfGated, ZG_ACT_GELU_TANH, T>(a, units, s);
-            default: return launch<kFfGated, ZG_ACT_RELU, T>(a, units, s);
+            case ZG_ACT_SILU: return launch<kFfGated, ZG_ACT_SILU, T>(a, s);
+            case ZG_ACT_GELU: return launch<kFfGated, ZG_ACT_GELU, T>(a, s);
+            case ZG_ACT_GELU_TANH: return launch<kFfGated, ZG_ACT_GELU_TANH, T>(a, s);
+            default: return launch<kFfGated, ZG_ACT_RELU, T>(a, s);
         }
     switch (act) {
-        case ZG_ACT_SILU: return launch<kFfSlope, ZG_ACT_SILU, T>(a, units, s);
-        case ZG_ACT_GELU: return launch<kFfSlope, ZG_ACT_GELU, T>(a, units, s);
-        case ZG_ACT_GELU_TANH: return launch<kFfSlope, ZG_ACT_GELU_TANH, T>(a, units, s);
-        default: return launch<kFfSlope, ZG_ACT_RELU, T>(a, units, s);
+        case ZG_ACT_SILU: return launch<kFfSlope, ZG_ACT_SILU, T>(a, s);
+        case ZG_ACT_GELU: return launch<kFfSlope, ZG_ACT_GELU, T>(a, s);
+        case ZG_ACT_GELU_TANH: return launch<kFfSlope, ZG_ACT_GELU_TANH, T>(a, s);
+        default: return launch<kFfSlope, ZG_ACT_RELU, T>(a, s);
     }
 }
 
 }  // namespace
 
-int ff_splits(const FfProduct* products, int count) { return splits_of(products, count, kBK); }
-
 uint64_t ff_split_bytes(const FfProduct* products, int count) {
-    return split_bytes(products, count, ff_splits(products, count));
+    return split_bytes(products, count, kBK);
 }
 
 int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, int count,
@@ -450,10 +446,10 @@ int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, 
     std::memset(&args, 0, sizeof(args));
     args.count = count;
     int rc = status_word(&args.status), tiles = 0;
-    const int splits = epi == kFfStore ? ff_splits(products, count) : 1;
+    int splits[kMaxProblems] = {1, 1, 1, 1};
+    if (epi == kFfStore) splits_of(products, count, kBK, splits);
     SumArgs sum;
-    sum.count = count, sum.splits = splits;
-    int64_t groups = 0;
+    sum.count = 0;
     const int cols = epi == kFfGated ? 128 : 256;
     for (int i = 0; i < count && !rc; ++i) {
         const FfProduct& f = products[i];
@@ -465,36 +461,35 @@ int ff_pair(uint32_t dtype, FfEpilogue epi, int act, const FfProduct* products, 
         p.vec_c = f.ldc % 8 == 0 && aligned16(f.c) && aligned16(f.c2) && aligned16(f.c3);
         p.vec_pre = f.N % 4 == 0 && aligned16(f.pre_g) && aligned16(f.pre_u);
         for (int seg = 0; seg < 2; ++seg) p.nkb[seg] = (f.k[seg] + kBK - 1) / kBK;
-        p.splits = splits;
-        if (splits > 1) {  // f32 parts first
-            const int ldp = (f.N + 3) / 4 * 4;
-            p.plane = static_cast<int64_t>(f.M) * ldp;
-            groups += p.plane / 4;
-            sum.m[i] = {parts, f.c, p.plane, groups, f.N, ldp};
-            p.c = parts, p.ldc = ldp;
-            parts += p.plane * splits;
+        p.splits = splits[i];
+        if (splits[i] > 1) {  // f32 parts first
+            p.c = parts;
+            add_parts(sum, f, splits[i], parts);
+            p.plane = sum.m[sum.count - 1].plane, p.ldc = sum.m[sum.count - 1].ldp;
         }
         rc = operand_map(&p.a[0], dtype, f.a[0], f.M, f.k[0]);
         if (!rc) rc = operand_map(&p.b[0], dtype, f.b[0], f.N, f.k[0]);
         if (!rc && f.k[1]) rc = operand_map(&p.a[1], dtype, f.a[1], f.M, f.k[1]);
         if (!rc && f.b[1].p) rc = operand_map(&p.b[1], dtype, f.b[1], f.N, f.k[1] ? f.k[1] : f.k[0]);
         const int64_t total =
-            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + cols - 1) / cols) * splits;
+            tiles + static_cast<int64_t>((f.M + 255) / 256) * ((f.N + cols - 1) / cols) * splits[i];
         if (total > (1 << 29)) return set_error(ZG_ERR_DISPATCH, "gated_ff: too many tiles");
         p.tiles = tiles = static_cast<int>(total);
     }
     if (rc) return rc;
+    // the last wave's tiles in halves, where the units are of one kind
     const int pairs = sm_pairs(), rem = tiles % pairs;
-    args.split = rem > 0 && 2 * rem <= pairs ? 2 : 1;
+    args.split = count == 1 && rem > 0 && 2 * rem <= pairs ? 2 : 1;
     args.full_units = args.split > 1 ? tiles - rem : tiles;
-    const int units = args.full_units + (tiles - args.full_units) * args.split;
-    rc = dtype == ZG_DTYPE_BF16 ? launch_epi<__nv_bfloat16>(epi, act, args, units, s)
-                                : launch_epi<__half>(epi, act, args, units, s);
-    if (rc || splits == 1) return rc;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((groups + 255) / 256, 148 * 16));
-    return dtype == ZG_DTYPE_BF16
-               ? launch_dependent("gated_ff sum", ff_sum_kernel<__nv_bfloat16>, grid, 256, 0, s, sum)
-               : launch_dependent("gated_ff sum", ff_sum_kernel<__half>, grid, 256, 0, s, sum);
+    auto unit_time = [&](int i) {  // in stages; an epilogue takes about eight
+        return (args.p[i].nkb[0] + args.p[i].nkb[1]) / splits[i] + 8;
+    };
+    args.deal = deal_of(args.full_units + (tiles - args.full_units) * args.split, pairs,
+                        args.p[0].tiles, count > 1 ? unit_time(0) / unit_time(1) : 0);
+    rc = dtype == ZG_DTYPE_BF16 ? launch_epi<__nv_bfloat16>(epi, act, args, s)
+                                : launch_epi<__half>(epi, act, args, s);
+    if (rc) return rc;
+    return dtype == ZG_DTYPE_BF16 ? launch_sum<__nv_bfloat16>(sum, s) : launch_sum<__half>(sum, s);
 }
 
 }  // namespace zg

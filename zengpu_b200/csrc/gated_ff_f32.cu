@@ -222,7 +222,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 uint32_t v[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[32 * h + i]);
-                store_block<float>(p.c + w.part * p.plane + row0 * p.ldc + col, p.ldc, rows, cols,
+                store_block<float, 32>(p.c + w.part * p.plane + row0 * p.ldc + col, p.ldc, rows, cols,
                                    p.vec_c, v, turn, lane);
             }
         }

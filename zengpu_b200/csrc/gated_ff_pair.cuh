@@ -52,14 +52,14 @@ __device__ __forceinline__ int unit_at(const Deal& d, int pair, int j) {
 // of either kind meet no bank twice.
 template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
 
-// Stores a warp's 32 x 32 block of T, row `lane` in the words of v, at `dst` (its
-// row 0, column 0); `rows` and `cols` of it lie inside the matrix.  vec: 16-byte
-// pieces of rows; otherwise (odd pitch or base) neighbours side by side.
-template <class T>
+// Stores a warp's block of 32 rows of WORDS 32-bit words, row `lane` in v, at `dst` (its
+// row 0, column 0); `rows` rows and `cols` elements of T of it lie inside the matrix.
+// vec: 16-byte pieces of rows; otherwise (odd pitch or base) neighbours side by side.
+template <class T, int WORDS>
 __device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int cols, bool vec,
-                                            const uint32_t (&v)[8 * sizeof(T)], uint8_t* turn,
-                                            int lane) {
-    constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer, kTurnPitch = kPitch<T>;
+                                            const uint32_t (&v)[WORDS], uint8_t* turn, int lane) {
+    constexpr int kPieces = WORDS / 4, kPer = 16 / sizeof(T), kTurnPitch = WORDS * 4 + 16;
+    constexpr int kCols = WORDS * 4 / sizeof(T);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
@@ -75,20 +75,20 @@ __device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int co
                     *reinterpret_cast<const uint4*>(turn + r * kTurnPitch + piece * 16);
         }
     } else if (sizeof(T) == 2) {
-        // two rows a turn, 16 lanes each, in aligned words of two elements: 2 l and
-        // 2 l + 1, or in a row that starts inside a word one further, and then
-        // elements 0 and 31 alone
-        const int l = lane & 15;
-        for (int r = lane >> 4; r < rows; r += 2) {
+        // WORDS lanes to a row, in aligned words of two elements: 2 l and 2 l + 1, or in
+        // a row that starts inside a word one further, and then the first and the last
+        // element alone
+        const int l = lane % WORDS, most = min(cols, kCols);
+        for (int r = lane / WORDS; r < rows; r += 32 / WORDS) {
             T* to = dst + r * ld;
             const T* from = reinterpret_cast<const T*>(turn + r * kTurnPitch);
             const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1, e = 2 * l + odd;
-            if (e + 1 < min(cols, 32)) {
+            if (e + 1 < most) {
                 T pair[2] = {from[e], from[e + 1]};
                 uint32_t word;
                 __builtin_memcpy(&word, pair, 4);
                 *reinterpret_cast<uint32_t*>(to + e) = word;
-            } else if (e < cols) {
+            } else if (e < most) {
                 to[e] = from[e];
             }
             if (odd && l == 0 && cols > 0) to[0] = from[0];

@@ -330,25 +330,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 T* c = static_cast<T*>(p.c) + at;
                 auto f = [](uint32_t x) { return __uint_as_float(x); };
                 if (EPI == kFfStore && p.splits > 1) {
-                    store_block<float>(static_cast<float*>(p.c) + w.part * p.plane + at, p.ldc, rows,
+                    store_block<float, 32>(static_cast<float*>(p.c) + w.part * p.plane + at, p.ldc, rows,
                                        cols, true, r, turn, lane);
                 } else if (EPI == kFfStore) {
+                    // 64 columns a turn: 128 bytes of each row
+                    uint32_t w64[32];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
-                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                    for (int i = 0; i < 16; ++i) w64[i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
+                    tmem_ld_32x32b_x32(d + c0 + 32, r);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        w64[16 + i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
+                    store_block<T, 32>(c, p.ldc, rows, p.N - col, p.vec_c, w64, turn, lane);
+                    c0 += 32;
                 }
                 if (EPI == kFfGated) {
                     uint32_t x[32];
                     tmem_ld_32x32b_x32(d + w.width / 2 + c0, x);
                     if (p.pre_g) {
-                        store_block<float>(p.pre_g + pre, p.N, rows, cols, p.vec_pre, r, turn, lane);
-                        store_block<float>(p.pre_u + pre, p.N, rows, cols, p.vec_pre, x, turn, lane);
+                        store_block<float, 32>(p.pre_g + pre, p.N, rows, cols, p.vec_pre, r, turn, lane);
+                        store_block<float, 32>(p.pre_u + pre, p.N, rows, cols, p.vec_pre, x, turn, lane);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         o[i] = pair16<T>(activate<ACT, true>(f(r[2 * i])).a * f(x[2 * i]),
                                          activate<ACT, true>(f(r[2 * i + 1])).a * f(x[2 * i + 1]));
-                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                    store_block<T, 16>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
                 }
                 if (EPI == kFfSlope) {
                     uint32_t ou[16], oh[16];
@@ -380,10 +387,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                     if (c0 + 32 < end) fetch(c0 + 32);  // while this block is stored
-                    store_block<T>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
-                    store_block<T>(static_cast<T*>(p.c2) + at, p.ldc, rows, cols, p.vec_c, ou, turn,
+                    store_block<T, 16>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                    store_block<T, 16>(static_cast<T*>(p.c2) + at, p.ldc, rows, cols, p.vec_c, ou, turn,
                                    lane);
-                    store_block<T>(static_cast<T*>(p.c3) + at, p.ldc, rows, cols, p.vec_c, oh, turn,
+                    store_block<T, 16>(static_cast<T*>(p.c3) + at, p.ldc, rows, cols, p.vec_c, oh, turn,
                                    lane);
                 }
             }

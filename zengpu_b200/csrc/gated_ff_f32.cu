@@ -219,11 +219,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int col = w.n0 + group * 64 + 32 * h, cols = min(p.N - col, 32);
-                uint32_t v[32];
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[32 * h + i]);
-                store_block<float, 32>(p.c + w.part * p.plane + row0 * p.ldc + col, p.ldc, rows, cols,
-                                   p.vec_c, v, turn, lane);
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4*>(turn + lane * kPitch<float> + i * 4) =
+                        make_float4(acc[32 * h + i], acc[32 * h + i + 1], acc[32 * h + i + 2],
+                                    acc[32 * h + i + 3]);
+                __syncwarp();
+                flush_block<float, 32>(p.c + w.part * p.plane + row0 * p.ldc + col, p.ldc, rows,
+                                       cols, p.vec_c, turn, kPitch<float>, 16, lane);
             }
         }
     }

@@ -52,50 +52,51 @@ __device__ __forceinline__ int unit_at(const Deal& d, int pair, int j) {
 // of either kind meet no bank twice.
 template <class T> constexpr int kPitch = sizeof(T) * 32 + 16;
 
-// Stores a warp's block of 32 rows of WORDS 32-bit words, row `lane` in v, at `dst` (its
-// row 0, column 0); `rows` rows and `cols` elements of T of it lie inside the matrix.
-// vec: 16-byte pieces of rows; otherwise (odd pitch or base) neighbours side by side.
-template <class T, int WORDS>
-__device__ __forceinline__ void store_block(T* dst, int64_t ld, int rows, int cols, bool vec,
-                                            const uint32_t (&v)[WORDS], uint8_t* turn, int lane) {
-    constexpr int kPieces = WORDS / 4, kPer = 16 / sizeof(T), kTurnPitch = WORDS * 4 + 16;
-    constexpr int kCols = WORDS * 4 / sizeof(T);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-        *reinterpret_cast<uint4*>(turn + lane * kTurnPitch + i * 16) =
-            make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    __syncwarp();
+// Stores a warp's block of 32 rows and COLS columns of T from shared memory, rows `pitch`
+// bytes apart and their 16-byte pieces `step`, to `dst` (its row 0, column 0); `rows`
+// rows and `cols` columns of it lie inside the matrix.  vec: 16-byte pieces of rows;
+// otherwise (odd pitch or base) neighbours side by side.
+template <class T, int COLS>
+__device__ __forceinline__ void flush_block(T* dst, int64_t ld, int rows, int cols, bool vec,
+                                            const uint8_t* turn, int pitch, int step, int lane) {
+    constexpr int kPer = 16 / sizeof(T), kPieces = COLS / kPer;
     if (vec) {
-#pragma unroll
+#pragma unroll 4
         for (int j = 0; j < kPieces; ++j) {
             const int r = (j * 32 + lane) / kPieces, piece = lane % kPieces;
             if (r < rows && piece * kPer < cols)
                 *reinterpret_cast<uint4*>(dst + r * ld + piece * kPer) =
-                    *reinterpret_cast<const uint4*>(turn + r * kTurnPitch + piece * 16);
+                    *reinterpret_cast<const uint4*>(turn + r * pitch + piece * step);
         }
-    } else if (sizeof(T) == 2) {
-        // WORDS lanes to a row, in aligned words of two elements: 2 l and 2 l + 1, or in
+    } else if constexpr (sizeof(T) == 2) {
+        // COLS / 2 lanes to a row, in aligned words of two elements: 2 l and 2 l + 1, or in
         // a row that starts inside a word one further, and then the first and the last
         // element alone
-        const int l = lane % WORDS, most = min(cols, kCols);
-        for (int r = lane / WORDS; r < rows; r += 32 / WORDS) {
+        constexpr int kLanes = COLS / 2;
+        const int l = lane % kLanes, most = min(cols, COLS);
+        auto word = [&](int r, int w) {
+            return *reinterpret_cast<const uint32_t*>(turn + r * pitch + w / 4 * step + w % 4 * 4);
+        };
+        auto low = [](uint32_t w) {
+            T t;
+            __builtin_memcpy(&t, &w, 2);
+            return t;
+        };
+#pragma unroll 4
+        for (int r = lane / kLanes; r < rows; r += 32 / kLanes) {
             T* to = dst + r * ld;
-            const T* from = reinterpret_cast<const T*>(turn + r * kTurnPitch);
             const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1, e = 2 * l + odd;
-            if (e + 1 < most) {
-                T pair[2] = {from[e], from[e + 1]};
-                uint32_t word;
-                __builtin_memcpy(&word, pair, 4);
-                *reinterpret_cast<uint32_t*>(to + e) = word;
-            } else if (e < most) {
-                to[e] = from[e];
-            }
-            if (odd && l == 0 && cols > 0) to[0] = from[0];
+            const uint32_t first = word(r, l);
+            // the word after a row's last is its padding, read and not stored
+            const uint32_t pair = odd ? __funnelshift_r(first, word(r, l + 1), 16) : first;
+            if (e + 1 < most) *reinterpret_cast<uint32_t*>(to + e) = pair;
+            else if (e < most) to[e] = low(pair);
+            if (odd && l == 0 && cols > 0) to[0] = low(first);
         }
     } else if (lane < cols) {
+#pragma unroll 4
         for (int r = 0; r < rows; ++r)
-            dst[r * ld + lane] = reinterpret_cast<const T*>(turn + r * kTurnPitch)[lane];
+            dst[r * ld + lane] = *reinterpret_cast<const T*>(turn + r * pitch + lane * 4);
     }
 }
 

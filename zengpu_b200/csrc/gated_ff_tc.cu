@@ -322,76 +322,129 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after();
             const uint32_t d = lane_base + buf * 256;
-            for (int c0 = begin; c0 < end; c0 += 32) {
-                uint32_t r[32], o[16];
-                tmem_ld_32x32b_x32(d + c0, r);
-                const int col = w.n0 + c0, cols = min(p.N - col, 32);
+            constexpr int kStep = EPI == kFfStore ? 64 : 32;  // columns a turn
+            for (int c0 = begin; c0 < end; c0 += kStep) {
+                const int col = w.n0 + c0, cols = p.N - col;
                 const int64_t at = row0 * p.ldc + col, pre = row0 * p.N + col;
                 T* c = static_cast<T*>(p.c) + at;
+                uint8_t* mine32 = turn + lane * kPitch<float>;
+                uint8_t* mine16 = turn + lane * kPitch<T>;
                 auto f = [](uint32_t x) { return __uint_as_float(x); };
+                // 32 columns of D from `from` on, as they are, to an f32 matrix
+                auto put32 = [&](uint32_t from, float* to, int64_t ld, int width, bool vec) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < 32; i += 16) {
+                        uint32_t r[16];
+                        tmem_ld_32x32b_x16(from + i, r);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<uint4*>(mine32 + (i + e) * 4) =
+                                make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+                    }
+                    __syncwarp();
+                    flush_block<float, 32>(to, ld, rows, width, vec, turn, kPitch<float>, 16, lane);
+                };
                 if (EPI == kFfStore && p.splits > 1) {
-                    store_block<float, 32>(static_cast<float*>(p.c) + w.part * p.plane + at, p.ldc, rows,
-                                       cols, true, r, turn, lane);
+                    float* part = static_cast<float*>(p.c) + w.part * p.plane + at;
+#pragma unroll 1
+                    for (int h = 0; h < 64; h += 32)
+                        put32(d + c0 + h, part + h, p.ldc, cols - h, true);
                 } else if (EPI == kFfStore) {
-                    // 64 columns a turn: 128 bytes of each row
-                    uint32_t w64[32];
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < 64; i += 16) {
+                        uint32_t r[16];
+                        tmem_ld_32x32b_x16(d + c0 + i, r);
+                        uint32_t o[8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w64[i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
-                    tmem_ld_32x32b_x32(d + c0 + 32, r);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        w64[16 + i] = pair16<T>(f(r[2 * i]), f(r[2 * i + 1]));
-                    store_block<T, 32>(c, p.ldc, rows, p.N - col, p.vec_c, w64, turn, lane);
-                    c0 += 32;
+                        for (int e = 0; e < 8; ++e) o[e] = pair16<T>(f(r[2 * e]), f(r[2 * e + 1]));
+                        *reinterpret_cast<uint4*>(mine32 + i * 2) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(mine32 + i * 2 + 16) =
+                            make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                    __syncwarp();
+                    flush_block<T, 64>(c, p.ldc, rows, cols, p.vec_c, turn, kPitch<float>, 16, lane);
                 }
                 if (EPI == kFfGated) {
-                    uint32_t x[32];
-                    tmem_ld_32x32b_x32(d + w.width / 2 + c0, x);
+                    const uint32_t u0 = d + w.width / 2 + c0;
                     if (p.pre_g) {
-                        store_block<float, 32>(p.pre_g + pre, p.N, rows, cols, p.vec_pre, r, turn, lane);
-                        store_block<float, 32>(p.pre_u + pre, p.N, rows, cols, p.vec_pre, x, turn, lane);
+#pragma unroll 1
+                        for (int which = 0; which < 2; ++which)
+                            put32(which ? u0 : d + c0, (which ? p.pre_u : p.pre_g) + pre, p.N, cols,
+                                  p.vec_pre);
                     }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t g[8], x[8], o[4];
+                        tmem_ld_32x32b_2x8(d + c0 + i, u0 + i, g, x);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        o[i] = pair16<T>(activate<ACT, true>(f(r[2 * i])).a * f(x[2 * i]),
-                                         activate<ACT, true>(f(r[2 * i + 1])).a * f(x[2 * i + 1]));
-                    store_block<T, 16>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
+                        for (int e = 0; e < 4; ++e)
+                            o[e] = pair16<T>(
+                                activate<ACT, true>(f(g[2 * e])).a * f(x[2 * e]),
+                                activate<ACT, true>(f(g[2 * e + 1])).a * f(x[2 * e + 1]));
+                        *reinterpret_cast<uint4*>(mine16 + i * 2) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                    __syncwarp();
+                    flush_block<T, 32>(c, p.ldc, rows, cols, p.vec_c, turn, kPitch<T>, 16, lane);
                 }
                 if (EPI == kFfSlope) {
-                    uint32_t ou[16], oh[16];
+                    uint8_t* my_g = turn_g + lane * kPitch<float>;
+                    const uint8_t* my_u = turn_u + lane * kPitch<float>;
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     __syncwarp();
+                    // dg to `turn`; du and h take the places of the g they came from
+#pragma unroll 1
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t r[8], o[12];
+                        tmem_ld_32x32b_x8(d + c0 + i, r);
+                        float g[8], x[8];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float4 g4 =
-                            *reinterpret_cast<const float4*>(turn_g + lane * kPitch<float> + i * 8);
-                        const float4 u4 =
-                            *reinterpret_cast<const float4*>(turn_u + lane * kPitch<float> + i * 8);
-                        const float g[4] = {g4.x, g4.y, g4.z, g4.w};
-                        const float x[4] = {u4.x, u4.y, u4.z, u4.w};
-                        float dg[4], du[4], h[4];
+                        for (int e = 0; e < 8; e += 4) {
+                            const float4 g4 = *reinterpret_cast<const float4*>(my_g + (i + e) * 4);
+                            const float4 u4 = *reinterpret_cast<const float4*>(my_u + (i + e) * 4);
+                            g[e] = g4.x, g[e + 1] = g4.y, g[e + 2] = g4.z, g[e + 3] = g4.w;
+                            x[e] = u4.x, x[e + 1] = u4.y, x[e + 2] = u4.z, x[e + 3] = u4.w;
+                        }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const ActValue a = activate<ACT, true>(g[e]);
-                            const float dh = f(r[2 * i + e]);
-                            dg[e] = dh * x[e] * a.slope;
-                            du[e] = dh * a.a;
-                            h[e] = a.a * x[e];
-                        }
+                            float v[3][2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            o[i + e] = pair16<T>(dg[2 * e], dg[2 * e + 1]);
-                            ou[i + e] = pair16<T>(du[2 * e], du[2 * e + 1]);
-                            oh[i + e] = pair16<T>(h[2 * e], h[2 * e + 1]);
+                            for (int q = 0; q < 2; ++q) {
+                                const ActValue a = activate<ACT, true>(g[2 * e + q]);
+                                const float dh = f(r[2 * e + q]), u = x[2 * e + q];
+                                v[0][q] = dh * u * a.slope;
+                                v[1][q] = dh * a.a;
+                                v[2][q] = a.a * u;
+                            }
+#pragma unroll
+                            for (int t = 0; t < 3; ++t) o[4 * t + e] = pair16<T>(v[t][0], v[t][1]);
                         }
+                        *reinterpret_cast<uint4*>(mine16 + i * 2) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(my_g + i * 4) =
+                            make_uint4(o[4], o[5], o[6], o[7]);
+                        *reinterpret_cast<uint4*>(my_g + i * 4 + 16) =
+                            make_uint4(o[8], o[9], o[10], o[11]);
                     }
                     __syncwarp();
-                    if (c0 + 32 < end) fetch(c0 + 32);  // while this block is stored
-                    store_block<T, 16>(c, p.ldc, rows, cols, p.vec_c, o, turn, lane);
-                    store_block<T, 16>(static_cast<T*>(p.c2) + at, p.ldc, rows, cols, p.vec_c, ou, turn,
-                                   lane);
-                    store_block<T, 16>(static_cast<T*>(p.c3) + at, p.ldc, rows, cols, p.vec_c, oh, turn,
-                                   lane);
+#pragma unroll 1
+                    for (int t = 2; t >= 0; --t) {
+                        // the next block's g and u, while dg is stored
+                        if (t == 0) {
+                            __syncwarp();
+                            if (c0 + 32 < end) fetch(c0 + 32);
+                        }
+                        void* to = t == 2 ? p.c3 : t == 1 ? p.c2 : p.c;
+                        flush_block<T, 32>(static_cast<T*>(to) + at, p.ldc, rows, cols, p.vec_c,
+                                           t == 0 ? turn : turn_g + (t - 1) * 16,
+                                           t == 0 ? kPitch<T> : kPitch<float>, t == 0 ? 16 : 32,
+                                           lane);
+                    }
+                    __syncwarp();
                 }
             }
             tc_fence_before();

@@ -13,7 +13,7 @@
 // finishes the rows r with r % cluster size == its rank.
 //
 // Bound by HBM: what counts is bytes in flight, a ring of 64-of-the-sum stages (32 KB
-// of weights for the gated pair, 16 KB for Wd) of about 100 KB per CTA, two CTAs to
+// of weights for the gated pair, 16 KB for Wd) of up to 110 KB per CTA, two CTAs to
 // an SM.  y's kernel is launched while h's still runs (programmatic dependent
 // launch): it fills its ring with Wd, which nobody writes meanwhile, before it waits
 // for h.
@@ -42,6 +42,7 @@ struct alignas(64) RowsArgs {
     float* pre_u;
     int64_t ldc;
     int M, N, nkb, stages;
+    int vec;  // rows of c, pre_g and pre_u: four columns at a time are aligned
     uint32_t* status;
 };
 
@@ -195,6 +196,28 @@ __global__ void __launch_bounds__(kRowsThreads)
             *c = FfElem<T>::put(g);
         }
     };
+    auto finish4 = [&](int row, int col, float4 g, float4 u) {
+        if (args.vec && col + 4 <= args.N) {
+            const float v[4] = {g.x, g.y, g.z, g.w}, w[4] = {u.x, u.y, u.z, u.w};
+            T t[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                t[e] = FfElem<T>::put(GATED ? activate<ACT, true>(v[e]).a * w[e] : v[e]);
+            uint2 q;
+            __builtin_memcpy(&q, t, 8);
+            *reinterpret_cast<uint2*>(static_cast<T*>(args.c) + row * args.ldc + col) = q;
+            if (GATED && args.pre_g) {
+                const int64_t pre = static_cast<int64_t>(row) * args.N + col;
+                *reinterpret_cast<float4*>(args.pre_g + pre) = g;
+                *reinterpret_cast<float4*>(args.pre_u + pre) = u;
+            }
+        } else {
+            finish(row, col, g.x, u.x);
+            finish(row, col + 1, g.y, u.y);
+            finish(row, col + 2, g.z, u.z);
+            finish(row, col + 3, g.w, u.w);
+        }
+    };
     bool ok = true;
     if (warp >= 2) {
         ok = mbar_wait_bounded(&acc_full, 0, args.status, kErrFfEpilogue);
@@ -233,25 +256,35 @@ __global__ void __launch_bounds__(kRowsThreads)
         }
         cluster_sync();
         if (warp >= 2) {
-            // a warp to a row, four columns to a lane; one rank's loads of a row (and
-            // of both products) are in flight together.  After an expired wait the
-            // sums mean nothing, as the status word says, but are in bounds.
+            // A warp to a row, four columns to a lane, the loads of several ranks
+            // and rows in flight together (one from another SM takes about 300 ns).  After an expired wait the sums
+            // mean nothing, as the status word says, but are in bounds.
             const uint32_t at = smem_u32(part) + lane * 16;
-            for (int row = rank + split * (warp - 2); row < args.M; row += split * 4) {
-                float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f), u = g;
+            constexpr int kBatch = ROWS == 16 ? 1 : 2;
+            const int col = n0 + lane * 4, step = split * 4;
+            for (int row = rank + split * (warp - 2); row < args.M; row += kBatch * step) {
+                float4 g[kBatch], u[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) g[i] = u[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
                 for (int p = 0; p < split; ++p) {
-                    const float4 x = ld_cluster_f32x4(at + row * (kColumns * 4), p);
-                    g.x += x.x, g.y += x.y, g.z += x.z, g.w += x.w;
-                    if (GATED) {
-                        const float4 z = ld_cluster_f32x4(at + (ROWS + row) * (kColumns * 4), p);
-                        u.x += z.x, u.y += z.y, u.z += z.z, u.w += z.w;
+                    float4 x[kBatch], z[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        const int r = min(row + i * step, args.M - 1);  // loaded, not stored
+                        x[i] = ld_cluster_f32x4(at + r * (kColumns * 4), p);
+                        if (GATED) z[i] = ld_cluster_f32x4(at + (ROWS + r) * (kColumns * 4), p);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        g[i].x += x[i].x, g[i].y += x[i].y, g[i].z += x[i].z, g[i].w += x[i].w;
+                        if (GATED)
+                            u[i].x += z[i].x, u[i].y += z[i].y, u[i].z += z[i].z, u[i].w += z[i].w;
                     }
                 }
-                finish(row, n0 + lane * 4, g.x, u.x);
-                finish(row, n0 + lane * 4 + 1, g.y, u.y);
-                finish(row, n0 + lane * 4 + 2, g.z, u.z);
-                finish(row, n0 + lane * 4 + 3, g.w, u.w);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    if (row + i * step < args.M) finish4(row + i * step, col, g[i], u[i]);
             }
         }
         cluster_sync();  // nobody leaves while its memory is read
@@ -275,22 +308,26 @@ int rows_sms() {
 template <bool GATED, int ACT, class T, int ROWS>
 int launch_rows(RowsArgs& args, cudaStream_t s) {
     constexpr int kStage = (GATED ? 2 : 1) * kWeightBytes + ROWS * 128;
-    constexpr int kRing = 104 * 1024;  // two CTAs to an SM
     constexpr int kPart = (GATED ? 2 : 1) * ROWS * kColumns * 4;
-    const int tiles = (args.N + kColumns - 1) / kColumns;
+    const int tiles = (args.N + kColumns - 1) / kColumns, sms = rows_sms();
     int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * rows_sms() && 2 * split <= args.nkb) split *= 2;
+    while (split < 8 && 2 * split * tiles <= 2 * sms && 2 * split <= args.nkb) split *= 2;
     const int per = (args.nkb + split - 1) / split;
-    args.stages = std::min(std::min(std::max(kRing / kStage, 2), kRowsMaxStages), per);
-    // at least half an SM's shared memory each, so that no third CTA waits for TMEM
-    const int smem = std::max(std::max(args.stages * kStage, split > 1 ? kPart : 0), kRing) + 1024;
+    // two CTAs to an SM, or with fewer CTAs than SMs one that holds more of its weights
+    // before h arrives
+    const int ring = (!GATED && split * tiles <= sms ? 200 : 110) * 1024;
+    args.stages = std::min(std::min(std::max(ring / kStage, 2), kRowsMaxStages), per);
+    // TMEM holds four CTAs (128 columns at most), which 56 KB of shared memory each ensure;
+    // with 64 rows' short rings (two stages) a third CTA took 2 us more than two
+    constexpr int kLeast = (ROWS > 32 ? 104 : 56) * 1024;
+    const int smem = std::max({args.stages * kStage, split > 1 ? kPart : 0, kLeast}) + 1024;
     auto kernel = ff_rows_kernel<GATED, ACT, T, ROWS>;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
     if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 202 * 1024);
         if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     }
     if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
@@ -333,6 +370,8 @@ int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& f, cudaStream_
     RowsArgs args;
     std::memset(&args, 0, sizeof(args));
     args.c = f.c, args.ldc = f.ldc, args.pre_g = f.pre_g, args.pre_u = f.pre_u;
+    args.vec = f.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(f.c) & 7) == 0 &&
+               (!f.pre_g || f.N % 4 == 0);
     args.M = f.M, args.N = f.N, args.nkb = (f.k[0] + kSumStep - 1) / kSumStep;
     const int rows = f.M <= 16 ? 16 : f.M <= 32 ? 32 : 64;
     int rc = status_word(&args.status);

@@ -273,6 +273,17 @@ def _ff_sizes(x: torch.Tensor, w_gate: torch.Tensor, w_down: torch.Tensor) -> tu
     return sizes
 
 
+def _ff_ready(index: int, dtype: torch.dtype, pairs) -> bool:
+    """Whether each (tensor, shape) is as the kernels take it, on the current device."""
+    if index != torch._C._cuda_getDevice():
+        return False
+    for t, shape in pairs:
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != index or \
+                not t.is_contiguous() or t.data_ptr() & 15:
+            return False
+    return True
+
+
 @functools.lru_cache(maxsize=1024)
 def _ff_workspace_bytes(dtype: int, mode: int, m: int, k: int, f: int, d: int,
                         backward: int) -> int:
@@ -288,23 +299,30 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: 
     returns (y, saved), `saved` being what gated_ff_backward needs: the two inner
     products before the activation, f32 [m, f] each."""
     m, k, f, d = _ff_sizes(x, w_gate, w_down)
-    index, act, mode = x.get_device(), int(act), int(mode)
-    with _on(index):
-        x = _ff_operand("x", x, (m, k), x)
-        w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
-        w_up = _ff_operand("w_up", w_up, (k, f), x)
-        w_down = _ff_operand("w_down", w_down, (f, d), x)
-        y = _ff_output("out", out, (m, d), x)
-        saved = (x.new_empty((m, f), dtype=torch.float32),
-                 x.new_empty((m, f), dtype=torch.float32)) if save else None
-        dt, stream = _FLOATS[x.dtype].value, _raw_stream(index)
-        need = _ff_workspace_bytes(dt, mode, m, k, f, d, 0)
-        ws = _scratch(index, stream, need)
-        check(L.load().zg_gated_ff(
-            dt, mode, act, m, k, f, d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-            w_down.data_ptr(), y.data_ptr(), saved[0].data_ptr() if save else None,
-            saved[1].data_ptr() if save else None, ws.data_ptr() if ws is not None else None, need,
-            stream))
+    index = x.get_device()
+    if not _ff_ready(index, x.dtype, ((x, (m, k)), (w_gate, (k, f)), (w_up, (k, f)),
+                                      (w_down, (f, d)))):
+        with _on(index):
+            x = _ff_operand("x", x, (m, k), x)
+            w_gate = _ff_operand("w_gate", w_gate, (k, f), x)
+            w_up = _ff_operand("w_up", w_up, (k, f), x)
+            w_down = _ff_operand("w_down", w_down, (f, d), x)
+            return _gated_ff(index, m, k, f, d, x, w_gate, w_up, w_down, act, mode, save, out)
+    return _gated_ff(index, m, k, f, d, x, w_gate, w_up, w_down, act, mode, save, out)
+
+
+def _gated_ff(index, m, k, f, d, x, w_gate, w_up, w_down, act, mode, save, out):
+    y = _ff_output("out", out, (m, d), x)
+    saved = (x.new_empty((m, f), dtype=torch.float32),
+             x.new_empty((m, f), dtype=torch.float32)) if save else None
+    dt, stream, mode = _FLOATS[x.dtype].value, _raw_stream(index), int(mode)
+    need = _ff_workspace_bytes(dt, mode, m, k, f, d, 0)
+    ws = _scratch(index, stream, need)
+    check(L.load().zg_gated_ff(
+        dt, mode, int(act), m, k, f, d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+        w_down.data_ptr(), y.data_ptr(), saved[0].data_ptr() if save else None,
+        saved[1].data_ptr() if save else None, ws.data_ptr() if ws is not None else None, need,
+        stream))
     return (y, saved) if save else y
 
 

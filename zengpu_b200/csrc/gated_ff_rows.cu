@@ -16,7 +16,8 @@
 // of weights for the gated pair, 16 KB for Wd) of up to 110 KB per CTA, two CTAs to
 // an SM.  y's kernel is launched while h's still runs (programmatic dependent
 // launch): it fills its ring with Wd, which nobody writes meanwhile, before it waits
-// for h.
+// for h.  One bf16 token, 4096 -> 12288: 53 us for 302 MB (5.7 TB/s); 48 f16 tokens 63
+// us, of which the cluster's exchange of 48 rows takes about 4 twice.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>

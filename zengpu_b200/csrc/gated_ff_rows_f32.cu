@@ -15,7 +15,9 @@
 //
 // Up to 16 rows the weights' 4 bytes each bound it; beyond, the f32 pipe (8 rows a
 // weight take 16 cycles of an SM's 128 lanes for 1 KB of weights, which HBM delivers
-// in 44).
+// in 44).  One token, 4096 -> 12288: 128 us for 604 MB (4.7 TB/s); 32 tokens 439 us.
+// From 33 rows on the tensor cores are faster (2048 -> 6144: 217 us at 33 rows, 64 rows
+// here took 230).
 #include <algorithm>
 #include <atomic>
 #include <cstdint>

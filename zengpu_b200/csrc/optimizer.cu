@@ -251,10 +251,10 @@ __device__ __forceinline__ float block_scale(float top, float& inv) {
     return top < INFINITY ? s : __int_as_float(0x7fc00000);
 }
 
+// The largest over a warp of values that are not negative, or NaN: the order of their
+// bits, with NaN last.
 __device__ __forceinline__ float warp_top(float top) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    return top;
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
 }
 
 // Eight m of a block as codes, and the block's scale.

@@ -327,10 +327,11 @@ __device__ __forceinline__ float encode_root(const F2 (&v)[4], const F2 (&r)[4],
 
 // What bounds it: HBM.  f32 weights, gradients and moments move 28 bytes per
 // element, 16-bit weights with a master and 8-bit moments 16.1; the latter are
-// as near to the issue rate: roots and quotients are then the approximate
+// near the issue rate too: roots and quotients are then the approximate
 // instructions (a quotient is within 2 units of its last place, on a change of the
-// weight that is small beside it; the roots' codes are exact, see encode_root).  277 M
-// elements: 1.147 ms (6.8 TB/s) and 0.85 ms (5.2 TB/s).
+// weight that is small beside it; the roots' codes are exact, see encode_root), and
+// what a whole call decides (exact roots, a master) branches once a block, not once
+// a pair (795 -> 713 us).  277 M elements: 1.144 ms (6.8 TB/s) and 0.713 ms (6.2 TB/s).
 template <class P, class G, int BITS, int CAP>
 __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
     adamw_kernel(const __grid_constant__ Table<CAP, zg_adamw_tensor> tab, int64_t chunk, Factors f,
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
           reinterpret_cast<uintptr_t>(t.exp_avg_sq)) & 15) == 0;
 
     // Whole blocks of aligned tensors come through shared memory: the next one (with 8-bit
-    // moments the next two, 806 us for 277 M elements against 831) is on its way while
+    // moments the next two, 795 us for 277 M elements against 831) is on its way while
     // this one is worked on, at no cost in registers.
     constexpr int kMoment = BITS == 32 ? 4 : 1;
     constexpr int kG = kBlockElems * sizeof(G), kW = kBlockElems * 4, kM = kBlockElems * kMoment;
@@ -415,8 +416,13 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
         auto take = [&](bool v, const G* gb, const float* wb, const P* pb, const uint8_t* mb,
                         const uint8_t* vb) {
             load8<G>(gb, v, lane, left, gv);
-            if (master) load8<float>(wb, v, lane, left, wv);
-            else load8<P>(pb, v, lane, left, pv);
+            if (master) {
+                load8<float>(wb, v, lane, left, wv);
+            } else {
+                load8<P>(pb, v, lane, left, pv);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) wv[e] = Elem<P>::get(pv[e]);
+            }
             if (BITS == 32) {
                 load8<float>(reinterpret_cast<const float*>(mb), v, lane, left, mv);
                 load8<float>(reinterpret_cast<const float*>(vb), v, lane, left, vv);
@@ -453,15 +459,24 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
             m[e] = add2(mul2(m[e], both(f.b1)), mul2(ge, both(f.c1)), both(f.one));
             v[e] = add2(mul2(v[e], both(f.b2)), mul2(mul2(ge, both(f.c2)), ge), both(f.one));
             const float2 v2 = unpack(v[e]);
-            r[e] = BITS == 32 || exact_roots ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
+            r[e] = BITS == 32 ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
                               : pack(sqrt_approx(v2.x), sqrt_approx(v2.y));
+        }
+        if (BITS == 8 && exact_roots) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 v2 = unpack(v[e]);
+                r[e] = pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
             const float2 den = unpack(add2(mul2(r[e], both(f.root)), both(f.eps), both(f.one)));
             const float2 num = unpack(mul2(m[e], both(-f.step_size)));
             const F2 quot = BITS == 32
                                 ? pack(__fdiv_rn(num.x, den.x), __fdiv_rn(num.y, den.y))
                                 : pack(num.x * rcp_approx(den.x), num.y * rcp_approx(den.y));
-            w[e] = add2(mul2(master ? widen(wv, e) : widen(pv, e), both(f.decay)), quot,
-                        both(f.one));
+            w[e] = add2(mul2(widen(wv, e), both(f.decay)), quot, both(f.one));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -258,8 +258,9 @@ __global__ void __launch_bounds__(kRowsThreads)
         cluster_sync();
         if (warp >= 2) {
             // A warp to a row, four columns to a lane, the loads of several ranks
-            // and rows in flight together (one from another SM takes about 300 ns).  After an expired wait the sums
-            // mean nothing, as the status word says, but are in bounds.
+            // and rows in flight together (one from another SM takes about 300 ns).
+            // After an expired wait the sums mean nothing, as the status word says, but
+            // are in bounds.
             const uint32_t at = smem_u32(part) + lane * 16;
             constexpr int kBatch = ROWS == 16 ? 1 : 2;
             const int col = n0 + lane * 4, step = split * 4;

@@ -43,9 +43,10 @@ struct RowsF32Args {
     int vec_w, vec_x;  // 16-byte aligned rows
 };
 
-__device__ __forceinline__ void copy16(uint32_t to, const float* from, bool in) {
+// Copies the first `count` of four floats, zeros after them.
+__device__ __forceinline__ void copy16(uint32_t to, const float* from, int count) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from),
-                 "r"(in ? 16 : 0)
+                 "r"(4 * count)
                  : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool in) {
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
                         const int c = threadIdx.x % (kRCols / 4) * 4;
                         const bool in = k0 + k < a.K && n0 + c < a.N;
                         copy16(to + (k * kRCols + c) * 4,
-                               in ? from + (k0 + k) * a.ldw + n0 + c : from, in);
+                               in ? from + (k0 + k) * a.ldw + n0 + c : from, in ? 4 : 0);
                     }
                 } else {
 #pragma unroll 4
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(kRThreads, 2)
             if (a.vec_x) {
                 for (int j = threadIdx.x; j < ROWS * (kRStep / 4); j += kRThreads) {
                     const int r = j / (kRStep / 4), k = j % (kRStep / 4) * 4;
-                    const bool in = k0 + k < a.K && r < a.M;
+                    // a row of h goes on past the sum, with what scratch memory held
+                    const int in = r < a.M ? max(min(a.K - (k0 + k), 4), 0) : 0;
                     copy16(to + (r * kXPitch + k) * 4, in ? a.x + r * a.ldx + k0 + k : a.x, in);
                 }
             } else {

@@ -271,8 +271,8 @@ __device__ __forceinline__ float encode_m(const F2 (&m)[4], uint32_t (&codes)[2]
     return s;
 }
 
-// Both flush subnormals: a v below 2^-126 gives root 0 (see kTinyEps), and a
-// denominator, at least 2^-75 or zero, is none.
+// Both flush subnormals: a v below 2^-126 gives root 0, and a denominator below 2^-126
+// an infinite reciprocal.  With an eps that this matters to (kTinyEps) neither is called.
 __device__ __forceinline__ float sqrt_approx(float x) {
     float r;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -283,8 +283,11 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// With eps this small the root of a subnormal v counts: exact roots then.
-constexpr float kTinyEps = 1e-12f;
+// Times 1 / sqrt(1 - b2), the most that a root is scaled up by (at step 1): with an eps
+// below that the root of a subnormal v, up to 2^-63 = 1.1e-19 before the scaling, may count
+// for 2^-23 of the denominator or more, and where v is zero eps is all of it, subnormal or
+// not.  Roots and quotients are exact then.
+constexpr double kTinyEps = 1e-12;
 
 // Eight roots of a block as codes, from v and r, the roots to within three units of
 // the last place (sqrt.approx: one or two): codes are those of the correctly rounded
@@ -330,9 +333,10 @@ __device__ __forceinline__ float encode_root(const F2 (&v)[4], const F2 (&r)[4],
 // near the issue rate too: roots and quotients are then the approximate
 // instructions (a quotient is within 2 units of its last place, on a change of the
 // weight that is small beside it; the roots' codes are exact, see encode_root), and
-// what a whole call decides (exact roots, a master) branches once a block, not once
-// a pair (795 -> 713 us).  277 M elements: 1.144 ms (6.8 TB/s) and 0.713 ms (6.2 TB/s).
-template <class P, class G, int BITS, int CAP>
+// what a whole call decides is not asked for each pair (exact roots: another kernel; a
+// master: a branch a block; 795 -> 713 us).  277 M elements: 1.144 ms (6.8 TB/s) and 0.713 ms (6.2 TB/s).
+// EXACT: correctly rounded roots and quotients in the weight's change; always with 32 bits.
+template <class P, class G, int BITS, bool EXACT, int CAP>
 __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
     adamw_kernel(const __grid_constant__ Table<CAP, zg_adamw_tensor> tab, int64_t chunk, Factors f,
                  const zg_adamw_hyper hyper, const DeviceHyper dev) {
@@ -395,7 +399,6 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
-    const bool exact_roots = f.eps < kTinyEps;
     int64_t b = begin + warp * kBlockElems;
     int place = 0;
     ask(b, 0);
@@ -459,23 +462,15 @@ __global__ void __launch_bounds__(kOptThreads, BITS == 8 ? 3 : 2)
             m[e] = add2(mul2(m[e], both(f.b1)), mul2(ge, both(f.c1)), both(f.one));
             v[e] = add2(mul2(v[e], both(f.b2)), mul2(mul2(ge, both(f.c2)), ge), both(f.one));
             const float2 v2 = unpack(v[e]);
-            r[e] = BITS == 32 ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
-                              : pack(sqrt_approx(v2.x), sqrt_approx(v2.y));
-        }
-        if (BITS == 8 && exact_roots) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 v2 = unpack(v[e]);
-                r[e] = pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y));
-            }
+            r[e] = EXACT ? pack(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y))
+                         : pack(sqrt_approx(v2.x), sqrt_approx(v2.y));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 den = unpack(add2(mul2(r[e], both(f.root)), both(f.eps), both(f.one)));
             const float2 num = unpack(mul2(m[e], both(-f.step_size)));
-            const F2 quot = BITS == 32
-                                ? pack(__fdiv_rn(num.x, den.x), __fdiv_rn(num.y, den.y))
-                                : pack(num.x * rcp_approx(den.x), num.y * rcp_approx(den.y));
+            const F2 quot = EXACT ? pack(__fdiv_rn(num.x, den.x), __fdiv_rn(num.y, den.y))
+                                  : pack(num.x * rcp_approx(den.x), num.y * rcp_approx(den.y));
             w[e] = add2(mul2(widen(wv, e), both(f.decay)), quot, both(f.one));
         }
 #pragma unroll
@@ -653,6 +648,7 @@ void fill(Table<CAP, Tensor>& tab, const Tensor* t, int count, int64_t chunk) {
 }
 
 struct AdamCall {
+    bool exact;
     Factors f;
     zg_adamw_hyper hyper;
     DeviceHyper dev;
@@ -660,23 +656,23 @@ struct AdamCall {
     cudaStream_t stream;
 };
 
-template <class P, class G, int BITS, int CAP>
+template <class P, class G, int BITS, bool EXACT, int CAP>
 int launch_adamw_table(const zg_adamw_tensor* t, int count, const AdamCall& c) {
     static_assert(sizeof(Table<CAP, zg_adamw_tensor>) + 256 <= 32764, "kernel parameters");
     Table<CAP, zg_adamw_tensor> tab;
     fill(tab, t, count, c.chunk);
-    adamw_kernel<P, G, BITS, CAP><<<tab.first[count], kOptThreads, 0, c.stream>>>(
+    adamw_kernel<P, G, BITS, EXACT, CAP><<<tab.first[count], kOptThreads, 0, c.stream>>>(
         tab, c.chunk, c.f, c.hyper, c.dev);
     return cuda_status(cudaGetLastError(), "zg_adamw");
 }
 
-template <class P, class G, int BITS>
+template <class P, class G, int BITS, bool EXACT>
 int launch_adamw(const std::vector<zg_adamw_tensor>& t, const AdamCall& c) {
     for (size_t at = 0; at < t.size(); at += kLargeTable) {
         const int n = static_cast<int>(std::min<size_t>(t.size() - at, kLargeTable));
         const int rc = n <= kSmallTable
-                           ? launch_adamw_table<P, G, BITS, kSmallTable>(t.data() + at, n, c)
-                           : launch_adamw_table<P, G, BITS, kLargeTable>(t.data() + at, n, c);
+                           ? launch_adamw_table<P, G, BITS, EXACT, kSmallTable>(t.data() + at, n, c)
+                           : launch_adamw_table<P, G, BITS, EXACT, kLargeTable>(t.data() + at, n, c);
         if (rc) return rc;
     }
     return ZG_OK;
@@ -684,7 +680,8 @@ int launch_adamw(const std::vector<zg_adamw_tensor>& t, const AdamCall& c) {
 
 template <class P, class G>
 int launch_adamw_bits(int bits, const std::vector<zg_adamw_tensor>& t, const AdamCall& c) {
-    return bits == 8 ? launch_adamw<P, G, 8>(t, c) : launch_adamw<P, G, 32>(t, c);
+    if (bits == 32) return launch_adamw<P, G, 32, true>(t, c);
+    return c.exact ? launch_adamw<P, G, 8, true>(t, c) : launch_adamw<P, G, 8, false>(t, c);
 }
 
 template <class P>
@@ -793,10 +790,12 @@ extern "C" int zg_adamw(uint32_t param_dtype, uint32_t grad_dtype, int state_bit
     c.f.c1 = static_cast<float>(1.0 - h->beta1);
     c.f.b2 = static_cast<float>(h->beta2);
     c.f.c2 = static_cast<float>(1.0 - h->beta2);
-    c.f.eps = static_cast<float>(h->eps);
+    // an eps above zero stays above zero, so that 0 / (0 + eps) is 0
+    c.f.eps = h->eps > 0.0 ? std::max(static_cast<float>(h->eps), 0x1p-149f) : 0.0f;
     c.f.one = 1.0f;
     schedule(c.f, lr_dev ? 0.0 : h->lr, h->beta1, h->beta2, h->weight_decay,
              step_dev ? 1.0 : static_cast<double>(h->step));
+    c.exact = h->eps < kTinyEps / sqrt(1.0 - h->beta2);
     c.chunk = chunk_elems(total);
     c.stream = static_cast<cudaStream_t>(stream);
     switch (param_dtype) {

@@ -1,0 +1,120 @@
+"""Sums of the gated block past 16384 terms on 16-bit tensors.
+
+The tensor core's f32 additions cut off what does not fit, always toward zero.  What that
+takes from a sum of n terms of one sign grows with n unless the runs are bounded: 6.4e-9 n
+of the result, as sums left in the tensor core measured it (1.9e-3 at n = 300007, 8.3e-4
+at 131080).  Runs of at most 2^14 terms, added up by rounded additions (2^-24 each, of
+either sign), lose 1.05e-4 of it, less than 2^-13 = 1.22e-4.
+
+All inputs here are positive, so that every sum is of one sign and the loss is its
+largest.  It is measured as the mean of the signed relative error over many results, in
+which the roundings to the type (symmetric, at most half a step each) average out: their
+rms is eps / 2 / sqrt(3) for each result, so 2^-15 covers four deviations of the mean
+over 2000 results and more in f16, over 2^17 in bf16."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from zengpu_b200 import Activation, kernels as K
+
+pytestmark = pytest.mark.gpu
+
+BAR = 2.0 ** -13 + 2.0 ** -15
+ACT = Activation.RELU  # the identity on positive numbers, with slope 1
+
+
+def positive(gen, kind, scale, *shape):
+    """Values from half to one and a half times `scale`, each column of another size (once
+    to twice that), so that results lie anywhere between two steps of the type."""
+    t = torch.rand(*shape, generator=gen, device="cuda").add_(0.5).mul_(scale)
+    return t.mul_(1 + torch.rand(1, shape[1], generator=gen, device="cuda")).to(kind)
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def bias(got, want):
+    assert torch.isfinite(got).all()
+    return abs(float((got.double() / want - 1).mean()))
+
+
+def backward(x, wg, wu, wd, dy):
+    y, saved = K.gated_ff(x, wg, wu, wd, act=ACT, save=True)
+    return y, saved, K.gated_ff_backward(dy, x, wg, wu, wd, saved, act=ACT)
+
+
+@pytest.mark.parametrize("m,k", [(300_007, 1024), (600_001, 72)], ids=["one_part", "parts"])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_weight_gradients_of_many_rows(m, k, kind):
+    """dWg, dWu and dWd sum over the rows: in one part each (large layers), and in
+    several (small ones)."""
+    f, d = k, k
+    g = gen()
+    x, dy = positive(g, kind, 1.0, m, k), positive(g, kind, 1e-3, m, d)
+    wg, wu = positive(g, kind, 1.0 / k, k, f), positive(g, kind, 1.0 / k, k, f)
+    wd = positive(g, kind, 1.0 / d, f, d)
+    _, _, (dx, dwg, dwu, dwd) = backward(x, wg, wu, wd, dy)
+    cols = torch.arange(0, f, max(f // 32, 1), device="cuda")
+    want_g = torch.zeros(k, len(cols), dtype=torch.float64, device="cuda")
+    want_u, want_d = want_g.clone(), torch.zeros(len(cols), d, dtype=torch.float64, device="cuda")
+    wg64, wu64, wd64 = wg[:, cols].double(), wu[:, cols].double(), wd[cols].double()
+    for a in range(0, m, 50_000):
+        x64, dy64 = x[a:a + 50_000].double(), dy[a:a + 50_000].double()
+        gate, up, dh = x64 @ wg64, x64 @ wu64, dy64 @ wd64.t()
+        want_g += x64.t() @ (dh * up)
+        want_u += x64.t() @ (dh * gate)
+        want_d += (gate * up).t() @ dy64
+    bar = BAR if kind == torch.float16 or k > 500 else BAR + 2.0 ** -13
+    assert bias(dwg[:, cols], want_g) <= bar
+    assert bias(dwu[:, cols], want_u) <= bar
+    assert bias(dwd[cols], want_d) <= bar
+    assert K.kernel_status() == 0
+
+
+@pytest.mark.parametrize("m", [16, 130])
+def test_products_of_long_rows(m):
+    """x w_gate and x w_up over a long k, kept in f32."""
+    kind, k, f, d = torch.float16, 300_008, 256, 64
+    g = gen(1)
+    x = positive(g, kind, 3e-3, m, k)
+    wg, wu = positive(g, kind, 1e-3, k, f), positive(g, kind, 1e-3, k, f)
+    wd = positive(g, kind, 1.0 / f, f, d)
+    y, (pre_g, pre_u) = K.gated_ff(x, wg, wu, wd, act=ACT, save=True)
+    x64 = x.double()
+    gate, up = x64 @ wg.double(), x64 @ wu.double()
+    assert bias(pre_g, gate) <= BAR and bias(pre_u, up) <= BAR
+    assert bias(y, (gate * up) @ wd.double()) <= 2 * BAR + 2.0 ** -14  # both enter h
+    assert torch.equal(y, K.gated_ff(x, wg, wu, wd, act=ACT))
+    assert K.kernel_status() == 0
+
+
+def test_gradients_through_long_rows():
+    """dh = dy w_down^T over a long d."""
+    kind, m, k, f, d = torch.float16, 130, 64, 256, 300_008
+    g = gen(2)
+    x, dy = positive(g, kind, 1.0, m, k), positive(g, kind, 3e-3, m, d)
+    wg, wu = positive(g, kind, 1.0 / k, k, f), positive(g, kind, 1.0 / k, k, f)
+    wd = positive(g, kind, 1e-3, f, d)
+    _, _, (dx, dwg, dwu, _) = backward(x, wg, wu, wd, dy)
+    x64 = x.double()
+    gate, up, dh = x64 @ wg.double(), x64 @ wu.double(), dy.double() @ wd.double().t()
+    assert bias(dwg, x64.t() @ (dh * up)) <= BAR + 2.0 ** -15
+    assert bias(dwu, x64.t() @ (dh * gate)) <= BAR + 2.0 ** -15
+    assert bias(dx, (dh * up) @ wg.double().t() + (dh * gate) @ wu.double().t()) <= BAR + 2.0 ** -15
+    assert K.kernel_status() == 0
+
+
+@pytest.mark.parametrize("f", [100_000, 131_080])
+def test_few_rows_with_many_hidden_units(f):
+    """y of a few rows, where so many columns share the SMs that a sum is hardly split."""
+    kind, m, k, d = torch.float16, 4, 8, 19_072
+    g = gen(3)
+    x, wd = positive(g, kind, 1.0, m, k), positive(g, kind, 1e-3, f, d)
+    wg, wu = positive(g, kind, 0.1 / k, k, f), positive(g, kind, 0.1 / k, k, f)
+    y = K.gated_ff(x, wg, wu, wd, act=ACT)
+    h = (x.double() @ wg.double()) * (x.double() @ wu.double())
+    want = sum(h[:, a:a + 8192] @ wd[a:a + 8192].double() for a in range(0, f, 8192))
+    assert bias(y, want) <= BAR
+    assert K.kernel_status() == 0

@@ -247,9 +247,10 @@ int place_inputs(const FfCall& c, const FfLayout& l, uint8_t* ws, const void* co
 }
 
 // The forward pass of few rows (gated_ff_rows.cu, gated_ff_rows_f32.cu), whose grids
-// take 65535 tiles of 128 columns.
+// take 65535 tiles of 128 columns, and whose 16-bit sums eight runs.
 bool few_rows(const FfCall& c) {
-    return c.m <= (c.size == 2 ? kFfRows : kFfRowsF32) && std::max(c.f, c.d) <= 65535 * 128;
+    return c.m <= (c.size == 2 ? kFfRows : kFfRowsF32) && std::max(c.f, c.d) <= 65535 * 128 &&
+           (c.size == 4 || std::max(c.k, c.f) <= 8 * kFfRun);
 }
 bool f32_tensor(const FfCall& c) { return c.size == 4 && c.mode != ZG_GEMM_SIMT_FP32; }
 

@@ -18,6 +18,12 @@
 
 namespace zg {
 
+// Terms of a sum that 16-bit MMAs may add up in TMEM.  The tensor core's f32 additions
+// truncate, always toward zero: a sum of n terms of one sign lost 6.4e-9 n of itself
+// (n = 300007: 1.9e-3, half a bf16 step), so a run of these 1.05e-4, a fifth of half an f16
+// step.  Longer sums are added up from runs by rounded additions.
+constexpr int kFfRun = 16384;
+
 template <class T> struct FfElem;
 template <> struct FfElem<float> {
     __device__ static float get(float x) { return x; }

@@ -313,7 +313,10 @@ int launch_rows(RowsArgs& args, cudaStream_t s) {
     constexpr int kPart = (GATED ? 2 : 1) * ROWS * kColumns * 4;
     const int tiles = (args.N + kColumns - 1) / kColumns, sms = rows_sms();
     int split = 1;
-    while (split < 8 && 2 * split * tiles <= 2 * sms && 2 * split <= args.nkb) split *= 2;
+    // as many CTAs as two to an SM, and more where a CTA's part were longer than a run may be
+    while (split < 8 && 2 * split <= args.nkb &&
+           (2 * split * tiles <= 2 * sms || args.nkb > split * (kFfRun / kSumStep)))
+        split *= 2;
     const int per = (args.nkb + split - 1) / split;
     // two CTAs to an SM, or with fewer CTAs than SMs one that holds more of its weights
     // before h arrives

@@ -24,10 +24,12 @@
 // one launch.
 //
 // Roles as in the f32 kernels (sgemm_tc.cu): warp 0 TMA, warp 1 MMA (CTA 0 of the
-// pair issues), warps 2-9 epilogue.  The f32 accumulator stays in TMEM over the
-// whole sum: its additions truncate, about n / 16 2^-24 of the result for n terms,
-// which at n = 12288 is 5e-5, a tenth of half an f16 step.  Two accumulators: a
-// tile's epilogue overlaps the next tile's MMAs.  When the last wave would keep
+// pair issues), warps 2-9 epilogue.  The f32 accumulator stays in TMEM for up to kFfRun
+// of the sum: its additions truncate, which takes 1.1e-4 from a sum of that many terms of
+// one sign (gated_ff.cuh).  A longer sum comes in runs, which the epilogue warps add up,
+// rounding to nearest, while the MMAs fill the other accumulator (LONG: 128 values a
+// lane, in local memory; a run takes 70 us and more, its drain a few).  Two
+// accumulators: a tile's epilogue overlaps the next tile's MMAs.  When the last wave would keep
 // at most half of the pairs busy its tiles run as two column halves.  Products of
 // few tiles and a long sum are split along it into f32 parts, which a second kernel
 // adds up in order.  Each kernel is launched while the one before it drains
@@ -51,6 +53,7 @@ namespace {
 
 constexpr int kThreads = 320, kEpiWarps = 8;
 constexpr int kBK = 64, kBox = 64;             // of the sum per stage; rows per box
+constexpr int kRun = kFfRun / kBK;             // stages in a run
 constexpr int kBoxBytes = kBox * 128;          // 8 KB
 constexpr int kOperandBytes = 2 * kBoxBytes;   // 128 rows
 constexpr int kStageBytes = 2 * kOperandBytes; // A and B: 32 KB per CTA
@@ -181,7 +184,8 @@ __device__ __forceinline__ void fetch_block(const float* src, int64_t ld, int ro
     }
 }
 
-template <int EPI, int ACT, class T>
+// LONG: a unit's sum may take several runs.
+template <int EPI, int ACT, class T, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ff_pair_kernel(const __grid_constant__ PairArgs args) {
     constexpr int kStages = kStageCount[EPI];
@@ -261,36 +265,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // ---------------- MMA issuer (CTA 0) ----------------
         if (leader && lane == 0) {
             bool ok = true;
-            int it = 0;
-            for (int n = 0, u; ok && (u = unit_at(args.deal, pair, n)) >= 0; ++n) {
+            int it = 0, n = 0;  // stages and runs so far
+            for (int j = 0, u; ok && (u = unit_at(args.deal, pair, j)) >= 0; ++j) {
                 const Unit w = unit_of<EPI>(args, u);
                 const PairProblem& p = *w.p;
-                const int buf = n & 1;
-                const uint32_t d_tmem = tmem_base + buf * 256;
-                if (n >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((n >> 1) - 1) & 1, args.status,
-                                                 kErrFfMma)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
                 const uint32_t idesc = instr_desc<T>(w.width, p.a_mn, p.b_mn);
                 const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-                    const int s = it % kStages;
-                    if (!mbar_wait_bounded(&full[s], (it / kStages) & 1, args.status, kErrFfMma)) {
+                for (int k0 = w.kb0; k0 < w.kb1 && ok; k0 += kRun, ++n) {
+                    const int buf = n & 1;
+                    const uint32_t d_tmem = tmem_base + buf * 256;
+                    if (n >= 2 && !mbar_wait_bounded(&acc_empty[buf], ((n >> 1) - 1) & 1,
+                                                     args.status, kErrFfMma)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * kStageBytes), b = a + kOperandBytes;
+                    const int k1 = LONG ? min(w.kb1, k0 + kRun) : w.kb1;
+                    for (int kb = k0; kb < k1; ++kb, ++it) {
+                        const int s = it % kStages;
+                        if (!mbar_wait_bounded(&full[s], (it / kStages) & 1, args.status,
+                                               kErrFfMma)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a = smem_u32(smem + s * kStageBytes), b = a + kOperandBytes;
 #pragma unroll
-                    for (int i = 0; i < kBK / 16; ++i)
-                        mma_f16_ss_pair(d_tmem, smem_desc(a + i * a_step, kBoxBytes),
-                                        smem_desc(b + i * b_step, kBoxBytes), idesc,
-                                        kb != w.kb0 || i != 0);
-                    mma_commit_pair(&empty[s], 0x3);
+                        for (int i = 0; i < kBK / 16; ++i)
+                            mma_f16_ss_pair(d_tmem, smem_desc(a + i * a_step, kBoxBytes),
+                                            smem_desc(b + i * b_step, kBoxBytes), idesc,
+                                            kb != k0 || i != 0);
+                        mma_commit_pair(&empty[s], 0x3);
+                    }
+                    if (ok) mma_commit_pair(&acc_full[buf], 0x3);
+                    if (!LONG) break;
                 }
-                if (ok) mma_commit_pair(&acc_full[buf], 0x3);
+                if (!LONG) ++n;
             }
             if (!ok) {
                 mma_commit_pair(drain, 0x1);
@@ -305,7 +315,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t leader_empty1 = mapa_shared(&acc_empty[1], 0);
         uint8_t* turn = turns + (warp - 2) * kTurnBytes[EPI];
         uint8_t *turn_g = turn + kBlock16, *turn_u = turn_g + kBlock32;  // dh's epilogue
-        for (int n = 0, u; (u = unit_at(args.deal, pair, n)) >= 0; ++n) {
+        // what the runs before a sum's last one came to: D's columns of this warp, Wu's
+        // from 64 on in the gated form
+        float held[LONG ? 128 : 1];
+        int n = 0;
+        for (int j = 0, u; (u = unit_at(args.deal, pair, j)) >= 0; ++j, ++n) {
             const Unit w = unit_of<EPI>(args, u);
             const PairProblem& p = *w.p;
             const int64_t row0 = w.m0 + 128 * static_cast<int>(rank) + q * 32;
@@ -321,6 +335,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fetch_block(p.pre_u + pre, p.N, rows, cols, p.vec_pre, turn_u, lane);
             };
             if (EPI == kFfSlope) fetch(begin);  // on its way while the sums finish
+            const bool many = LONG && w.kb1 - w.kb0 > kRun;
+            auto add_held = [&](auto& r, int at) {
+                if (many) {
+#pragma unroll
+                    for (int e = 0; e < static_cast<int>(sizeof(r) / sizeof(r[0])); ++e)
+                        r[e] = __float_as_uint(held[at + e] + __uint_as_float(r[e]));
+                }
+            };
+            bool lost = false;
+            for (int k0 = w.kb0; many && k0 + kRun < w.kb1; k0 += kRun, ++n) {
+                const bool here = mbar_wait_bounded(&acc_full[n & 1], (n >> 1) & 1, args.status,
+                                                    kErrFfEpilogue);
+                if ((lost = !__all_sync(0xffffffffu, here))) break;
+                tc_fence_after();
+                for (int at = 0; at < (EPI == kFfGated ? 2 : 1) * span; at += 16) {
+                    const bool up = EPI == kFfGated && at >= span;  // Wu's half
+                    const int in = up ? at - span : at;
+                    uint32_t r[16];
+                    tmem_ld_32x32b_x16(lane_base + (n & 1) * 256 + (up ? w.width / 2 : 0) + begin + in,
+                                       r);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float& h = held[(up ? 64 : 0) + in + e];
+                        h = k0 == w.kb0 ? __uint_as_float(r[e]) : h + __uint_as_float(r[e]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(n & 1 ? leader_empty1 : leader_empty0);
+            }
+            if (lost) break;
             const int buf = n & 1;
             const bool got = mbar_wait_bounded(&acc_full[buf], (n >> 1) & 1, args.status,
                                                kErrFfEpilogue);
@@ -336,13 +381,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 uint8_t* mine32 = turn + lane * kPitch<float>;
                 uint8_t* mine16 = turn + lane * kPitch<T>;
                 auto f = [](uint32_t x) { return __uint_as_float(x); };
+                const int own = c0 - begin;  // of the columns in `held`
                 // 32 columns of D from `from` on, as they are, to an f32 matrix
-                auto put32 = [&](uint32_t from, float* to, int64_t ld, int width, bool vec) {
+                auto put32 = [&](uint32_t from, int at, float* to, int64_t ld, int width, bool vec) {
                     __syncwarp();
 #pragma unroll 1
                     for (int i = 0; i < 32; i += 16) {
                         uint32_t r[16];
                         tmem_ld_32x32b_x16(from + i, r);
+                        add_held(r, at + i);
 #pragma unroll
                         for (int e = 0; e < 16; e += 4)
                             *reinterpret_cast<uint4*>(mine32 + (i + e) * 4) =
@@ -355,13 +402,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     float* part = static_cast<float*>(p.c) + w.part * p.plane + at;
 #pragma unroll 1
                     for (int h = 0; h < 64; h += 32)
-                        put32(d + c0 + h, part + h, p.ldc, cols - h, true);
+                        put32(d + c0 + h, own + h, part + h, p.ldc, cols - h, true);
                 } else if (EPI == kFfStore) {
                     __syncwarp();
 #pragma unroll 1
                     for (int i = 0; i < 64; i += 16) {
                         uint32_t r[16];
                         tmem_ld_32x32b_x16(d + c0 + i, r);
+                        add_held(r, own + i);
                         uint32_t o[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[e] = pair16<T>(f(r[2 * e]), f(r[2 * e + 1]));
@@ -378,14 +426,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (p.pre_g) {
 #pragma unroll 1
                         for (int which = 0; which < 2; ++which)
-                            put32(which ? u0 : d + c0, (which ? p.pre_u : p.pre_g) + pre, p.N, cols,
-                                  p.vec_pre);
+                            put32(which ? u0 : d + c0, which ? 64 + own : own,
+                                  (which ? p.pre_u : p.pre_g) + pre, p.N, cols, p.vec_pre);
                     }
                     __syncwarp();
 #pragma unroll 1
                     for (int i = 0; i < 32; i += 8) {
                         uint32_t g[8], x[8], o[4];
                         tmem_ld_32x32b_2x8(d + c0 + i, u0 + i, g, x);
+                        add_held(g, own + i);
+                        add_held(x, 64 + own + i);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             o[e] = pair16<T>(
@@ -407,6 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 32; i += 8) {
                         uint32_t r[8], o[12];
                         tmem_ld_32x32b_x8(d + c0 + i, r);
+                        add_held(r, own + i);
                         float g[8], x[8];
 #pragma unroll
                         for (int e = 0; e < 8; e += 4) {
@@ -474,13 +525,22 @@ int operand_map(CUtensorMap* map, uint32_t dtype, const FfOperand& o, int rows, 
     return encode_16bit_map(map, dtype, o.p, o.mn ? rows : sum, o.mn ? sum : rows, o.ld, kBox, kBox);
 }
 
+template <int EPI, int ACT, class T, bool LONG>
+int launch_runs(const PairArgs& args, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(ff_pair_kernel<EPI, ACT, T, LONG>, smem_bytes(EPI), done);
+    if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
+    return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T, LONG>, 2 * args.deal.pairs,
+                            kThreads, smem_bytes(EPI), s, args);
+}
 template <int EPI, int ACT, class T>
 int launch(const PairArgs& args, cudaStream_t s) {
-    static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(ff_pair_kernel<EPI, ACT, T>, smem_bytes(EPI), done);
-    if (e != cudaSuccess) return cuda_status(e, "gated_ff shared memory");
-    return launch_dependent("gated_ff", ff_pair_kernel<EPI, ACT, T>, 2 * args.deal.pairs,
-                            kThreads, smem_bytes(EPI), s, args);
+    for (int i = 0; i < args.count; ++i) {
+        const PairProblem& p = args.p[i];
+        if ((p.nkb[0] + p.nkb[1] + p.splits - 1) / p.splits > kRun)
+            return launch_runs<EPI, ACT, T, true>(args, s);
+    }
+    return launch_runs<EPI, ACT, T, false>(args, s);
 }
 
 template <class T>

@@ -1755,17 +1755,19 @@ extern "C" int zg_level1_adamw(zg_device* dev, uint32_t count, const zg_device_a
         }
         deferred = deferred && buffer_memory(dev, p.buffer) == ZG_MEMORY_GPU_ONLY;
     }
-    std::sort(written.begin(), written.end());
-    bool twice = std::adjacent_find(written.begin(), written.end()) != written.end();
-    for (uint32_t g : read) twice = twice || std::binary_search(written.begin(), written.end(), g);
-    if (twice) return set_error(ZG_ERR_DISPATCH, "%s: one buffer is bound twice", op);
     const float* scale = nullptr;
     if (norm_scale) {
         const uint32_t two = 2;
         void* p = nullptr;
         if ((rc = array_ptr(dev, norm_scale, ZG_DTYPE_F32, 1, &two, op, "norm_scale", &p))) return rc;
         scale = static_cast<const float*>(p) + 1;
+        // every block reads it while others write their elements
+        read.push_back(norm_scale->buffer.index);
     }
+    std::sort(written.begin(), written.end());
+    bool twice = std::adjacent_find(written.begin(), written.end()) != written.end();
+    for (uint32_t g : read) twice = twice || std::binary_search(written.begin(), written.end(), g);
+    if (twice) return set_error(ZG_ERR_DISPATCH, "%s: one buffer is bound twice", op);
     if ((rc = zg_adamw(params[0].dtype, grads[0].dtype, state == ZG_DTYPE_U8 ? 8 : 32, count,
                        t.data(), h, nullptr, nullptr, scale, dev->stream)))
         return rc;

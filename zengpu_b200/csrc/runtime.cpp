@@ -43,17 +43,17 @@ namespace zg {
 
 // ---- errors -------------------------------------------------------------------
 namespace {
-thread_local std::string g_last_error;
+thread_local char g_last_error[512];  // no allocation: errors of allocation end here too
 thread_local zg_error_detail g_detail{};
 }
 
 int set_error(int code, const char* fmt, ...) {
-    char buf[512];
+    char buf[sizeof(g_last_error)];  // an argument may be the last error's text
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    g_last_error = buf;
+    std::memcpy(g_last_error, buf, sizeof(buf));
     g_detail = zg_error_detail{};
     g_detail.status = code;
     g_detail.memory = ZG_MEMORY_GPU_ONLY;  // a CUDA allocation (zengpu-cuda/src/error.rs:18)
@@ -556,7 +556,7 @@ uint32_t buffer_memory(zg_device* dev, zg_handle h) {
 // 1. Device runtime
 // ======================================================================
 
-extern "C" const char* zg_last_error(void) { return g_last_error.c_str(); }
+extern "C" const char* zg_last_error(void) { return g_last_error; }
 extern "C" int zg_last_error_detail(zg_error_detail* out) {
     if (!out) return ZG_ERR_BACKEND;
     *out = g_detail;
@@ -921,8 +921,8 @@ extern "C" int zg_shader_create(zg_device* dev, uint32_t kind, const void* code,
         img = image.data();
     }
     if ((rc = cu_status(d.moduleLoadData(&s.module, img), "cuModuleLoadData")) != ZG_OK) {
-        if (rc == ZG_ERR_BACKEND) g_last_error = "cuda: PTX/module error: " + g_last_error;
-        return rc == ZG_ERR_BACKEND ? set_error(ZG_ERR_SHADER_COMPILE, "%s", g_last_error.c_str())
+        return rc == ZG_ERR_BACKEND ? set_error(ZG_ERR_SHADER_COMPILE,
+                                                "cuda: PTX/module error: %s", g_last_error)
                                     : rc;
     }
     *out = dev->shaders.insert(s);
@@ -993,7 +993,7 @@ extern "C" int zg_pipeline_create(zg_device* dev, zg_handle shader, const char* 
         (rc = cu_status(d.funcSetAttribute(p.fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
                                            static_cast<int>(dynamic_smem)),
                         "cuFuncSetAttribute")))
-        return set_error(ZG_ERR_PIPELINE_CREATION, "%s", g_last_error.c_str());
+        return set_error(ZG_ERR_PIPELINE_CREATION, "%s", g_last_error);
     *out = dev->pipelines.insert(p);
     return ZG_OK;
 }
@@ -1558,19 +1558,35 @@ int array_ptr(zg_device* dev, const zg_device_array* a, uint32_t dtype, uint32_t
     return ZG_OK;
 }
 
-// Output arrays of one call: given back to the pool if the call fails.
+// Output arrays of one call, at most four: given back to the pool unless the call keeps
+// them, however it ends.
 struct PoolOutputs {
     zg_pool* pool;
-    std::vector<zg_device_array*> got;
+    zg_device_array* got[4];
+    int count = 0;
+    explicit PoolOutputs(zg_pool* p) : pool(p) {}
+    PoolOutputs(const PoolOutputs&) = delete;
     int alloc(uint32_t rows, uint32_t cols, uint32_t dtype, zg_device_array* out) {
         const uint32_t shape[2] = {rows, cols};
         const int rc = zg_pool_alloc(pool, shape, 2, dtype, out);
-        if (rc == ZG_OK) got.push_back(out);
+        if (rc == ZG_OK) got[count++] = out;
         return rc;
     }
-    int fail(int rc) {
-        for (zg_device_array* a : got) zg_pool_free(pool, a);
-        return rc;
+    void keep() { count = 0; }
+    ~PoolOutputs() {
+        if (!count) return;
+        // the error that ends the call outlives what giving back may report
+        char text[sizeof(g_last_error)];
+        std::memcpy(text, g_last_error, sizeof(text));
+        const zg_error_detail detail = g_detail;
+        for (int i = 0; i < count; ++i) {
+            try {
+                zg_pool_free(pool, got[i]);
+            } catch (const std::exception&) {  // no memory for the pool's list: the array is lost
+            }
+        }
+        std::memcpy(g_last_error, text, sizeof(text));
+        g_detail = detail;
     }
 };
 
@@ -1614,7 +1630,7 @@ extern "C" int zg_gemm_gated_ff(const zg_gemm_kernel* k, zg_device* dev, zg_pool
                                 const zg_device_array* x, const zg_device_array* w_gate,
                                 const zg_device_array* w_up, const zg_device_array* w_down,
                                 zg_device_array* out, zg_device_array* pre_gate,
-                                zg_device_array* pre_up) {
+                                zg_device_array* pre_up) try {
     const char* op = "gated_ff";
     if (!k || !dev || !pool || !out || (pre_gate == nullptr) != (pre_up == nullptr))
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
@@ -1633,21 +1649,24 @@ extern "C" int zg_gemm_gated_ff(const zg_gemm_kernel* k, zg_device* dev, zg_pool
         return rc;
     const uint64_t ws = zg_gated_ff_workspace_bytes(s.dtype, k->mode, s.m, s.k, s.f, s.d, 0);
     if ((rc = ensure_workspace(dev, ws))) return rc;
-    PoolOutputs outs{pool, {}};
+    PoolOutputs outs(pool);
     if ((rc = outs.alloc(s.m, s.d, s.dtype, out)) ||
         (pre_gate && ((rc = outs.alloc(s.m, s.f, ZG_DTYPE_F32, pre_gate)) ||
                       (rc = outs.alloc(s.m, s.f, ZG_DTYPE_F32, pre_up)))) ||
         (rc = array_ptr(dev, out, s.dtype, 2, ys, op, "out", &py)) ||
         (pre_gate && ((rc = array_ptr(dev, pre_gate, ZG_DTYPE_F32, 2, ps, op, "pre_gate", &pre[0])) ||
                       (rc = array_ptr(dev, pre_up, ZG_DTYPE_F32, 2, ps, op, "pre_up", &pre[1])))))
-        return outs.fail(rc);
+        return rc;
     if ((rc = zg_gated_ff(s.dtype, k->mode, act, s.m, s.k, s.f, s.d, px, pg, pu, pd, py,
                           static_cast<float*>(pre[0]), static_cast<float*>(pre[1]), dev->workspace,
                           dev->workspace_bytes, dev->stream))) {
         cudaStreamSynchronize(dev->stream);
-        return outs.fail(rc);
+        return rc;
     }
+    outs.keep();
     return finish_op(dev, pool->memory == ZG_MEMORY_GPU_ONLY);
+} catch (const std::exception& e) {  // the host ran out of memory
+    return set_error(ZG_ERR_BACKEND, "gated_ff: %s", e.what());
 }
 
 extern "C" int zg_gemm_gated_ff_backward(
@@ -1655,7 +1674,7 @@ extern "C" int zg_gemm_gated_ff_backward(
     const zg_device_array* x, const zg_device_array* w_gate, const zg_device_array* w_up,
     const zg_device_array* w_down, const zg_device_array* pre_gate, const zg_device_array* pre_up,
     zg_device_array* dx, zg_device_array* dw_gate, zg_device_array* dw_up,
-    zg_device_array* dw_down) {
+    zg_device_array* dw_down) try {
     const char* op = "gated_ff_backward";
     if (!k || !dev || !pool || !dx || !dw_gate || !dw_up || !dw_down)
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
@@ -1677,21 +1696,24 @@ extern "C" int zg_gemm_gated_ff_backward(
         return rc;
     const uint64_t ws = zg_gated_ff_workspace_bytes(s.dtype, k->mode, s.m, s.k, s.f, s.d, 1);
     if ((rc = ensure_workspace(dev, ws))) return rc;
-    PoolOutputs outs{pool, {}};
+    PoolOutputs outs(pool);
     zg_device_array* o[4] = {dx, dw_gate, dw_up, dw_down};
     const uint32_t* shapes[4] = {xs, gs, gs, ds};
     for (int i = 0; i < 4; ++i)
         if ((rc = outs.alloc(shapes[i][0], shapes[i][1], s.dtype, o[i])) ||
             (rc = array_ptr(dev, o[i], s.dtype, 2, shapes[i], op, "output", &po[i])))
-            return outs.fail(rc);
+            return rc;
     if ((rc = zg_gated_ff_backward(s.dtype, k->mode, act, s.m, s.k, s.f, s.d, pdy, px, pg, pu, pd,
                                    static_cast<float*>(pre[0]), static_cast<float*>(pre[1]), po[0],
                                    po[1], po[2], po[3], dev->workspace, dev->workspace_bytes,
                                    dev->stream))) {
         cudaStreamSynchronize(dev->stream);
-        return outs.fail(rc);
+        return rc;
     }
+    outs.keep();
     return finish_op(dev, pool->memory == ZG_MEMORY_GPU_ONLY);
+} catch (const std::exception& e) {  // the host ran out of memory
+    return set_error(ZG_ERR_BACKEND, "gated_ff_backward: %s", e.what());
 }
 
 extern "C" int zg_level1_adamw(zg_device* dev, uint32_t count, const zg_device_array* params,

@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import threading
 from typing import Sequence
 
 import torch
@@ -22,6 +23,11 @@ ADAMW_BLOCK = 256  # elements that share a scale in 8-bit moments (ZG_ADAMW_BLOC
 # One scratch tensor per (device, stream): GEMMs issued on different streams
 # may overlap, and each stream reuses its own scratch in stream order.
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+# A call queues several kernels that pass data through that scratch, and the interpreter
+# lets other threads run meanwhile: a second call on the same stream must not queue its
+# kernels between them.  (Reentrant: a finaliser may run a call of its own meanwhile.)
+_queueing = threading.RLock()
 
 
 def _stream(t: torch.Tensor) -> C.c_void_p:
@@ -120,12 +126,14 @@ def sgemm(a: torch.Tensor, b: torch.Tensor, mode: int = GemmMode.TF32X3, alpha: 
     out = torch.empty((m, n), dtype=torch.float32, device=a.device) if out is None else out
     _f32_cuda(out)
     need = workspace_bytes(mode, m, n, k)
-    ws = workspace if workspace is not None else workspace_for(a.device, need)
-    ws_ptr = ws.data_ptr() if ws is not None else None
-    ws_len = ws.numel() if ws is not None else 0
-    check(L.load().zg_sgemm_f32(int(mode), m, n, k, float(alpha), a.data_ptr(), b.data_ptr(),
-                                out.data_ptr(), bias.data_ptr() if bias is not None else None,
-                                1 if relu else 0, ws_ptr, ws_len, _stream(a)))
+    with _queueing:
+        ws = workspace if workspace is not None else workspace_for(a.device, need)
+        ws_ptr = ws.data_ptr() if ws is not None else None
+        ws_len = ws.numel() if ws is not None else 0
+        rc = L.load().zg_sgemm_f32(int(mode), m, n, k, float(alpha), a.data_ptr(), b.data_ptr(),
+                                   out.data_ptr(), bias.data_ptr() if bias is not None else None,
+                                   1 if relu else 0, ws_ptr, ws_len, _stream(a))
+    check(rc)
     return out
 
 
@@ -317,12 +325,14 @@ def _gated_ff(index, m, k, f, d, x, w_gate, w_up, w_down, act, mode, save, out):
              x.new_empty((m, f), dtype=torch.float32)) if save else None
     dt, stream, mode = _FLOATS[x.dtype].value, _raw_stream(index), int(mode)
     need = _ff_workspace_bytes(dt, mode, m, k, f, d, 0)
-    ws = _scratch(index, stream, need)
-    check(L.load().zg_gated_ff(
-        dt, mode, int(act), m, k, f, d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-        w_down.data_ptr(), y.data_ptr(), saved[0].data_ptr() if save else None,
-        saved[1].data_ptr() if save else None, ws.data_ptr() if ws is not None else None, need,
-        stream))
+    with _queueing:
+        ws = _scratch(index, stream, need)
+        rc = L.load().zg_gated_ff(
+            dt, mode, int(act), m, k, f, d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+            w_down.data_ptr(), y.data_ptr(), saved[0].data_ptr() if save else None,
+            saved[1].data_ptr() if save else None, ws.data_ptr() if ws is not None else None,
+            need, stream)
+    check(rc)
     return (y, saved) if save else y
 
 
@@ -352,11 +362,14 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
                _ff_output("dw_up", out[2], (k, f), x), _ff_output("dw_down", out[3], (f, d), x))
         dt, stream = _FLOATS[x.dtype].value, _raw_stream(index)
         need = _ff_workspace_bytes(dt, mode, m, k, f, d, 1)
-        ws = _scratch(index, stream, need)
-        check(L.load().zg_gated_ff_backward(
-            dt, mode, act, m, k, f, d, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
-            w_up.data_ptr(), w_down.data_ptr(), pre[0].data_ptr(), pre[1].data_ptr(),
-            *[t.data_ptr() for t in got], ws.data_ptr() if ws is not None else None, need, stream))
+        with _queueing:
+            ws = _scratch(index, stream, need)
+            rc = L.load().zg_gated_ff_backward(
+                dt, mode, act, m, k, f, d, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+                w_up.data_ptr(), w_down.data_ptr(), pre[0].data_ptr(), pre[1].data_ptr(),
+                *[t.data_ptr() for t in got], ws.data_ptr() if ws is not None else None, need,
+                stream)
+        check(rc)
     return got
 
 
@@ -490,8 +503,10 @@ class GradNorm:
         with _on(index):
             stream = _raw_stream(index)
             out = self.grads[0].new_empty(2, dtype=torch.float32)
-            ws = _scratch(index, stream, self._ws_bytes)
-            check(L.load().zg_grad_norm(self._type, len(self._sizes), self._ptrs, self._sizes,
-                                        max_norm, out.data_ptr(), ws.data_ptr(), self._ws_bytes,
-                                        stream))
+            with _queueing:
+                ws = _scratch(index, stream, self._ws_bytes)
+                rc = L.load().zg_grad_norm(self._type, len(self._sizes), self._ptrs, self._sizes,
+                                           max_norm, out.data_ptr(), ws.data_ptr(),
+                                           self._ws_bytes, stream)
+            check(rc)
         return out

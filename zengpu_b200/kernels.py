@@ -270,6 +270,19 @@ def _ff_output(name: str, t: torch.Tensor | None, shape: tuple[int, ...],
     return t
 
 
+def _apart(outs: dict[str, torch.Tensor | None], ins: dict[str, torch.Tensor]) -> None:
+    """Refuses given outputs that overlap an input, or each other: kernels read the one
+    while they write the other."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+    given = [(name, t, *span(t)) for name, t in outs.items() if t is not None and t.numel()]
+    others = given + [(name, t, *span(t)) for name, t in ins.items()]
+    for i, (name, t, a, b) in enumerate(given):
+        for other, o, c, d in others[i + 1:]:
+            if a < d and c < b and t.device == o.device:
+                raise ValueError(f"{name}: overlaps {other}")
+
+
 def _ff_sizes(x: torch.Tensor, w_gate: torch.Tensor, w_down: torch.Tensor) -> tuple[int, ...]:
     if not x.is_cuda or x.dtype not in _FLOATS:
         raise ValueError("gated_ff: expected f32, bf16 or f16 CUDA tensors")
@@ -305,9 +318,11 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: 
     and w_up [k, f], w_down [f, d] of one dtype: f32 (in `mode`, as sgemm), bf16 or
     f16 (f32 sums; the inner product is rounded once to the dtype).  save=True
     returns (y, saved), `saved` being what gated_ff_backward needs: the two inner
-    products before the activation, f32 [m, f] each."""
+    products before the activation, f32 [m, f] each.  `out` overlaps no input."""
     m, k, f, d = _ff_sizes(x, w_gate, w_down)
     index = x.get_device()
+    if out is not None:
+        _apart({"out": out}, {"x": x, "w_gate": w_gate, "w_up": w_up, "w_down": w_down})
     if not _ff_ready(index, x.dtype, ((x, (m, k)), (w_gate, (k, f)), (w_up, (k, f)),
                                       (w_down, (f, d)))):
         with _on(index):
@@ -343,13 +358,17 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor,
                       out: Sequence[torch.Tensor | None] = (None, None, None, None)):
     """(dx, dw_gate, dw_up, dw_down) of gated_ff for dy, the gradient of its y;
     `saved` as gated_ff(..., save=True) gave it for the same x and weights.  `out`
-    takes tensors to write them to."""
+    takes tensors to write them to, which overlap neither an input nor one another."""
     m, k, f, d = _ff_sizes(x, w_gate, w_down)
     index, act, mode = x.get_device(), int(act), int(mode)
     if len(saved) != 2 or any(t is None for t in saved):
         raise ValueError("gated_ff_backward: saved has two tensors")
     if len(out) != 4:
         raise ValueError("gated_ff_backward: out has four places")
+    if any(t is not None for t in out):
+        _apart(dict(zip(("dx", "dw_gate", "dw_up", "dw_down"), out)),
+               {"dy": dy, "x": x, "w_gate": w_gate, "w_up": w_up, "w_down": w_down,
+                "saved[0]": saved[0], "saved[1]": saved[1]})
     with _on(index):
         x = _ff_operand("x", x, (m, k), x)
         dy = _ff_operand("dy", dy, (m, d), x)

@@ -440,15 +440,17 @@ int zg_fill_normal_f32(float *x, uint64_t n, uint64_t seed, void *stream);
  *
  * x [m, k], w_gate and w_up [k, f], w_down [f, d], y and dy [m, d]; gradients have
  * their tensors' shapes.  All row-major and contiguous, of one dtype: F32, BF16
- * or F16, 16-byte aligned.  Sums are f32.  BF16 and F16 run on the tensor cores
- * as they are (mode is not read), whose f32 additions truncate: in runs of at most 16384
- * terms, which takes up to 1.1e-4 from a sum of terms of one sign, and rounded additions
- * between runs; h = act(x w_gate) * (x w_up), and in the
- * backward pass the gradients of the two products, are rounded once to the
- * dtype, as operands of the next product.  F32 runs in `mode` (ZG_GEMM_*): TF32X3
- * with sums that end within 1e-6 of float64 (relative Frobenius norm, two chained
- * products), the other tensor-core modes at sgemm's accuracy for each product,
- * SIMT_FP32 in plain f32; a forward pass of up to 32 rows is plain f32 in every mode.
+ * or F16, 16-byte aligned.  Sums are f32.
+ *     BF16 and F16 run on the tensor cores as they are (mode is not read), whose f32
+ * additions truncate: in runs of at most 16384 terms, which takes up to 1.1e-4 from a sum
+ * of terms of one sign, with rounded additions between runs.  h = act(x w_gate) *
+ * (x w_up), and in the backward pass the gradients of the two products, are rounded
+ * once to the dtype, as operands of the next product (an F16 value past 65504 becomes
+ * infinite there); activations are within 2^-14, relative, before that rounding.
+ *     F32 runs in `mode` (ZG_GEMM_*): TF32X3 with sums that end within 1.1e-6 of
+ * float64 (relative Frobenius norm, two chained products), the other tensor-core modes
+ * at sgemm's accuracy for each product, SIMT_FP32 in plain f32; a forward pass of up to
+ * 32 rows is plain f32 in every mode.
  *     pre_gate, pre_up: f32 [m, f], written by the forward pass when both are
  * given (x w_gate and x w_up before the activation), read by the backward pass.
  *     workspace: zg_gated_ff_workspace_bytes(...), 256-byte aligned, not shared by
@@ -478,7 +480,9 @@ int zg_gated_ff_backward(uint32_t dtype, int mode, int act, int m, int k, int f,
  * of them), in place:
  *     g' = s g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
  *     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
- * in f32, each operation rounded on its own.  Weights: F32, or BF16 / F16 with
+ * in f32, each operation rounded on its own; with state_bits 8 the moments, their codes
+ * and scales too, but the weight's change (the quotient) is within 2^-21 of itself, from
+ * approximate roots and reciprocals, unless eps < 1e-12 / sqrt(1 - b2).  Weights: F32, or BF16 / F16 with
  * an f32 `master` (the sum lives there, the weight is its rounding) or without
  * (master NULL: the sum is rounded to the weight's type).  Gradients: F32, BF16
  * or F16.  state_bits 32: exp_avg and exp_avg_sq are f32 of n elements (m and

@@ -171,8 +171,8 @@ int ff_f32_slope(int act, const float* g, const float* u, const float* dh, int m
 
 // The forward products for up to kFfRows rows of 16-bit tensors (gated_ff_rows.cu):
 // `gated` as kFfGated, else as kFfStore of one product, launched right behind the
-// gated one whose result it reads.  At 4096 x 12288 in bf16 64 rows take 77 us here
-// and 85 on the CTA pairs, 65 rows and more took 101 here.
+// gated one whose result it reads.  At 4096 x 12288 in bf16 64 rows take 65 us here
+// and 65 rows 93 on the CTA pairs (this form took 101 from 65 rows on).
 constexpr int kFfRows = 64;
 int ff_rows(uint32_t dtype, bool gated, int act, const FfProduct& product, cudaStream_t s);
 

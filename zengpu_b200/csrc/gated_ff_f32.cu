@@ -9,7 +9,7 @@
 // half a unit of the last place an addition, always downwards.  Here it stays for 48
 // of the sum, 18 additions (sgemm_tc.cu: 512, 192); sixteen epilogue warps then add
 // it to f32 registers, rounding to nearest, 64 columns a lane, while the MMAs fill
-// the other accumulator.  Two chained products so end within 1e-6 of float64, about
+// the other accumulator.  Two chained products so end within 1.1e-6 of float64, about
 // what plain f32 sums give.  A drain reads 128 KB of TMEM per SM, 2000 cycles and
 // more beside the MMAs, whose chunk takes 2500; with 32 of the sum a chunk the MMAs
 // would wait for it (a training pass 1.3 times as long).

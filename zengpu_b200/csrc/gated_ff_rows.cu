@@ -16,8 +16,9 @@
 // of weights for the gated pair, 16 KB for Wd) of up to 110 KB per CTA, two CTAs to
 // an SM.  y's kernel is launched while h's still runs (programmatic dependent
 // launch): it fills its ring with Wd, which nobody writes meanwhile, before it waits
-// for h.  One bf16 token, 4096 -> 12288: 53 us for 302 MB (5.7 TB/s); 48 f16 tokens 63
-// us, of which the cluster's exchange of 48 rows takes about 4 twice.
+// for h.  4096 -> 12288: one token 54 us for 302 MB (5.6 TB/s), 16 rows 57, 48 rows 64-67: what
+// grows is the cluster's exchange of the rows' partial sums, in both kernels, and past
+// 32 rows the gated ring holds two stages.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>

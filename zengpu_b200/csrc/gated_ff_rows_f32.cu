@@ -13,9 +13,12 @@
 // memory (two of them the eight rows' x, four of the sum at a time).  Partial results meet in shared memory, across the
 // cluster as in gated_ff_rows.cu, in a fixed order.
 //
-// Up to 16 rows the weights' 4 bytes each bound it; beyond, the f32 pipe (8 rows a
-// weight take 16 cycles of an SM's 128 lanes for 1 KB of weights, which HBM delivers
-// in 44).  One token, 4096 -> 12288: 128 us for 604 MB (4.7 TB/s); 32 tokens 439 us.
+// Up to 4 rows the weights' 4 bytes each bound it: 4096 -> 12288 takes 111 us for one token
+// (604 MB, 5.5 TB/s) and 125 for 4.  Beyond, 8 rows take 165, 16 rows 234 and 32 rows 362.
+// The f32 pipe is part of that (8 rows a weight are 16 cycles of an SM's 128 lanes for 1 KB
+// of weights, which HBM delivers in 44; 32 rows are 64 cycles, 135 us); the rest is
+// latency, a barrier of the CTA for every 32 of the sum, and unequal dealing: the split of
+// the sum is a power of two, so that h's 96 tiles are 192 CTAs on 148 SMs.
 // From 33 rows on the tensor cores are faster (2048 -> 6144: 217 us at 33 rows, 64 rows
 // here took 230).
 #include <algorithm>

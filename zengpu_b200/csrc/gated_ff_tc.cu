@@ -158,7 +158,7 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
 }
 
 // The reverse for f32, asynchronous: copies the block's rows into `turn`, zeros
-// outside the matrix.  Pieces as store_block's.
+// outside the matrix.  Pieces as flush_block's.
 __device__ __forceinline__ void fetch_block(const float* src, int64_t ld, int rows, int cols,
                                             bool vec, uint8_t* turn, int lane) {
     const uint32_t to = smem_u32(turn);

@@ -10,7 +10,10 @@
 //     p  = p (1 - lr wd) - ((lr / (1 - b1^t)) m) / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // in f32, every operation rounded on its own in the order written, as the
 // other elementwise kernels here do: the result does not depend on which
-// vector or scalar path an element takes, nor on the launch.  Weights are
+// vector or scalar path an element takes, nor on the launch.  (The one exception:
+// with 8-bit moments the last line's root and quotient are approximate instructions,
+// which change the weight's step by up to 2^-21 of itself; m, v and their codes are as
+// written.)  Weights are
 // f32, or bf16 / f16 either with an f32 master that carries the sum (the
 // 16-bit weight is its rounding) or without one (the sum itself is rounded).
 //

@@ -1558,6 +1558,13 @@ int array_ptr(zg_device* dev, const zg_device_array* a, uint32_t dtype, uint32_t
     return ZG_OK;
 }
 
+// A pool's arrays are buffers of its own device: on another one the same handle may name
+// a buffer in use.
+int own_pool(const zg_device* dev, const zg_pool* pool, const char* op) {
+    return pool->dev == dev ? ZG_OK
+                            : set_error(ZG_ERR_DISPATCH, "%s: the pool belongs to another device", op);
+}
+
 // Output arrays of one call, at most four: given back to the pool unless the call keeps
 // them, however it ends.
 struct PoolOutputs {
@@ -1636,7 +1643,7 @@ extern "C" int zg_gemm_gated_ff(const zg_gemm_kernel* k, zg_device* dev, zg_pool
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
     FfShapes s;
     int rc = ff_shapes(x, w_gate, w_down, op, &s);
-    if (rc) return rc;
+    if (rc || (rc = own_pool(dev, pool, op))) return rc;
     std::lock_guard<std::recursive_mutex> lk(dev->mu);
     if ((rc = set_device(dev))) return rc;
     void *px, *pg, *pu, *pd, *py, *pre[2] = {nullptr, nullptr};
@@ -1680,7 +1687,7 @@ extern "C" int zg_gemm_gated_ff_backward(
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
     FfShapes s;
     int rc = ff_shapes(x, w_gate, w_down, op, &s);
-    if (rc) return rc;
+    if (rc || (rc = own_pool(dev, pool, op))) return rc;
     std::lock_guard<std::recursive_mutex> lk(dev->mu);
     if ((rc = set_device(dev))) return rc;
     void *px, *pg, *pu, *pd, *pdy, *pre[2], *po[4];
@@ -1804,7 +1811,8 @@ extern "C" int zg_level1_grad_norm(zg_device* dev, zg_pool* pool, uint32_t count
     const char* op = "grad_norm";
     if (!dev || !pool || !out || (count && !grads))
         return set_error(ZG_ERR_DISPATCH, "%s: null argument", op);
-    int rc;
+    int rc = own_pool(dev, pool, op);
+    if (rc) return rc;
     std::lock_guard<std::recursive_mutex> lk(dev->mu);
     if ((rc = set_device(dev))) return rc;
     std::vector<const void*> ptrs(count);

@@ -98,7 +98,9 @@ __device__ __forceinline__ ActValue activate(float g) {
     const float k = 0.79788456080286536f;
     const float q = k * (g + 0.044715f * g * g * g);
     const float c = logistic<FAST>(2.0f * q);
-    return {g * c, c + g * 2.0f * c * (1.0f - c) * k * (1.0f + 3.0f * 0.044715f * g * g)};
+    // c (1 - c) is zero long before b differs from g; an infinite b^2 would make that NaN
+    const float b = fminf(fmaxf(g, -1e9f), 1e9f);
+    return {g * c, c + b * 2.0f * c * (1.0f - c) * k * (1.0f + 3.0f * 0.044715f * b * b)};
 }
 
 // One operand of a product over `k`: row r (of M or N), position i of the sum.

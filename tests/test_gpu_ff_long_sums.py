@@ -13,6 +13,10 @@ rms is eps / 2 / sqrt(3) for each result, so 2^-15 covers four deviations of the
 over 2000 results and more in f16, over 2^17 in bf16."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -118,3 +122,32 @@ def test_few_rows_with_many_hidden_units(f):
     want = sum(h[:, a:a + 8192] @ wd[a:a + 8192].double() for a in range(0, f, 8192))
     assert bias(y, want) <= BAR
     assert K.kernel_status() == 0
+
+
+FIRST = """
+import torch
+from zengpu_b200 import kernels as K
+x, wg, wu, wd, dy = (torch.rand(s, device="cuda").to(torch.bfloat16) * 0.01
+                     for s in ((130, 20008), (20008, 136), (20008, 136), (136, 20008), (130, 20008)))
+torch.cuda.synchronize()
+def run():
+    y, saved = K.gated_ff(x, wg, wu, wd, save=True)
+    return y, *saved, *K.gated_ff_backward(dy, x, wg, wu, wd, saved)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = run()
+for t in held:
+    t.zero_()
+for _ in range(3):
+    graph.replay()
+    run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, run())) and K.kernel_status() == 0
+"""
+
+
+def test_first_long_call_of_a_process_may_be_captured():
+    """Replays beside eager calls give their bits, the kernel's local memory included."""
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=Path(__file__).resolve().parents[1],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

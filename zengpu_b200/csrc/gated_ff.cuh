@@ -52,7 +52,7 @@ struct ActValue {
 };
 
 // FAST (16-bit tensors): __expf, whose error grows to 2^-16 relative where the result nears
-// 2^-126, and a polynomial for erfc, within 2^-18: together with the rounding of their
+// 2^-126, and a polynomial for erfc, within 2^-21: together with the rounding of their
 // arguments under 2^-14, an eighth of half an f16 step.  f32 tensors take expf, erfcf and
 // a true quotient.
 // (The correctly rounded reciprocal branches, and took 60 cycles a value one after the
@@ -75,18 +75,21 @@ __device__ __forceinline__ ActValue activate(float g) {
         return {g * s, s * (1.0f + g * (1.0f - s))};
     }
     if (ACT == ZG_ACT_GELU && FAST) {
-        // erfc(z) = (a1 t + ... + a6 t^6) e^(-z^2) for z >= 0, t = 1 / (1 + 0.4352 z), the form of
-        // Abramowitz and Stegun 7.1.26, whose coefficients keep the absolute error small (0.4 %
-        // of erfc at z = 4).  These are fitted (least squares, reweighted towards the largest
-        // deviation) to e^(z^2) erfc(z) from z = 0 to 9.6 in relative terms: within 3.8e-6.
-        // z = |g| / sqrt 2 makes the exponential the density's.
+        // erfc(z) = (a1 t + ... + a8 t^8) e^(-z^2) for z >= 0, t = 1 / (1 + 0.43 z), the form of
+        // Abramowitz and Stegun 7.1.26, whose five coefficients keep the absolute error small
+        // (0.4 % of erfc at z = 4).  These are fitted (least squares, reweighted towards the
+        // largest deviation) to e^(z^2) erfc(z) from z = 0 to 9.6 in relative terms: within
+        // 8.5e-8, and 4e-7 in f32 arithmetic.  z = |g| / sqrt 2 makes the exponential the
+        // density's.
         const float e = __expf(-0.5f * g * g);
-        const float t = rcp_fast(fmaf(0.43520227f * 0.70710678118654752f, fabsf(g), 1.0f));
-        float p = fmaf(-0.15149690f, t, 0.38239519f);
-        p = fmaf(p, t, 0.011472087f);
-        p = fmaf(p, t, 0.27432605f);
-        p = fmaf(p, t, 0.23724045f);
-        p = fmaf(p, t, 0.24605942f);
+        const float t = rcp_fast(fmaf(0.43f * 0.70710678118654752f, fabsf(g), 1.0f));
+        float p = fmaf(0.073669054f, t, -0.31021592f);
+        p = fmaf(p, t, 0.38344166f);
+        p = fmaf(p, t, -0.085488908f);
+        p = fmaf(p, t, 0.24672212f);
+        p = fmaf(p, t, 0.20498736f);
+        p = fmaf(p, t, 0.24436975f);
+        p = fmaf(p, t, 0.24251497f);
         const float tail = 0.5f * p * t * e;  // Phi(-|g|)
         const float c = g > 0.0f ? 1.0f - tail : tail;
         return {g * c, fmaf(g * 0.39894228040143268f, e, c)};

@@ -78,10 +78,15 @@ def workspace_bytes(mode: int, m: int, n: int, k: int) -> int:
 
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor | None:
     """Scratch tensor of the current stream on `device`, grown on demand
-    (reused in stream order, so only GEMMs on that stream share it)."""
+    (reused in stream order, so only GEMMs on that stream share it).  A capture gets
+    memory of its own, which no other graph or stream shares: its graph may be
+    replayed on any stream."""
     if nbytes == 0:
         return None
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    with _on(idx):
+        if torch._C._cuda_isCurrentStreamCapturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (idx, torch.cuda.current_stream(idx).cuda_stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -239,15 +244,13 @@ def _raw_stream(index: int) -> int:
 
 
 def _scratch(index: int, stream: int, nbytes: int) -> torch.Tensor | None:
-    """workspace_for of a device and stream known by number.  A capture gets memory
-    of its own, which no other graph or stream shares."""
+    """workspace_for of a device, the current one, and a stream known by number."""
     if nbytes == 0:
         return None
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
     ws = _workspaces.get((index, stream))
-    return ws if ws is not None and ws.numel() >= nbytes \
-        else workspace_for(torch.device("cuda", index), nbytes)
+    if ws is not None and ws.numel() >= nbytes and not torch._C._cuda_isCurrentStreamCapturing():
+        return ws
+    return workspace_for(torch.device("cuda", index), nbytes)
 
 
 def _ff_operand(name: str, t: torch.Tensor, shape: tuple[int, ...],
